@@ -133,6 +133,7 @@ def _declare(L):
         "xdna_attention_bf16": ([p, p, p, i64, p, p, p, i64, i64, i, i, ctypes.c_float, p, p], i),
         "xdna_silu_mul_bf16": ([p, i64, i64, p, p], i),
         "xdna_add_f32": ([p, p, i64, p], i),
+        "xdna_linear_w4": ([p, i, i64, p, p, i, p, p, i, p, i64, i64, i64, i64, p], i),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -150,7 +151,7 @@ EXPORTS = ("xdna_abi_version", "xdna_last_error", "xdna_device_info", "xdna_quan
            "xdna_nhwc_to_nchw_i8",
            "xdna_tile_set", "xdna_tile_get", "xdna_tile_plan", "xdna_tile_clear", "xdna_rmsnorm_bf16",
            "xdna_add_rmsnorm_bf16", "xdna_qk_norm_rope",
-           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32")
+           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4")
 
 
 def _check(status, what):
@@ -793,3 +794,32 @@ def add_(x, y):
         with _on(dev):
             _check(lib().xdna_add_f32(_ptr(x), _ptr(y), x.numel(), _stream(dev)), "add_f32")
     return x
+
+
+# ------------------------------------------------------------------------------ language model operators
+def _rows16(x2d):
+    """x2d with contiguous rows that start on 16 bytes: itself, or a copy with rows as wide as it takes."""
+    if x2d.stride(1) == 1 and x2d.data_ptr() % 16 == 0 and (x2d.stride(0) * x2d.element_size() % 16 == 0
+                                                            or x2d.shape[0] == 1):
+        return x2d
+    return x2d.contiguous()
+
+
+def linear_w4(x2d, qweight, scales, zeros, bias):
+    """y [R, N] of x2d [R, K] and 4-bit weights (lm.linear_w4 checks the arguments), in one launch."""
+    dev = _need_gpu(x2d, qweight, scales, zeros, bias)
+    R, K = x2d.shape
+    N = qweight.shape[0]
+    y = torch.empty((R, N), dtype=x2d.dtype, device=dev)
+    if R and N:
+        x2d = _rows16(x2d)                      # K % 32 == 0: a contiguous copy has rows of whole 16 bytes
+        if qweight.data_ptr() % 16:
+            raise ValueError("linear_w4: qweight must be 16-byte aligned")
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        with _on(dev):
+            _check(lib().xdna_linear_w4(_ptr(x2d), _DTYPE_CODE[x2d.dtype], x2d.stride(0) if R > 1 else K, _ptr(qweight),
+                                        _ptr(scales), _DTYPE_CODE[scales.dtype], _ptr(zeros), _ptr(bias),
+                                        _bias_code(bias), _ptr(y), R, N, K, K // scales.shape[1], _stream(dev)),
+                   "linear_w4")
+    return y

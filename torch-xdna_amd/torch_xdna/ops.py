@@ -1,7 +1,8 @@
 """xdna::linear / linear_cat / linear_i8 / conv3x3, the custom ops the backend puts in place of
 offloadable GEMMs and convs; xdna::conv3x3_fused and xdna::conv3x3_chain, the GPU forms of the conv
 composite and of a chain of them; and xdna::qwen3_stack, the fused transformer-stack op (its GPU
-implementation is stack.py).
+implementation is stack.py). xdna::linear_w4 and the ops after it are the language model operators of lm.py, which
+programs call themselves.
 
 The schemas, fake (meta) functions and the `cfg_id` indirection are those of the reference
 (torch_xdna/ops.py:14-89 in the reference), so graphs built for it run unchanged. To the rest of
@@ -14,7 +15,7 @@ from typing import Optional
 import torch
 import torch._dynamo
 
-from . import conv, runtime, stack
+from . import conv, lm, runtime, stack
 
 try:    # what custom_op registers for autograd (below)
     from torch._library.autograd import make_autograd_impl as _make_autograd_impl
@@ -133,6 +134,18 @@ def _(x, mask, stack_id, cfg_id):
     return x.new_empty((x.shape[0], x.shape[1], stack.out_features(stack_id)))
 
 
+@torch.library.custom_op("xdna::linear_w4", mutates_args=())
+def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+              bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """lm.linear_w4: a linear with 4-bit weights and group scales."""
+    return lm.linear_w4(x, qweight, scales, zeros, bias)
+
+
+@linear_w4.register_fake
+def _(x, qweight, scales, zeros=None, bias=None):
+    return x.new_empty(*x.shape[:-1], qweight.shape[0])
+
+
 # ------------------------------------------------------------------------------ GPU calls that need no autograd
 # custom_op's own route from the dispatcher to the function above passes through its autograd and backend wrappers in
 # Python, 9 us a call, as much as a small op's launches. A call whose tensors are ordinary GPU tensors, none of which
@@ -183,4 +196,5 @@ if hasattr(linear, "_opoverload"):
     _direct(conv3x3_fused, lambda x, w, b, relu, cid: conv.conv3x3_fused(_configs[cid], x, w, b, relu), _lib)
     _direct(conv3x3_chain, lambda x, ws, bs, relus, after, pools, cid: conv.conv3x3_chain(
         _configs[cid], cid, x, list(ws), list(bs), list(relus), list(after), list(pools)), _lib)
+    _direct(linear_w4, lm.linear_w4, _lib)
     _direct(qwen3_stack, lambda x, mask, sid, cid: stack.run(_configs[cid], sid, x, mask), _lib)
