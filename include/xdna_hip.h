@@ -368,6 +368,38 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* qweight,
                    const void* zeros, const void* bias, int bias_dtype, void* y, int64_t m, int64_t n, int64_t k,
                    int64_t group, void* stream);
 
+/* Causal attention of packed prompts, bfloat16 or float16 (dtype), float32 sums: out [T, nh, d] (contiguous), token t of q
+ * head h = softmax over the tokens start(t) .. t of (q . k * scale), times v, of kv head h / (nh / nkv). starts [nseq + 1]:
+ * the first token of each sequence, ascending, and T; start(t) is the largest of them that is not above t (0 if
+ * none is), so that no value of them reads out of range. d a multiple of 8, at most 128. strides (elements, multiples of
+ * 8, below 2^24): {q token, q head, k token, k head, v token, v head}. Pointers 16-byte aligned. Rows whose scores are all
+ * -inf are zero. No counterpart in the reference. */
+int xdna_attention_causal(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                          const int32_t* starts, int64_t nseq, int64_t T, int nh, int nkv, int d, float scale, void* out,
+                          void* stream);
+
+/* One decode step's attention of B sequences that share a prefix: out [B, nh, d], sequence b's row over the P keys of kp /
+ * vp and the first lens[b] (clamped to 0 .. S) of the S of kc / vc [b]. Types, d, scale, alignment and empty rows as in
+ * xdna_attention_causal; strides: {q sequence, q head, kp token, kp head, vp token, vp head, kc sequence, kc token,
+ * kc head, vc sequence, vc token, vc head}, those of sequences of any size. ws: xdna_attention_prefix_ws_bytes(..) bytes
+ * (0: none needed) that the call may overwrite, 16-byte aligned. No counterpart in the reference. */
+int64_t xdna_attention_prefix_ws_bytes(int64_t P, int64_t S, int64_t B, int nh, int nkv, int d);
+int xdna_attention_prefix(const void* q, const void* kp, const void* vp, const void* kc, const void* vc, int dtype,
+                          const int64_t* strides, const int32_t* lens, int64_t P, int64_t S, int64_t B, int nh, int nkv,
+                          int d, float scale, void* out, void* ws, int64_t ws_bytes, void* stream);
+
+/* Logits before a token is chosen, y [B, V] (contiguous, of dtype F32 / BF16 / F16), in float32 and rounded once: with n =
+ * how often token v is among the first lens[b] (clamped to 0 .. L) of tokens [b] (ids outside 0 .. V - 1 count nowhere),
+ *   x = logits[b][v];  if n: x = x > 0 ? x / repetition[b] : x * repetition[b];
+ *   x -= frequency[b] * n + presence[b] * (n > 0), one after the other;  x += bias[b][v];  y = allowed bit ? x : -inf.
+ * tokens int32 or int64 (wide = 1). Any of tokens (with lens), repetition, presence, frequency, bias and allowed may be NULL:
+ * no history, 1, 0, 0, 0, all. ld: elements from row to row; ldb 0: one bias for all rows; allowed: 32 tokens a
+ * word, the lowest bit first, lda words from row to row. No counterpart in the reference. */
+int xdna_logits_adjust(const void* logits, int dtype, int64_t ld, const void* tokens, int wide, int64_t ldt, int64_t L,
+                       const int32_t* lens, const float* repetition, const float* presence, const float* frequency,
+                       const float* bias, int64_t ldb, const int32_t* allowed, int64_t lda, void* y, int64_t B, int64_t V,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,685 @@
+// Attention of a language model that serves prompts and their continuations, for gfx950 (MI355X), bfloat16 and float16:
+//
+//   attention_causal   packed prompts: token t of q head h sees the tokens start(t) .. t of its sequence
+//   attention_prefix   one new token of every sequence: it sees a prefix that the batch shares, held once, and
+//                      its sequence's own keys
+//
+//   out = sum over seen keys j of p_j v_j / sum of p_j,   p_j = 2^(c (s_j - m)),  s_j = q . k_j,  c = scale log2 e
+//
+// with m the running maximum of s (one pass over the keys; sums and outputs rescaled when it grows), float32
+// throughout except for p, which is rounded to the inputs' type for its product with V on the matrix units. A row that
+// sees nothing, or only scores of -inf, is zero.
+//
+// A wave has 32 rows: rows of a kv head are the pairs (token, q head of its group), so the heads that share K and V
+// share their loads. MFMA 32x32x16 (srcA = X, srcB = Y) gives lane l row l % 32 of Y and, in element 4 g + r, row
+// 8 g + 4 (l / 32) + r of X; lane l supplies values 8 (l / 32) .. + 7 of the 16-deep step of its operand's row l % 32.
+// S = K Q^T leaves in a lane 16 of 32 keys of its row, and these are, 8 at a time, what O^T = V^T P^T takes from that
+// lane if step u's k slot 8 h + i stands for key 16 u + 8 (i / 4) + 4 h + i % 4. V keeps its rows of one key each: the transposed
+// LDS read (16 lanes, 4 rows of 16 values: lane i gets column i) makes the V^T fragments in that order.
+//
+// Tiles of KT keys come into LDS by the DMA form of the buffer load, whose bounds check fills keys past the end, and
+// dims past the head's, with zeros. A 16-byte chunk's place in its row is XORed with the row so that the lanes that
+// read together cover the banks: K by the row (a fragment read takes one chunk of 16 rows), V by 64 bytes (a
+// transposed read takes 64 bytes of 4 rows).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "xdna_common.h"
+#include "xdna_hip.h"
+
+namespace xdna {
+namespace {
+
+typedef float f32x16a __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8a __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8a __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2a __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void* lds_void;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+template <int DT>
+__device__ __forceinline__ f32x16a mfma32(const i32x4& a, const i32x4& b, const f32x16a& c) {
+  if constexpr (DT == XDNA_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8a, a), __builtin_bit_cast(f16x8a, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8a, a), __builtin_bit_cast(bf16x8a, b), c, 0, 0,
+                                                   0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == XDNA_F16) return f32x2_to_f16x2_bits(lo, hi);
+  else return f32x2_to_bf16x2_bits(lo, hi);
+}
+
+// the larger of a lane's value and that of lane l ^ 32 (NaN if one is), and their sum
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// float16 p are held 2^14 times as large (the sum of p too, so it cancels): p down to 2^-28 of the largest stay normal
+// numbers, which a sum over 10^5 keys needs; bfloat16 has float32's range.
+template <int DT>
+constexpr float P_BIAS = DT == XDNA_F16 ? 14.0f : 0.0f;
+template <int DT>
+constexpr uint32_t EXP_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
+
+// The keys of a workgroup: up to two runs of consecutive keys, one tile after another (no tile holds keys of both).
+struct Keys {
+  const char *k, *v;          // first key of the run
+  const char *k2, *v2;
+  int64_t kp, vp, kp2, vp2;   // bytes from key to key
+  int n, n2;
+};
+
+// What a lane's row sees (keys lo .. hi of the run), and what holds for all rows of its wave, where that is known: keys
+// below first or above last are seen by no row, keys from_all .. to_all by every row. Used where CAUSAL; else
+// every row sees every key.
+struct Seen {
+  int lo, hi, first, last, from_all, to_all;
+};
+
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return D == 128 ? row & 15 : (row >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+  return D == 128 ? row & 3 : (row >> 1) & 1;
+}
+
+// LDS bytes of a workgroup: K and V of ST tiles of KT keys for each of KW groups of waves
+template <int D, int KW, int KT, int ST>
+constexpr int LDS_BYTES = KW * ST * 2 * KT * 2 * D;
+
+// Attention of QW x KW waves: wave w has the 32 rows w % QW (fragments qf, in the MFMA's order) and the tiles
+// kg, kg + KW, ... of group kg = w / QW; the groups meet in LDS. ST == 2: tile t + 1 loads while t is used, one workgroup barrier a tile.
+// ST == 1 (QW == 1, a group's LDS is its wave's own): K of the next tile loads once S is done, V after the tile.
+// store(chunk, o, m, l) receives dims 8 (chunk % 4) + 32 (chunk / 4) + 4 (lane / 32) .. + 3 of the lane's row: the sum
+// of p v, the maximum and the sum of p.
+template <int DT, int D, int QW, int KW, int KT, int ST, bool CAUSAL, class Store>
+__device__ __forceinline__ void attend(int8_t* lds_all, float* ml, const Keys& ks, int d, const i32x4 (&qf)[D / 16],
+                                       const Seen& seen, float c, Store&& store) {
+  static_assert(ST == 2 || (QW == 1 && KT == 32), "a single stage is one wave's own and one block of keys");
+  constexpr int RB = 2 * D, KB = KT * RB, STAGE = 2 * KB, NB = KT / 32, DB = D / 32;
+  constexpr int CH = D / 8, RPL = 64 / CH;    // 16-byte chunks of a row, rows of one 1 KB load
+  constexpr int NI = KB / 1024 / QW;          // 1 KB loads of K, and of V, per wave and tile
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / QW, qw = wave - kg * QW;
+  int8_t* const lds = lds_all + kg * (ST * STAGE);
+  // this lane's share of load j: row lrow + j * RPL of the tile, chunk lane % CH of its LDS row
+  int lrow[NI];
+  uint32_t kc[NI], vc[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    lrow[j] = (qw * NI + j) * RPL + lane / CH;
+    kc[j] = (uint32_t)(((lane % CH) ^ k_swizzle<D>(lrow[j])) * 16);
+    vc[j] = (uint32_t)(((lane % CH) ^ (v_swizzle<D>(lrow[j]) * 4)) * 16);
+  }
+  const int t1 = (int)cdiv(ks.n, KT), tiles = t1 + (int)cdiv(ks.n2, KT), nt = (int)cdiv(tiles, KW);
+  auto load = [&](bool v, int tile, int8_t* dst) {
+    const bool two = tile >= t1;
+    const int k0 = (two ? tile - t1 : tile) * KT, left = (two ? ks.n2 : ks.n) - k0;
+    const int64_t pitch = v ? (two ? ks.vp2 : ks.vp) : (two ? ks.kp2 : ks.kp);
+    const char* base = (v ? (two ? ks.v2 : ks.v) : (two ? ks.k2 : ks.k)) + k0 * pitch;
+    const auto r = make_rsrc(base, left > 0 ? (uint32_t)(min(left, KT) - 1) * (uint32_t)pitch + 2u * d : 0u);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const uint32_t at = v ? vc[j] : kc[j];
+      const uint32_t off = at < 2u * d ? (uint32_t)lrow[j] * (uint32_t)pitch + at : OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void)(dst + ((qw * NI + j) << 10)), 16, (int)off, 0, 0, 0);
+    }
+  };
+  f32x16a o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x16a{};
+  float m = -INFINITY, l = 0.0f;
+  const int krd = row * RB, kx = k_swizzle<D>(row);
+  const int vkey = 4 * half + ((lane & 15) >> 2);      // of each 8 keys
+  const int vrd = vkey * RB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3), vx = v_swizzle<D>(vkey);
+  // the V^T fragment of step u and dims 32 db .. + 31 of a block of 32 keys
+  auto v_frag = [&](const int8_t* vb, int u, int db) {
+    const int8_t* at = vb + vrd + ((db ^ vx) << 6) + u * 16 * RB;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * RB));
+    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+    return i32x4{(int)x.x, (int)x.y, (int)y.x, (int)y.y};
+  };
+  if (kg < tiles) {
+    load(false, kg, lds);
+    load(true, kg, lds + KB);
+  }
+  for (int t = 0; t < nt; ++t) {
+    const int tile = t * KW + kg, next = tile + KW;
+    int8_t* const cur = lds + (ST == 2 ? (t & 1) * STAGE : 0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if constexpr (ST == 2) {
+      __builtin_amdgcn_s_barrier();          // tile t is whole; every wave is done with tile t - 1
+      __builtin_amdgcn_sched_barrier(0);
+      if (next < tiles) {
+        load(false, next, lds + ((t + 1) & 1) * STAGE);
+        load(true, next, lds + ((t + 1) & 1) * STAGE + KB);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (tile >= tiles) continue;             // uniform over the group, at its last tile
+    const int k0 = (tile >= t1 ? tile - t1 : tile) * KT, left = (tile >= t1 ? ks.n2 : ks.n) - k0;
+    if (CAUSAL && (k0 > seen.last || k0 + KT - 1 < seen.first)) {        // no row of this wave sees a key of the tile
+      if constexpr (ST == 1) {
+        if (next < tiles) {
+          load(false, next, cur);
+          load(true, next, cur + KB);
+        }
+      }
+      continue;
+    }
+    const bool part = CAUSAL ? (k0 < seen.from_all || k0 + KT - 1 > seen.to_all) : left < KT;   // uniform over the wave
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int8_t* const kb = cur + b * 32 * RB;
+      const int8_t* const vb = cur + KB + b * 32 * RB;
+      f32x16a sc = f32x16a{};
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        sc = mfma32<DT>(*reinterpret_cast<const i32x4*>(kb + krd + (((2 * s + half) ^ kx) << 4)), qf[s], sc);
+      if constexpr (ST == 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (next < tiles) load(false, next, cur);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      auto visible = [&](int e) {
+        const int key = k0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3);
+        return CAUSAL ? key >= seen.lo && key <= seen.hi : key - k0 < left;
+      };
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!visible(e)) sc[e] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2)
+        mx = __builtin_elementwise_maximum(mx, __builtin_elementwise_maximum(sc[e], sc[e + 1]));
+      mx = pair_max(mx);
+      const bool grow = mx > m;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float mn = grow ? mx : m;
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= alpha;
+        m = mn;
+      }
+      const float mc = (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
+      float p[16], ps[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc));     // unseen: 2^-inf, c > 0
+      }
+      i32x4 pf[2];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        ps[0] += p[e];
+        ps[1] += p[e + 1];
+        pf[e >> 3][(e & 7) >> 1] = (int)pack2<DT>(p[e], p[e + 1]);
+      }
+      l += ps[0] + ps[1];
+      bool odd = false;
+      if (CAUSAL && part) {
+        // A value of V that is not finite may belong to a key that some rows do not see: 0 times it would be NaN.
+        u16x2a big = {0, 0};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const i32x4 vf = v_frag(vb, u, db);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2a, (uint32_t)vf[e] & 0x7fff7fffu));
+          }
+        odd = __builtin_amdgcn_ballot_w64(big[0] >= EXP_ONES<DT> || big[1] >= EXP_ONES<DT>) != 0;
+      }
+      if (CAUSAL && odd) {
+        // its finite values by the matrix units, the others one by one to the rows that see them
+        auto finite = [&](uint32_t w) {
+          if ((w & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffff0000u;
+          if ((w >> 16 & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffffu;
+          return (int)w;
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            i32x4 vf = v_frag(vb, u, db);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[e] = finite((uint32_t)vf[e]);
+            o[db] = mfma32<DT>(vf, pf[u], o[db]);
+          }
+#pragma unroll 1
+        for (int kk = 0; kk < 32; ++kk) {
+          const int want = 4 * (kk >> 3) + (kk & 3);
+          float pk = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk = e == want ? p[e] : pk;
+          pk = __shfl(pk, row + 32 * ((kk >> 2) & 1), 64);
+          const int key = k0 + 32 * b + kk;
+          const bool vis = key >= seen.lo && key <= seen.hi;
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const uint2 w = *reinterpret_cast<const uint2*>(vb + kk * RB + ((db ^ v_swizzle<D>(kk)) << 6) + 16 * g + 8 * half);
+              const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float v = DT == XDNA_F16 ? f16_bits_to_f32(h[r]) : bf16_bits_to_f32(h[r]);
+                if (vis && (h[r] & EXP_ONES<DT>) == EXP_ONES<DT>) o[db][4 * g + r] += pk * v;
+              }
+              asm volatile("" ::: "memory");      // one read at a time: this path is to take no registers from the others
+            }
+        }
+      } else {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db] = mfma32<DT>(v_frag(vb, u, db), pf[u], o[db]);
+        __builtin_amdgcn_s_setprio(0);
+      }
+    }
+    if constexpr (ST == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (next < tiles) load(true, next, cur + KB);
+    }
+  }
+  l = pair_sum(l);
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store(4 * db + g, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]}, m, l);
+  } else {
+    // each wave leaves its m, l and O; wave (kg, qw) then joins chunks kg, kg + KW, ... of the 32 rows of qw
+    constexpr int OB = 32 * D * 4;           // bytes of a wave's O
+    static_assert(QW * KW * OB <= LDS_BYTES<D, KW, KT, ST>, "the outputs meet where the tiles were");
+    __syncthreads();
+    ml[wave * 64 + lane] = m;
+    ml[(QW * KW + wave) * 64 + lane] = l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(lds_all + wave * OB + (db * 4 + g) * 1024 + lane * 16) =
+            f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    __syncthreads();
+    float mt = -INFINITY, lt = 0.0f, w[KW];
+#pragma unroll
+    for (int g = 0; g < KW; ++g) mt = fmaxf(mt, ml[(g * QW + qw) * 64 + lane]);
+#pragma unroll
+    for (int g = 0; g < KW; ++g) {
+      const float mg = ml[(g * QW + qw) * 64 + lane];
+      w[g] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mg - mt) * c);     // a group without keys: nothing
+      const float lg = ml[(QW * KW + g * QW + qw) * 64 + lane];
+      lt += mg == -INFINITY ? lg : lg * w[g];            // lg is 0 then, or NaN
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * DB / KW; ++i) {
+      const int chunk = kg + i * KW;
+      f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int g = 0; g < KW; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lds_all + (g * QW + qw) * OB + chunk * 1024 + lane * 16);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += x[r] * w[g];
+      }
+      store(chunk, v, mt, lt);
+    }
+  }
+}
+
+// A row's q in the MFMA's order, its sign bits flipped where the scale is negative, zeros past the head's dims.
+template <int D>
+__device__ __forceinline__ void load_q(i32x4 (&qf)[D / 16], const uint16_t* q, int half, int d, uint32_t sign) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    qf[s] = i32x4{0, 0, 0, 0};
+    if (16 * s + 8 * half < d) qf[s] = *reinterpret_cast<const i32x4*>(q + 16 * s + 8 * half);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qf[s][e] ^= (int)sign;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(uint16_t* p, const f32x4& v, float inv) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv));
+}
+
+// ------------------------------------------------------------------------------ packed prompts, causal
+// The first token of t's sequence: the largest of the starts that is not above t, 0 if none is. Whatever the starts
+// hold, the result lies in 0 .. t.
+__device__ __forceinline__ int seq_start(const int32_t* __restrict__ starts, int n, int t) {
+  int s = 0;
+  if (n <= 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int v = starts[min(i, n - 1)];
+      s = v <= t ? max(s, v) : s;
+    }
+  } else {
+    int lo = 0, hi = n;                     // starts[0 .. lo) <= t
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    s = lo ? starts[lo - 1] : 0;
+  }
+  return max(0, min(s, t));
+}
+
+struct CausalArgs {
+  const uint16_t *q, *k, *v;
+  int64_t qt, qh, kt, kh, vt, vh;           // elements from token to token and from head to head
+  const int32_t* starts;
+  int nstarts, T, nh, nkv, d;
+  float c;
+  uint32_t sign;
+  uint16_t* out;
+};
+
+// Tiles of 32 QW rows over all tokens, whatever sequences they fall into: a tile's keys run from the first token of
+// its first row's sequence to its last row's token, and each row's mask does the rest. Last tiles first: in
+// a long prompt they are the longest.
+template <int DT, int D, int QW, int KW, int KT, int ST>
+__global__ __launch_bounds__(QW* KW * 64, 2) void causal_kernel(CausalArgs a) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[LDS_BYTES<D, KW, KT, ST>];
+  __shared__ float ml[KW > 1 ? 2 * QW * KW * 64 : 1];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = a.nh / a.nkv, nrows = a.T * grp;
+  const int kvh = blockIdx.x % a.nkv, tile = gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv;
+  const int row0 = tile * (32 * QW), wrow0 = min(row0 + 32 * (wave % QW), nrows - 1);
+  const int tfirst = row0 / grp, tlast = (min(row0 + 32 * QW, nrows) - 1) / grp;
+  const int first = __builtin_amdgcn_readfirstlane(seq_start(a.starts, a.nstarts, tfirst));
+  const int last = __builtin_amdgcn_readfirstlane(seq_start(a.starts, a.nstarts, tlast));
+  const int idx = min(wrow0 + (lane & 31), nrows - 1);
+  const int tok = idx / grp, head = kvh * grp + idx - tok * grp;
+  const int lo = first == last ? first : seq_start(a.starts, a.nstarts, tok);
+  Seen seen;
+  seen.lo = lo - first;
+  seen.hi = tok - first;
+  seen.first = __builtin_amdgcn_readfirstlane(seen.lo);           // rows and their starts ascend with the lane
+  seen.to_all = __builtin_amdgcn_readfirstlane(seen.hi);
+  seen.from_all = __builtin_amdgcn_readlane(seen.lo, 31);
+  seen.last = __builtin_amdgcn_readlane(seen.hi, 31);
+  i32x4 qf[D / 16];
+  load_q<D>(qf, a.q + tok * a.qt + head * a.qh, half, a.d, a.sign);
+  Keys ks;
+  ks.k = reinterpret_cast<const char*>(a.k + first * a.kt + kvh * a.kh);
+  ks.v = reinterpret_cast<const char*>(a.v + first * a.vt + kvh * a.vh);
+  ks.kp = 2 * a.kt;
+  ks.vp = 2 * a.vt;
+  ks.n = tlast + 1 - first;
+  ks.k2 = ks.v2 = nullptr;
+  ks.kp2 = ks.vp2 = 0;
+  ks.n2 = 0;
+  const bool mine = row0 + 32 * (wave % QW) + (lane & 31) < nrows;
+  uint16_t* const orow = a.out + ((int64_t)tok * a.nh + head) * a.d;
+  attend<DT, D, QW, KW, KT, ST, true>(lds, ml, ks, a.d, qf, seen, a.c, [&](int chunk, const f32x4& o, float, float l) {
+    const int dim = 8 * chunk + 4 * half;
+    if (mine && dim < a.d) store4<DT>(orow + dim, o, l == 0.0f ? 0.0f : 1.0f / l);
+  });
+}
+
+template <int DT, int D>
+int causal_go(const CausalArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.T * (a.nh / a.nkv);
+  const bool wide = 4 * cdiv(rows, 128) * a.nkv >= 3 * (int64_t)device_cus();
+  const int64_t grid = cdiv(rows, wide ? 128 : 32) * a.nkv;
+  if (wide) causal_kernel<DT, D, 4, 1, 64, 2><<<(unsigned)grid, 256, 0, st>>>(a);
+  else causal_kernel<DT, D, 1, 4, 32, 1><<<(unsigned)grid, 256, 0, st>>>(a);
+  return launch_status("attention_causal");
+}
+
+// ------------------------------------------------------------------------------ a shared prefix and own keys
+struct PrefixArgs {
+  const uint16_t *q, *kp, *vp, *kc, *vc;
+  int64_t qb, qh, kpt, kph, vpt, vph, kcb, kct, kch, vcb, vct, vch;   // elements from sequence, token, head to the next
+  const int32_t* lens;
+  int P, S, B, nh, nkv, d;
+  int np, no;                 // parts of the prefix and of the own keys; 0 and 0: one workgroup for all keys of (sequence, kv head)
+  int pkeys, okeys;           // keys of a part
+  int rblocks;                // blocks of rows that the prefix's workgroups take
+  float c;
+  uint32_t sign;
+  float *po, *pml;            // [np + no][B * nh][d] sums, [np + no][B * nh][2] maxima and sums of p
+  uint16_t* out;
+};
+
+// Workgroups 0 .. nkv rblocks np - 1 take a part of the prefix for the rows (sequence, q head) of a kv head, 32 QW at a
+// time; the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a workgroup
+// takes all the keys of its (sequence, kv head) and writes the output itself.
+template <int DT, int D, int QW, int KW>
+__global__ __launch_bounds__(256, 2) void prefix_kernel(PrefixArgs a) {
+  constexpr int KT = KW == 1 ? 64 : 32, ST = QW == 1 ? 1 : 2;
+  __shared__ __attribute__((aligned(1024))) int8_t
+      lds[LDS_BYTES<D, KW, KT, ST> > LDS_BYTES<D, 4, 32, 1> ? LDS_BYTES<D, KW, KT, ST> : LDS_BYTES<D, 4, 32, 1>];
+  __shared__ float ml[2 * 4 * 64];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = a.nh / a.nkv;
+  const int kvh = blockIdx.x % a.nkv;
+  const int rest = blockIdx.x / a.nkv;
+  Keys ks;
+  ks.kp = 2 * a.kpt;
+  ks.vp = 2 * a.vpt;
+  ks.kp2 = ks.vp2 = 0;
+  ks.k2 = ks.v2 = nullptr;
+  ks.n2 = 0;
+  const Seen seen = {};
+  i32x4 qf[D / 16];
+  auto write = [&](int part, int64_t out_row, bool mine) {
+    return [=](int chunk, const f32x4& o, float m, float l) {
+      const int dim = 8 * chunk + 4 * half;
+      if (!mine || dim >= a.d) return;
+      if (part < 0) {
+        store4<DT>(a.out + out_row * a.d + dim, o, l == 0.0f ? 0.0f : 1.0f / l);
+      } else {
+        const int64_t at = (int64_t)part * a.B * a.nh + out_row;
+        *reinterpret_cast<f32x4*>(a.po + at * a.d + dim) = o;
+        if (dim == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = make_float2(m, l);
+      }
+    };
+  };
+  if (rest < a.rblocks * a.np) {
+    const int rb = rest % a.rblocks, part = rest / a.rblocks, nrows = a.B * grp;
+    const int want = rb * (32 * QW) + 32 * (wave % QW) + (lane & 31), idx = min(want, nrows - 1);
+    const int b = idx / grp, head = kvh * grp + idx - b * grp;
+    load_q<D>(qf, a.q + b * a.qb + head * a.qh, half, a.d, a.sign);
+    const int k0 = part * a.pkeys;
+    ks.k = reinterpret_cast<const char*>(a.kp + k0 * a.kpt + kvh * a.kph);
+    ks.v = reinterpret_cast<const char*>(a.vp + k0 * a.vpt + kvh * a.vph);
+    ks.n = max(0, min(a.pkeys, a.P - k0));
+    attend<DT, D, QW, KW, KT, ST, false>(lds, ml, ks, a.d, qf, seen, a.c,
+                                         write(part, (int64_t)b * a.nh + head, want < nrows));
+    return;
+  }
+  // rows: the q heads of one (sequence, kv head), 32 at a time
+  const int hb = (grp + 31) / 32, own = rest - a.rblocks * a.np, parts = max(1, a.no);
+  const int b = own / (hb * parts), at = own - b * (hb * parts), part = at / hb, want = (at - part * hb) * 32 + (lane & 31);
+  const int head = kvh * grp + min(want, grp - 1);
+  load_q<D>(qf, a.q + b * a.qb + head * a.qh, half, a.d, a.sign);
+  const int len = min(max(a.lens[b], 0), a.S);
+  const char* kc = reinterpret_cast<const char*>(a.kc + b * a.kcb + kvh * a.kch);
+  const char* vc = reinterpret_cast<const char*>(a.vc + b * a.vcb + kvh * a.vch);
+  const bool all = a.no == 0;
+  if (all) {
+    ks.k = reinterpret_cast<const char*>(a.kp + kvh * a.kph);
+    ks.v = reinterpret_cast<const char*>(a.vp + kvh * a.vph);
+    ks.n = a.P;
+    ks.k2 = kc;
+    ks.v2 = vc;
+    ks.kp2 = 2 * a.kct;
+    ks.vp2 = 2 * a.vct;
+    ks.n2 = len;
+  } else {
+    const int64_t k0 = (int64_t)part * a.okeys;
+    ks.k = kc + k0 * a.kct * 2;
+    ks.v = vc + k0 * a.vct * 2;
+    ks.kp = 2 * a.kct;
+    ks.vp = 2 * a.vct;
+    ks.n = (int)max<int64_t>(0, min<int64_t>(a.okeys, len - k0));
+  }
+  attend<DT, D, 1, 4, 32, 1, false>(lds, ml, ks, a.d, qf, seen, a.c,
+                                    write(all ? -1 : a.np + part, (int64_t)b * a.nh + head, want < grp));
+}
+
+// The parts of a row joined, in their order: a wave per row, lane l dims 2 l, 2 l + 1.
+template <int DT>
+__global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restrict__ po, const float* __restrict__ pml,
+                                                          int parts, int64_t rows, int d, float c,
+                                                          uint16_t* __restrict__ out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float mt = -INFINITY;
+  for (int i = lane; i < parts; i += 64) mt = fmaxf(mt, pml[(i * rows + row) * 2]);
+  mt = wave_max(mt);
+  float l = 0.0f, x = 0.0f, y = 0.0f;
+  const bool mine = 2 * lane < d;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float2 p = *reinterpret_cast<const float2*>(pml + (i * rows + row) * 2);
+    const float w = p.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((p.x - mt) * c);
+    l += p.x == -INFINITY ? p.y : p.y * w;
+    if (mine) {
+      const float2 v = *reinterpret_cast<const float2*>(po + (i * rows + row) * d + 2 * lane);
+      x += v.x * w;
+      y += v.y * w;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (mine) *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack2<DT>(x * inv, y * inv);
+}
+
+// How a call is split: two workgroups a CU where there are keys enough, no part under 256 keys (128 of a sequence's
+// own). One part of both and few keys: a workgroup for each (sequence, kv head), one launch.
+void prefix_plan(PrefixArgs& a) {
+  const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), want = 2 * device_cus();
+  const int64_t rows = a.B * grp;
+  a.rblocks = (int)cdiv(rows, rows <= 32 ? 32 : rows <= 64 ? 64 : 128);
+  if ((int64_t)a.P + a.S <= 1024) {
+    a.np = a.no = 0;
+    a.pkeys = a.okeys = 0;
+    return;
+  }
+  const int64_t np = std::max<int64_t>(1, std::min(want / (a.rblocks * a.nkv), cdiv(a.P, 256)));
+  const int64_t no = std::max<int64_t>(1, std::min(want / (a.B * hb * a.nkv), cdiv(a.S, 128)));
+  a.pkeys = (int)(cdiv(cdiv(a.P, np), 64) * 64);
+  a.okeys = (int)(cdiv(cdiv(a.S, no), 32) * 32);
+  a.np = a.P ? (int)cdiv(a.P, a.pkeys) : 0;
+  a.no = a.S ? (int)cdiv(a.S, a.okeys) : 1;
+}
+
+template <int DT, int D>
+int prefix_go(const PrefixArgs& a, hipStream_t st) {
+  const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), rows = a.B * grp;
+  const int64_t grid = (a.np * (int64_t)a.rblocks + a.B * hb * std::max(1, a.no)) * a.nkv;
+  if (rows <= 32 || a.np == 0) prefix_kernel<DT, D, 1, 4><<<(unsigned)grid, 256, 0, st>>>(a);
+  else if (rows <= 64) prefix_kernel<DT, D, 2, 2><<<(unsigned)grid, 256, 0, st>>>(a);
+  else prefix_kernel<DT, D, 4, 1><<<(unsigned)grid, 256, 0, st>>>(a);
+  if (a.np + a.no > 0)
+    prefix_join_kernel<DT><<<(unsigned)cdiv((int64_t)a.B * a.nh, 4), 256, 0, st>>>(
+        a.po, a.pml, a.np + a.no, (int64_t)a.B * a.nh, a.d, a.c, a.out);
+  return launch_status("attention_prefix");
+}
+
+// above 0, so that an unseen key's -inf stays one: scale 0 weighs all keys alike with it
+float scale_c(float scale) { return std::max(fabsf(scale) * 1.44269504088896340736f, 1.17549435e-38f); }
+
+// a stride in elements that keeps 16-byte alignment and whose offsets within a tile of 64 keys fit 31 bits
+bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (1ll << 24); }
+
+}  // namespace
+}  // namespace xdna
+
+using namespace xdna;
+
+extern "C" {
+
+int xdna_attention_causal(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                          const int32_t* starts, int64_t nseq, int64_t T, int nh, int nkv, int d, float scale, void* out,
+                          void* stream) {
+  XDNA_REQUIRE(dtype == XDNA_BF16 || dtype == XDNA_F16, "dtype must be BF16/F16");
+  XDNA_REQUIRE(T >= 0 && nseq >= 0 && nseq < (1ll << 30) && nh >= 1 && nkv >= 1 && nh % nkv == 0, "bad sizes");
+  XDNA_REQUIRE(d >= 8 && d <= 128 && d % 8 == 0, "head dims must be a multiple of 8, at most 128");
+  if (T == 0) return XDNA_OK;
+  XDNA_REQUIRE(q && k && v && strides && starts && out, "null pointer");
+  XDNA_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16), "operands must be 16-byte aligned");
+  for (int i = 0; i < 6; ++i) XDNA_REQUIRE(stride_ok(strides[i]), "strides must be multiples of 8 below 2^24");
+  XDNA_REQUIRE(strides[2] >= d && strides[4] >= d, "a token's keys and values must not overlap the next one's");
+  // 31-bit row numbers, and the launch's threads
+  XDNA_REQUIRE(T * (nh / nkv) < (1ll << 31) - 128 && cdiv(T * (nh / nkv), 128) * nkv <= MAX_LAUNCH_THREADS / 256, "too many tokens");
+  CausalArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+               strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], starts, (int)nseq + 1, (int)T, nh, nkv, d,
+               scale_c(scale), scale < 0.0f ? 0x80008000u : 0u, static_cast<uint16_t*>(out)};
+  if (dtype == XDNA_BF16) return d > 64 ? causal_go<XDNA_BF16, 128>(a, as_stream(stream)) : causal_go<XDNA_BF16, 64>(a, as_stream(stream));
+  return d > 64 ? causal_go<XDNA_F16, 128>(a, as_stream(stream)) : causal_go<XDNA_F16, 64>(a, as_stream(stream));
+}
+
+static bool prefix_sizes_ok(int64_t P, int64_t S, int64_t B, int nh, int nkv, int d) {
+  return P >= 0 && S >= 0 && B >= 0 && P < (1ll << 30) && S < (1ll << 30) && nh >= 1 && nkv >= 1 && nh % nkv == 0 &&
+         nh < (1 << 16) && B * nh < (1ll << 22) && d >= 8 && d <= 128 && d % 8 == 0;
+}
+
+int64_t xdna_attention_prefix_ws_bytes(int64_t P, int64_t S, int64_t B, int nh, int nkv, int d) {
+  XDNA_REQUIRE(prefix_sizes_ok(P, S, B, nh, nkv, d), "bad sizes");
+  if (B == 0) return 0;
+  PrefixArgs a{};
+  a.P = (int)P, a.S = (int)S, a.B = (int)B, a.nh = nh, a.nkv = nkv, a.d = d;
+  prefix_plan(a);
+  return (int64_t)(a.np + a.no) * B * nh * (d + 2) * 4;
+}
+
+int xdna_attention_prefix(const void* q, const void* kp, const void* vp, const void* kc, const void* vc, int dtype,
+                          const int64_t* strides, const int32_t* lens, int64_t P, int64_t S, int64_t B, int nh, int nkv,
+                          int d, float scale, void* out, void* ws, int64_t ws_bytes, void* stream) {
+  XDNA_REQUIRE(dtype == XDNA_BF16 || dtype == XDNA_F16, "dtype must be BF16/F16");
+  XDNA_REQUIRE(prefix_sizes_ok(P, S, B, nh, nkv, d), "bad sizes (head dims: a multiple of 8, at most 128)");
+  if (B == 0) return XDNA_OK;
+  XDNA_REQUIRE(q && strides && lens && out && (P == 0 || (kp && vp)) && (S == 0 || (kc && vc)), "null pointer");
+  XDNA_REQUIRE(aligned(q, 16) && aligned(kp, 16) && aligned(vp, 16) && aligned(kc, 16) && aligned(vc, 16) && aligned(out, 16),
+               "operands must be 16-byte aligned");
+  for (int i = 0; i < 12; ++i)
+    XDNA_REQUIRE(i == 0 || i == 6 || i == 9 ? strides[i] >= 0 && strides[i] % 8 == 0 : stride_ok(strides[i]),
+                 "strides must be multiples of 8, those of tokens and heads below 2^24");
+  XDNA_REQUIRE(strides[2] >= d && strides[4] >= d && strides[7] >= d && strides[10] >= d,
+               "a token's keys and values must not overlap the next one's");
+  PrefixArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kp), static_cast<const uint16_t*>(vp),
+               static_cast<const uint16_t*>(kc), static_cast<const uint16_t*>(vc), strides[0], strides[1], strides[2],
+               strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10], strides[11],
+               lens, (int)P, (int)S, (int)B, nh, nkv, d, 0, 0, 0, 0, 0, scale_c(scale), scale < 0.0f ? 0x80008000u : 0u,
+               nullptr, nullptr, static_cast<uint16_t*>(out)};
+  prefix_plan(a);
+  const int64_t rows = B * nh, need = (int64_t)(a.np + a.no) * rows * (d + 2) * 4;
+  XDNA_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need), "workspace too small or misaligned");
+  a.po = static_cast<float*>(ws);
+  a.pml = a.po + (int64_t)(a.np + a.no) * rows * d;
+  if (dtype == XDNA_BF16) return d > 64 ? prefix_go<XDNA_BF16, 128>(a, as_stream(stream)) : prefix_go<XDNA_BF16, 64>(a, as_stream(stream));
+  return d > 64 ? prefix_go<XDNA_F16, 128>(a, as_stream(stream)) : prefix_go<XDNA_F16, 64>(a, as_stream(stream));
+}
+
+}  // extern "C"

@@ -134,6 +134,10 @@ def _declare(L):
         "xdna_silu_mul_bf16": ([p, i64, i64, p, p], i),
         "xdna_add_f32": ([p, p, i64, p], i),
         "xdna_linear_w4": ([p, i, i64, p, p, i, p, p, i, p, i64, i64, i64, i64, p], i),
+        "xdna_attention_causal": ([p, p, p, i, p, p, i64, i64, i, i, i, ctypes.c_float, p, p], i),
+        "xdna_attention_prefix_ws_bytes": ([i64, i64, i64, i, i, i], i64),
+        "xdna_attention_prefix": ([p, p, p, p, p, i, p, p, i64, i64, i64, i, i, i, ctypes.c_float, p, p, i64, p], i),
+        "xdna_logits_adjust": ([p, i, i64, p, i, i64, i64, p, p, p, p, p, i64, p, i64, p, i64, i64, p], i),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -151,7 +155,8 @@ EXPORTS = ("xdna_abi_version", "xdna_last_error", "xdna_device_info", "xdna_quan
            "xdna_nhwc_to_nchw_i8",
            "xdna_tile_set", "xdna_tile_get", "xdna_tile_plan", "xdna_tile_clear", "xdna_rmsnorm_bf16",
            "xdna_add_rmsnorm_bf16", "xdna_qk_norm_rope",
-           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4")
+           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4", "xdna_attention_causal",
+           "xdna_attention_prefix_ws_bytes", "xdna_attention_prefix", "xdna_logits_adjust")
 
 
 def _check(status, what):
@@ -822,4 +827,97 @@ def linear_w4(x2d, qweight, scales, zeros, bias):
                                         _ptr(scales), _DTYPE_CODE[scales.dtype], _ptr(zeros), _ptr(bias),
                                         _bias_code(bias), _ptr(y), R, N, K, K // scales.shape[1], _stream(dev)),
                    "linear_w4")
+    return y
+
+
+def _heads(t):
+    """t [.., heads, d] as the attention launchers read it, and its strides but the last's: itself where its last dim is
+    dense, it starts on 16 bytes, no token's values overlap the next one's and its strides (of dims longer than 1) are
+    multiples of 8 that fit the kernels' offsets; else a copy."""
+    d = t.shape[-1]
+    for _ in range(2):
+        st = [d if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+        if ((t.stride(-1) == 1 or d == 1) and t.data_ptr() % 16 == 0 and not any(s % 8 for s in st)
+                and d <= st[-2] < 1 << 24 and st[-1] < 1 << 24):
+            break
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, st
+
+
+def attention_causal(q, k, v, starts, scale):
+    """Causal attention of packed prompts (lm.attention_causal checks the arguments), in one launch."""
+    dev = _need_gpu(q, k, v, starts)
+    T, nh, d = q.shape
+    out = torch.empty((T, nh, d), dtype=q.dtype, device=dev)
+    if T:
+        (q, sq), (k, sk), (v, sv) = _heads(q), _heads(k), _heads(v)
+        with _on(dev):
+            _check(lib().xdna_attention_causal(_ptr(q), _ptr(k), _ptr(v), _DTYPE_CODE[q.dtype], (ctypes.c_int64 * 6)(*sq, *sk, *sv),
+                                               _ptr(starts), starts.shape[0] - 1, T, nh, k.shape[1], d, float(scale),
+                                               _ptr(out), _stream(dev)), "attention_causal")
+    return out
+
+
+_prefix_ws = {}     # workspace bytes of the shapes that attention_prefix was called with
+
+
+def attention_prefix(q, kp, vp, kc, vc, lens, scale):
+    """A decode step's attention over a shared prefix and own keys (lm.attention_prefix checks the arguments), in one launch
+    or two. The workspace is a tensor of the call: torch's allocator keeps it apart per stream and graph."""
+    dev = _need_gpu(q, kp, vp, kc, vc, lens)
+    B, nh, d = q.shape
+    out = torch.empty((B, nh, d), dtype=q.dtype, device=dev)
+    if B:
+        P, S, nkv = kp.shape[0], kc.shape[1], kp.shape[1]
+        parts = [_heads(t) for t in (q, kp, vp, kc, vc)]
+        strides = (ctypes.c_int64 * 12)(*(s for _, st in parts for s in st))
+        with _on(dev):
+            key = (dev.index, P, S, B, nh, nkv, d)
+            need = _prefix_ws.get(key)
+            if need is None:
+                need = lib().xdna_attention_prefix_ws_bytes(P, S, B, nh, nkv, d)
+                if need < 0:
+                    _check(need, "attention_prefix")
+                if len(_prefix_ws) >= MAX_PLANS:
+                    _prefix_ws.clear()
+                _prefix_ws[key] = need
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _check(lib().xdna_attention_prefix(*(_ptr(t) for t, _ in parts), _DTYPE_CODE[q.dtype], strides, _ptr(lens), P, S,
+                                               B, nh, nkv, d, float(scale), _ptr(out), _ptr(ws), need, _stream(dev)),
+                   "attention_prefix")
+    return out
+
+
+def logits_adjust(logits, tokens, lens, repetition, presence, frequency, bias, allowed):
+    """Penalties, bias and mask on logits [B, V] (lm.logits_adjust checks the arguments), in one launch."""
+    dev = _need_gpu(logits, tokens, lens, repetition, presence, frequency, bias, allowed)
+    B, V = logits.shape
+    y = torch.empty((B, V), dtype=logits.dtype, device=dev)
+
+    def rows(t):        # dense rows
+        return t if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[-1])) \
+            else t.contiguous()
+
+    def flat(t):
+        return None if t is None else t.contiguous()
+
+    def ld(t):
+        return 0 if t is None else t.shape[-1] if t.shape[0] == 1 else t.stride(0)
+
+    if B and V:
+        logits, tokens, allowed = rows(logits), rows(tokens), rows(allowed)
+        lens, repetition, presence, frequency = flat(lens), flat(repetition), flat(presence), flat(frequency)
+        ldb = 0
+        if bias is not None:
+            if bias.dim() == 1 or bias.shape[0] == 1:
+                bias = bias.contiguous()
+            elif bias.stride(0) or (bias.stride(1) != 1 and V != 1):     # else one row, expanded
+                bias = rows(bias)
+                ldb = ld(bias)
+        with _on(dev):
+            _check(lib().xdna_logits_adjust(_ptr(logits), _DTYPE_CODE[logits.dtype], ld(logits), _ptr(tokens),
+                                            int(tokens is not None and tokens.dtype == torch.int64), ld(tokens),
+                                            0 if tokens is None else tokens.shape[1], _ptr(lens), _ptr(repetition),
+                                            _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(allowed), ld(allowed),
+                                            _ptr(y), B, V, _stream(dev)), "logits_adjust")
     return y

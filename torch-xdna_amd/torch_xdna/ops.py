@@ -146,6 +146,44 @@ def _(x, qweight, scales, zeros=None, bias=None):
     return x.new_empty(*x.shape[:-1], qweight.shape[0])
 
 
+@torch.library.custom_op("xdna::attention_causal", mutates_args=())
+def attention_causal(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """lm.attention_causal: causal attention of packed prompts."""
+    return lm.attention_causal(q, k, v, starts, scale)
+
+
+@attention_causal.register_fake
+def _(q, k, v, starts, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("xdna::attention_prefix", mutates_args=())
+def attention_prefix(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
+                     lens: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """lm.attention_prefix: a decode step's attention over a shared prefix and each sequence's own keys."""
+    return lm.attention_prefix(q, kp, vp, kc, vc, lens, scale)
+
+
+@attention_prefix.register_fake
+def _(q, kp, vp, kc, vc, lens, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("xdna::logits_adjust", mutates_args=())
+def logits_adjust(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                  repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                  frequency: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """lm.logits_adjust: penalties, a bias and a grammar's mask on logits."""
+    return lm.logits_adjust(logits, tokens, lens, repetition, presence, frequency, bias, allowed)
+
+
+@logits_adjust.register_fake
+def _(logits, tokens=None, lens=None, repetition=None, presence=None, frequency=None, bias=None, allowed=None):
+    return logits.new_empty(logits.shape)
+
+
 # ------------------------------------------------------------------------------ GPU calls that need no autograd
 # custom_op's own route from the dispatcher to the function above passes through its autograd and backend wrappers in
 # Python, 9 us a call, as much as a small op's launches. A call whose tensors are ordinary GPU tensors, none of which
@@ -197,4 +235,7 @@ if hasattr(linear, "_opoverload"):
     _direct(conv3x3_chain, lambda x, ws, bs, relus, after, pools, cid: conv.conv3x3_chain(
         _configs[cid], cid, x, list(ws), list(bs), list(relus), list(after), list(pools)), _lib)
     _direct(linear_w4, lm.linear_w4, _lib)
+    _direct(attention_causal, lm.attention_causal, _lib)
+    _direct(attention_prefix, lm.attention_prefix, _lib)
+    _direct(logits_adjust, lm.logits_adjust, _lib)
     _direct(qwen3_stack, lambda x, mask, sid, cid: stack.run(_configs[cid], sid, x, mask), _lib)
