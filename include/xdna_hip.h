@@ -368,6 +368,14 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* qweight,
                    const void* zeros, const void* bias, int bias_dtype, void* y, int64_t m, int64_t n, int64_t k,
                    int64_t group, void* stream);
 
+/* xdna_linear_w4 with a workspace of xdna_linear_w4_ws_bytes(..) bytes (0: none needed) that the call may overwrite, 16-byte
+ * aligned: calls of few columns and long K then split K over workgroups, in a fixed order of sums. A smaller one, or NULL,
+ * is valid and splits nothing. */
+int64_t xdna_linear_w4_ws_bytes(int x_dtype, int64_t m, int64_t n, int64_t k);
+int xdna_linear_w4_ws(const void* x, int x_dtype, int64_t ldx, const void* qweight, const void* scales, int s_dtype,
+                      const void* zeros, const void* bias, int bias_dtype, void* y, int64_t m, int64_t n, int64_t k,
+                      int64_t group, void* ws, int64_t ws_bytes, void* stream);
+
 /* Causal attention of packed prompts, bfloat16 or float16 (dtype), float32 sums: out [T, nh, d] (contiguous), token t of q
  * head h = softmax over the tokens start(t) .. t of (q . k * scale), times v, of kv head h / (nh / nkv). starts [nseq + 1]:
  * the first token of each sequence, ascending, and T; start(t) is the largest of them that is not above t (0 if

@@ -134,6 +134,8 @@ def _declare(L):
         "xdna_silu_mul_bf16": ([p, i64, i64, p, p], i),
         "xdna_add_f32": ([p, p, i64, p], i),
         "xdna_linear_w4": ([p, i, i64, p, p, i, p, p, i, p, i64, i64, i64, i64, p], i),
+        "xdna_linear_w4_ws_bytes": ([i, i64, i64, i64], i64),
+        "xdna_linear_w4_ws": ([p, i, i64, p, p, i, p, p, i, p, i64, i64, i64, i64, p, i64, p], i),
         "xdna_attention_causal": ([p, p, p, i, p, p, i64, i64, i, i, i, ctypes.c_float, p, p], i),
         "xdna_attention_prefix_ws_bytes": ([i64, i64, i64, i, i, i], i64),
         "xdna_attention_prefix": ([p, p, p, p, p, i, p, p, i64, i64, i64, i, i, i, ctypes.c_float, p, p, i64, p], i),
@@ -155,7 +157,7 @@ EXPORTS = ("xdna_abi_version", "xdna_last_error", "xdna_device_info", "xdna_quan
            "xdna_nhwc_to_nchw_i8",
            "xdna_tile_set", "xdna_tile_get", "xdna_tile_plan", "xdna_tile_clear", "xdna_rmsnorm_bf16",
            "xdna_add_rmsnorm_bf16", "xdna_qk_norm_rope",
-           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4", "xdna_attention_causal",
+           "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4", "xdna_linear_w4_ws_bytes", "xdna_linear_w4_ws", "xdna_attention_causal",
            "xdna_attention_prefix_ws_bytes", "xdna_attention_prefix", "xdna_logits_adjust")
 
 
@@ -810,8 +812,26 @@ def _rows16(x2d):
     return x2d.contiguous()
 
 
+_lm_need = {}
+
+
+def _lm_ws(name, dev, *sizes):
+    """Workspace bytes of an operator's call of these sizes on the current device. The workspace itself is a tensor of the
+    call: torch's allocator keeps it apart per stream and captured graph."""
+    key = (name, dev.index, sizes)
+    need = _lm_need.get(key)
+    if need is None:
+        need = getattr(lib(), f"xdna_{name}_ws_bytes")(*sizes)
+        if need < 0:
+            _check(need, name)
+        if len(_lm_need) >= MAX_PLANS:
+            _lm_need.clear()
+        _lm_need[key] = need
+    return need
+
+
 def linear_w4(x2d, qweight, scales, zeros, bias):
-    """y [R, N] of x2d [R, K] and 4-bit weights (lm.linear_w4 checks the arguments), in one launch."""
+    """y [R, N] of x2d [R, K] and 4-bit weights (lm.linear_w4 checks the arguments), in one launch or two."""
     dev = _need_gpu(x2d, qweight, scales, zeros, bias)
     R, K = x2d.shape
     N = qweight.shape[0]
@@ -823,10 +843,12 @@ def linear_w4(x2d, qweight, scales, zeros, bias):
         if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
         with _on(dev):
-            _check(lib().xdna_linear_w4(_ptr(x2d), _DTYPE_CODE[x2d.dtype], x2d.stride(0) if R > 1 else K, _ptr(qweight),
-                                        _ptr(scales), _DTYPE_CODE[scales.dtype], _ptr(zeros), _ptr(bias),
-                                        _bias_code(bias), _ptr(y), R, N, K, K // scales.shape[1], _stream(dev)),
-                   "linear_w4")
+            need = _lm_ws("linear_w4", dev, _DTYPE_CODE[x2d.dtype], R, N, K)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _check(lib().xdna_linear_w4_ws(_ptr(x2d), _DTYPE_CODE[x2d.dtype], x2d.stride(0) if R > 1 else K, _ptr(qweight),
+                                           _ptr(scales), _DTYPE_CODE[scales.dtype], _ptr(zeros), _ptr(bias),
+                                           _bias_code(bias), _ptr(y), R, N, K, K // scales.shape[1], _ptr(ws), need,
+                                           _stream(dev)), "linear_w4")
     return y
 
 
@@ -858,7 +880,6 @@ def attention_causal(q, k, v, starts, scale):
     return out
 
 
-_prefix_ws = {}     # workspace bytes of the shapes that attention_prefix was called with
 
 
 def attention_prefix(q, kp, vp, kc, vc, lens, scale):
@@ -872,15 +893,7 @@ def attention_prefix(q, kp, vp, kc, vc, lens, scale):
         parts = [_heads(t) for t in (q, kp, vp, kc, vc)]
         strides = (ctypes.c_int64 * 12)(*(s for _, st in parts for s in st))
         with _on(dev):
-            key = (dev.index, P, S, B, nh, nkv, d)
-            need = _prefix_ws.get(key)
-            if need is None:
-                need = lib().xdna_attention_prefix_ws_bytes(P, S, B, nh, nkv, d)
-                if need < 0:
-                    _check(need, "attention_prefix")
-                if len(_prefix_ws) >= MAX_PLANS:
-                    _prefix_ws.clear()
-                _prefix_ws[key] = need
+            need = _lm_ws("attention_prefix", dev, P, S, B, nh, nkv, d)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _check(lib().xdna_attention_prefix(*(_ptr(t) for t, _ in parts), _DTYPE_CODE[q.dtype], strides, _ptr(lens), P, S,
                                                B, nh, nkv, d, float(scale), _ptr(out), _ptr(ws), need, _stream(dev)),
