@@ -96,6 +96,74 @@ __device__ __forceinline__ int v_swizzle(int row) {
   return D == 128 ? row & 3 : (row >> 1) & 1;
 }
 
+// l + the two halves of w, as they are rounded
+template <int DT>
+__device__ __forceinline__ float dot_ones(uint32_t w, float l) {
+  if constexpr (DT == XDNA_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), (f16x2_t){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
+}
+
+// A value of V that is not finite may belong to a key that some rows do not see: 0 times it would be NaN. Whether a
+// block of 32 keys has one (uniform), frag(u, db) its fragments;
+template <int DT, int DB, class Frag>
+__device__ __forceinline__ bool not_finite(Frag&& frag) {
+  u16x2a big = {0, 0};
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const i32x4 vf = frag(u, db);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2a, (uint32_t)vf[e] & 0x7fff7fffu));
+    }
+  return __builtin_amdgcn_ballot_w64(big[0] >= EXP_ONES<DT> || big[1] >= EXP_ONES<DT>) != 0;
+}
+
+// and O += P V then: the finite values by the matrix units, the others one by one to the rows that see their key.
+template <int DT, int D, class Frag, class Visible>
+__device__ __forceinline__ void add_not_finite(f32x16a (&o)[D / 32], const float (&p)[16], const i32x4 (&pf)[2], const int8_t* vb,
+                                               Frag&& frag, Visible&& visible) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
+  auto finite = [&](uint32_t w) {
+    if ((w & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffff0000u;
+    if ((w >> 16 & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffffu;
+    return (int)w;
+  };
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      i32x4 vf = frag(u, db);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vf[e] = finite((uint32_t)vf[e]);
+      o[db] = mfma32<DT>(vf, pf[u], o[db]);
+    }
+#pragma unroll 1
+  for (int kk = 0; kk < 32; ++kk) {
+    const int want = 4 * (kk >> 3) + (kk & 3);
+    float pk = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) pk = e == want ? p[e] : pk;
+    pk = __shfl(pk, row + 32 * ((kk >> 2) & 1), 64);
+    const bool vis = visible(kk);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint2 w = *reinterpret_cast<const uint2*>(vb + kk * 2 * D + ((db ^ v_swizzle<D>(kk)) << 6) + 16 * g + 8 * half);
+        const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = DT == XDNA_F16 ? f16_bits_to_f32(h[r]) : bf16_bits_to_f32(h[r]);
+          if (vis && (h[r] & EXP_ONES<DT>) == EXP_ONES<DT>) o[db][4 * g + r] += pk * v;
+        }
+        asm volatile("" ::: "memory");      // one read at a time: this path is to take no registers from the others
+      }
+  }
+}
+
 // LDS bytes of a workgroup: K and V of ST tiles of KT keys for each of KW groups of waves
 template <int D, int KW, int KT, int ST>
 constexpr int LDS_BYTES = KW * ST * 2 * KT * 2 * D;
@@ -236,59 +304,12 @@ __device__ __forceinline__ void attend(int8_t* lds_all, float* ml, const Keys& k
       }
       l += ps[0] + ps[1];
       bool odd = false;
-      if (CAUSAL && part) {
-        // A value of V that is not finite may belong to a key that some rows do not see: 0 times it would be NaN.
-        u16x2a big = {0, 0};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const i32x4 vf = v_frag(vb, u, db);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2a, (uint32_t)vf[e] & 0x7fff7fffu));
-          }
-        odd = __builtin_amdgcn_ballot_w64(big[0] >= EXP_ONES<DT> || big[1] >= EXP_ONES<DT>) != 0;
-      }
+      if (CAUSAL && part) odd = not_finite<DT, DB>([&](int u, int db) { return v_frag(vb, u, db); });
       if (CAUSAL && odd) {
-        // its finite values by the matrix units, the others one by one to the rows that see them
-        auto finite = [&](uint32_t w) {
-          if ((w & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffff0000u;
-          if ((w >> 16 & EXP_ONES<DT>) == EXP_ONES<DT>) w &= 0xffffu;
-          return (int)w;
-        };
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            i32x4 vf = v_frag(vb, u, db);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vf[e] = finite((uint32_t)vf[e]);
-            o[db] = mfma32<DT>(vf, pf[u], o[db]);
-          }
-#pragma unroll 1
-        for (int kk = 0; kk < 32; ++kk) {
-          const int want = 4 * (kk >> 3) + (kk & 3);
-          float pk = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pk = e == want ? p[e] : pk;
-          pk = __shfl(pk, row + 32 * ((kk >> 2) & 1), 64);
+        add_not_finite<DT, D>(o, p, pf, vb, [&](int u, int db) { return v_frag(vb, u, db); }, [&](int kk) {
           const int key = k0 + 32 * b + kk;
-          const bool vis = key >= seen.lo && key <= seen.hi;
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint2 w = *reinterpret_cast<const uint2*>(vb + kk * RB + ((db ^ v_swizzle<D>(kk)) << 6) + 16 * g + 8 * half);
-              const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float v = DT == XDNA_F16 ? f16_bits_to_f32(h[r]) : bf16_bits_to_f32(h[r]);
-                if (vis && (h[r] & EXP_ONES<DT>) == EXP_ONES<DT>) o[db][4 * g + r] += pk * v;
-              }
-              asm volatile("" ::: "memory");      // one read at a time: this path is to take no registers from the others
-            }
-        }
+          return key >= seen.lo && key <= seen.hi;
+        });
       } else {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -350,6 +371,217 @@ __device__ __forceinline__ void attend(int8_t* lds_all, float* ml, const Keys& k
   }
 }
 
+// The same for four waves of 32 rows that share every tile of 64 keys: the form for many rows. K and V of two tiles have
+// an LDS array each, so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way while
+// tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
+// go by one copy of the masked one.
+template <int DT, int D, bool CAUSAL, class Store>
+__device__ __forceinline__ void attend_wide(int8_t* k0_, int8_t* v0_, int8_t* k1_, int8_t* v1_, const Keys& ks, int d,
+                                            const i32x4 (&qf)[D / 16], const Seen& seen, float c, Store&& store) {
+  constexpr int QW = 4, KT = 64, RB = 2 * D, KB = KT * RB, DB = D / 32;
+  constexpr int CH = D / 8, RPL = 64 / CH, NI = KB / 1024 / QW;
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (int)cdiv(ks.n, KT);
+  // this lane's share of load j: row (4 NI wave + j) RPL + lane / CH of the tile, chunk lane % CH of its LDS row. V's chunk
+  // is the same for every j (a multiple of 4 rows apart).
+  uint32_t ko[NI], vo[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int r = (wave * NI + j) * RPL + lane / CH;
+    const uint32_t kc = (uint32_t)(((lane % CH) ^ k_swizzle<D>(r)) * 16), vc = (uint32_t)(((lane % CH) ^ (v_swizzle<D>(r) * 4)) * 16);
+    ko[j] = kc < 2u * d ? (uint32_t)r * (uint32_t)ks.kp + kc : OOB;
+    vo[j] = vc < 2u * d ? (uint32_t)r * (uint32_t)ks.vp + vc : OOB;
+  }
+  auto load = [&](int tile, int8_t* kd, int8_t* vd) {
+    const int left = min(ks.n - tile * KT, KT) - 1;           // below 0: nothing is read
+    const auto kr = make_rsrc(ks.k + (int64_t)tile * KT * ks.kp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.kp + 2u * d);
+    const auto vr = make_rsrc(ks.v + (int64_t)tile * KT * ks.vp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.vp + 2u * d);
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void)(kd + ((wave * NI + j) << 10)), 16, (int)ko[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void)(vd + ((wave * NI + j) << 10)), 16, (int)vo[j], 0, 0, 0);
+  };
+  f32x16a o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x16a{};
+  float m = -INFINITY, l = 0.0f;
+  // offsets of the lane's K fragments in their block of 32 keys, and of its V fragments'; kept out of the compiler's sight, which
+  // would hold a set of them for each array
+  uint32_t koff[D / 16], voff[DB];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    koff[s] = row * RB + (((2 * s + half) ^ k_swizzle<D>(row)) << 4);
+    asm volatile("" : "+v"(koff[s]));
+  }
+  const int vkey = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    voff[db] = vkey * RB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + ((db ^ v_swizzle<D>(vkey)) << 6);
+    asm volatile("" : "+v"(voff[db]));
+  }
+  auto v_frag = [&](const int8_t* vb, int u, int db) {
+    const int8_t* at = vb + u * 16 * RB + voff[db];
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * RB));
+    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+    return i32x4{(int)x.x, (int)x.y, (int)y.x, (int)y.y};
+  };
+  auto scores = [&](const int8_t* kb) {
+    f32x16a sc = f32x16a{};
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      sc = mfma32<DT>(*reinterpret_cast<const i32x4*>(kb + koff[s]), qf[s], sc);
+    return sc;
+  };
+  // the running maximum follows that of the new scores; p of 16 scores, packed, and their sum
+  auto follow = [&](float mx) {
+    mx = pair_max(mx);
+    const bool grow = mx > m;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float mn = grow ? mx : m;
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      m = mn;
+    }
+    return (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
+  };
+  auto max16 = [&](const f32x16a& sc) {
+    float mx = sc[0];
+#pragma unroll
+    for (int e = 1; e < 15; e += 2)
+      mx = __builtin_elementwise_maximum(mx, __builtin_elementwise_maximum(sc[e], sc[e + 1]));
+    return __builtin_elementwise_maximum(mx, sc[15]);
+  };
+  auto weigh = [&](const f32x16a& sc, float mc, i32x4 (&pf)[2]) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const uint32_t w = pack2<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc)),
+                                   __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], c, -mc)));
+      pf[e >> 3][(e & 7) >> 1] = (int)w;
+      l = dot_ones<DT>(w, l);
+    }
+  };
+  // The reads of K run six ahead of their products, those of V's first half go out before the softmax and the second half's under
+  // the first half's products: with two waves a SIMD little else hides a trip to LDS.
+  auto tile_all = [&](const int8_t* kt, const int8_t* vt) {
+    f32x16a sc[2];
+    i32x4 pf[2][2], vf[2][2][DB];
+    auto read_v = [&](int b) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) vf[b][u][db] = v_frag(vt + b * 32 * RB, u, db);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    sc[0] = sc[1] = f32x16a{};
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        sc[b] = mfma32<DT>(*reinterpret_cast<const i32x4*>(kt + b * 32 * RB + koff[s]), qf[s], sc[b]);
+    read_v(0);
+    constexpr int AHEAD = 6, KF = D / 8;                      // K's fragments
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);    // LDS reads
+#pragma unroll
+    for (int i = 0; i < KF - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (4 * DB + AHEAD - 1) / AHEAD, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    const float mc = follow(__builtin_elementwise_maximum(max16(sc[0]), max16(sc[1])));
+    weigh(sc[0], mc, pf[0]);
+    weigh(sc[1], mc, pf[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(1);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = mfma32<DT>(vf[b][u][db], pf[b][u], o[db]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto tile_part = [&](const int8_t* kt, const int8_t* vt, int tile) {
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+      const int first = tile * KT + 32 * b;
+      const int8_t* const vb = vt + b * 32 * RB;
+      auto visible = [&](int key) { return CAUSAL ? key >= seen.lo && key <= seen.hi : key < ks.n; };
+      f32x16a sc = scores(kt + b * 32 * RB);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!visible(first + 8 * (e >> 2) + 4 * half + (e & 3))) sc[e] = -INFINITY;
+      const float mc = follow(max16(sc));
+      i32x4 pf[2];
+      weigh(sc, mc, pf);
+      bool odd = false;
+      if (CAUSAL) odd = not_finite<DT, DB>([&](int u, int db) { return v_frag(vb, u, db); });
+      if (CAUSAL && odd) {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc));
+        add_not_finite<DT, D>(o, p, pf, vb, [&](int u, int db) { return v_frag(vb, u, db); },
+                              [&](int k) { return visible(first + k); });
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db] = mfma32<DT>(v_frag(vb, u, db), pf[u], o[db]);
+      }
+    }
+  };
+  auto arrive = [&](int tile, int8_t* kn, int8_t* vn) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();            // the tile is whole; every wave is done with the one before
+    __builtin_amdgcn_sched_barrier(0);
+    load(tile + 1, kn, vn);                  // whether there is one or not: past a branch the compiler would wait for more
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto masked = [&](int from, int to) {
+#pragma unroll 1
+    for (int t = from; t < to; ++t) {
+      const bool odd = t & 1;
+      arrive(t, odd ? k0_ : k1_, odd ? v0_ : v1_);
+      const int k0 = t * KT;
+      if (CAUSAL && (k0 > seen.last || k0 + KT - 1 < seen.first)) continue;      // no row of this wave sees a key of it
+      tile_part(odd ? k1_ : k0_, odd ? v1_ : v0_, t);
+    }
+  };
+  // The tiles that every row of this wave sees whole are a run of them; its pairs of an even tile and the next take the short
+  // path. Waves may disagree on it: each passes one barrier a tile in any case.
+  const int all0 = CAUSAL ? (int)(cdiv(seen.from_all, 2 * KT) * 2) : 0;
+  const int all1 = max(all0, (CAUSAL ? (seen.to_all + 1) / (2 * KT) : ks.n / (2 * KT)) * 2);
+  if (tiles > 0) load(0, k0_, v0_);
+  masked(0, min(all0, tiles));
+  for (int t = all0; t < all1; t += 2) {
+    arrive(t, k1_, v1_);
+    tile_all(k0_, v0_);
+    arrive(t + 1, k0_, v0_);
+    tile_all(k1_, v1_);
+  }
+  masked(min(all1, tiles), tiles);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the load past the end: LDS may be another's soon
+  l = pair_sum(l);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      store(4 * db + g, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]}, m, l);
+}
+
 // A row's q in the MFMA's order, its sign bits flipped where the scale is negative, zeros past the head's dims.
 template <int D>
 __device__ __forceinline__ void load_q(i32x4 (&qf)[D / 16], const uint16_t* q, int half, int d, uint32_t sign) {
@@ -403,10 +635,10 @@ struct CausalArgs {
 // Tiles of 32 QW rows over all tokens, whatever sequences they fall into: a tile's keys run from the first token of
 // its first row's sequence to its last row's token, and each row's mask does the rest. Last tiles first: in
 // a long prompt they are the longest.
-template <int DT, int D, int QW, int KW, int KT, int ST>
-__global__ __launch_bounds__(QW* KW * 64, 2) void causal_kernel(CausalArgs a) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds[LDS_BYTES<D, KW, KT, ST>];
-  __shared__ float ml[KW > 1 ? 2 * QW * KW * 64 : 1];
+// WIDE: 128 rows by attend_wide, else 32 rows whose keys four waves share out.
+template <int DT, int D, bool WIDE>
+__global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
+  constexpr int QW = WIDE ? 4 : 1;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.nh / a.nkv, nrows = a.T * grp;
@@ -438,10 +670,21 @@ __global__ __launch_bounds__(QW* KW * 64, 2) void causal_kernel(CausalArgs a) {
   ks.n2 = 0;
   const bool mine = row0 + 32 * (wave % QW) + (lane & 31) < nrows;
   uint16_t* const orow = a.out + ((int64_t)tok * a.nh + head) * a.d;
-  attend<DT, D, QW, KW, KT, ST, true>(lds, ml, ks, a.d, qf, seen, a.c, [&](int chunk, const f32x4& o, float, float l) {
+  auto store = [&](int chunk, const f32x4& o, float, float l) {
     const int dim = 8 * chunk + 4 * half;
     if (mine && dim < a.d) store4<DT>(orow + dim, o, l == 0.0f ? 0.0f : 1.0f / l);
-  });
+  };
+  if constexpr (WIDE) {
+    __shared__ __attribute__((aligned(1024))) int8_t k0[128 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t v0[128 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t k1[128 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t v1[128 * D];
+    attend_wide<DT, D, true>(k0, v0, k1, v1, ks, a.d, qf, seen, a.c, store);
+  } else {
+    __shared__ __attribute__((aligned(1024))) int8_t lds[LDS_BYTES<D, 4, 32, 1>];
+    __shared__ float ml[2 * 4 * 64];
+    attend<DT, D, 1, 4, 32, 1, true>(lds, ml, ks, a.d, qf, seen, a.c, store);
+  }
 }
 
 template <int DT, int D>
@@ -449,8 +692,8 @@ int causal_go(const CausalArgs& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.T * (a.nh / a.nkv);
   const bool wide = 4 * cdiv(rows, 128) * a.nkv >= 3 * (int64_t)device_cus();
   const int64_t grid = cdiv(rows, wide ? 128 : 32) * a.nkv;
-  if (wide) causal_kernel<DT, D, 4, 1, 64, 2><<<(unsigned)grid, 256, 0, st>>>(a);
-  else causal_kernel<DT, D, 1, 4, 32, 1><<<(unsigned)grid, 256, 0, st>>>(a);
+  if (wide) causal_kernel<DT, D, true><<<(unsigned)grid, 256, 0, st>>>(a);
+  else causal_kernel<DT, D, false><<<(unsigned)grid, 256, 0, st>>>(a);
   return launch_status("attention_causal");
 }
 
