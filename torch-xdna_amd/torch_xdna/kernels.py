@@ -804,133 +804,33 @@ def add_(x, y):
 
 
 # ------------------------------------------------------------------------------ language model operators
-def _rows16(x2d):
-    """x2d with contiguous rows that start on 16 bytes: itself, or a copy with rows as wide as it takes."""
-    if x2d.stride(1) == 1 and x2d.data_ptr() % 16 == 0 and (x2d.stride(0) * x2d.element_size() % 16 == 0
-                                                            or x2d.shape[0] == 1):
-        return x2d
-    return x2d.contiguous()
+# torch.ops.xdna.linear_w4, attention_causal, attention_prefix and logits_adjust reach the library from C++ (csrc/
+# xdna_torch.cpp), registered for GPU tensors when it is loaded.
+TORCH_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libxdna_torch.so")
+_torch_lib = None
 
 
-_lm_need = {}
+def torch_lib():
+    """The library with the operators' GPU kernels, registered with torch's dispatcher; raises if it is not built."""
+    global _torch_lib
+    if _torch_lib is None:
+        with _lock:
+            if _torch_lib is None:
+                if not os.path.exists(TORCH_LIB_PATH):
+                    raise RuntimeError(f"operator library not built: {TORCH_LIB_PATH} (run `make -C torch-xdna_amd` or "
+                                       "__graft_entry__.build())")
+                lib()                                           # checks the ABI version first
+                torch.ops.load_library(TORCH_LIB_PATH)
+                L = ctypes.CDLL(TORCH_LIB_PATH)
+                L.xdna_torch_counts.argtypes, L.xdna_torch_counts.restype = [ctypes.c_void_p, ctypes.c_int], None
+                _torch_lib = L
+    return _torch_lib
 
 
-def _lm_ws(name, dev, *sizes):
-    """Workspace bytes of an operator's call of these sizes on the current device. The workspace itself is a tensor of the
-    call: torch's allocator keeps it apart per stream and captured graph."""
-    key = (name, dev.index, sizes)
-    need = _lm_need.get(key)
-    if need is None:
-        need = getattr(lib(), f"xdna_{name}_ws_bytes")(*sizes)
-        if need < 0:
-            _check(need, name)
-        if len(_lm_need) >= MAX_PLANS:
-            _lm_need.clear()
-        _lm_need[key] = need
-    return need
-
-
-def linear_w4(x2d, qweight, scales, zeros, bias):
-    """y [R, N] of x2d [R, K] and 4-bit weights (lm.linear_w4 checks the arguments), in one launch or two."""
-    dev = _need_gpu(x2d, qweight, scales, zeros, bias)
-    R, K = x2d.shape
-    N = qweight.shape[0]
-    y = torch.empty((R, N), dtype=x2d.dtype, device=dev)
-    if R and N:
-        x2d = _rows16(x2d)                      # K % 32 == 0: a contiguous copy has rows of whole 16 bytes
-        if qweight.data_ptr() % 16:
-            raise ValueError("linear_w4: qweight must be 16-byte aligned")
-        if bias is not None and not bias.is_contiguous():
-            bias = bias.contiguous()
-        with _on(dev):
-            need = _lm_ws("linear_w4", dev, _DTYPE_CODE[x2d.dtype], R, N, K)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _check(lib().xdna_linear_w4_ws(_ptr(x2d), _DTYPE_CODE[x2d.dtype], x2d.stride(0) if R > 1 else K, _ptr(qweight),
-                                           _ptr(scales), _DTYPE_CODE[scales.dtype], _ptr(zeros), _ptr(bias),
-                                           _bias_code(bias), _ptr(y), R, N, K, K // scales.shape[1], _ptr(ws), need,
-                                           _stream(dev)), "linear_w4")
-    return y
-
-
-def _heads(t):
-    """t [.., heads, d] as the attention launchers read it, and its strides but the last's: itself where its last dim is
-    dense, it starts on 16 bytes, no token's values overlap the next one's and its strides (of dims longer than 1) are
-    multiples of 8 that fit the kernels' offsets; else a copy."""
-    d = t.shape[-1]
-    for _ in range(2):
-        st = [d if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-        if ((t.stride(-1) == 1 or d == 1) and t.data_ptr() % 16 == 0 and not any(s % 8 for s in st)
-                and d <= st[-2] < 1 << 24 and st[-1] < 1 << 24):
-            break
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, st
-
-
-def attention_causal(q, k, v, starts, scale):
-    """Causal attention of packed prompts (lm.attention_causal checks the arguments), in one launch."""
-    dev = _need_gpu(q, k, v, starts)
-    T, nh, d = q.shape
-    out = torch.empty((T, nh, d), dtype=q.dtype, device=dev)
-    if T:
-        (q, sq), (k, sk), (v, sv) = _heads(q), _heads(k), _heads(v)
-        with _on(dev):
-            _check(lib().xdna_attention_causal(_ptr(q), _ptr(k), _ptr(v), _DTYPE_CODE[q.dtype], (ctypes.c_int64 * 6)(*sq, *sk, *sv),
-                                               _ptr(starts), starts.shape[0] - 1, T, nh, k.shape[1], d, float(scale),
-                                               _ptr(out), _stream(dev)), "attention_causal")
-    return out
-
-
-
-
-def attention_prefix(q, kp, vp, kc, vc, lens, scale):
-    """A decode step's attention over a shared prefix and own keys (lm.attention_prefix checks the arguments), in one launch
-    or two. The workspace is a tensor of the call: torch's allocator keeps it apart per stream and graph."""
-    dev = _need_gpu(q, kp, vp, kc, vc, lens)
-    B, nh, d = q.shape
-    out = torch.empty((B, nh, d), dtype=q.dtype, device=dev)
-    if B:
-        P, S, nkv = kp.shape[0], kc.shape[1], kp.shape[1]
-        parts = [_heads(t) for t in (q, kp, vp, kc, vc)]
-        strides = (ctypes.c_int64 * 12)(*(s for _, st in parts for s in st))
-        with _on(dev):
-            need = _lm_ws("attention_prefix", dev, P, S, B, nh, nkv, d)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _check(lib().xdna_attention_prefix(*(_ptr(t) for t, _ in parts), _DTYPE_CODE[q.dtype], strides, _ptr(lens), P, S,
-                                               B, nh, nkv, d, float(scale), _ptr(out), _ptr(ws), need, _stream(dev)),
-                   "attention_prefix")
-    return out
-
-
-def logits_adjust(logits, tokens, lens, repetition, presence, frequency, bias, allowed):
-    """Penalties, bias and mask on logits [B, V] (lm.logits_adjust checks the arguments), in one launch."""
-    dev = _need_gpu(logits, tokens, lens, repetition, presence, frequency, bias, allowed)
-    B, V = logits.shape
-    y = torch.empty((B, V), dtype=logits.dtype, device=dev)
-
-    def rows(t):        # dense rows
-        return t if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[-1])) \
-            else t.contiguous()
-
-    def flat(t):
-        return None if t is None else t.contiguous()
-
-    def ld(t):
-        return 0 if t is None else t.shape[-1] if t.shape[0] == 1 else t.stride(0)
-
-    if B and V:
-        logits, tokens, allowed = rows(logits), rows(tokens), rows(allowed)
-        lens, repetition, presence, frequency = flat(lens), flat(repetition), flat(presence), flat(frequency)
-        ldb = 0
-        if bias is not None:
-            if bias.dim() == 1 or bias.shape[0] == 1:
-                bias = bias.contiguous()
-            elif bias.stride(0) or (bias.stride(1) != 1 and V != 1):     # else one row, expanded
-                bias = rows(bias)
-                ldb = ld(bias)
-        with _on(dev):
-            _check(lib().xdna_logits_adjust(_ptr(logits), _DTYPE_CODE[logits.dtype], ld(logits), _ptr(tokens),
-                                            int(tokens is not None and tokens.dtype == torch.int64), ld(tokens),
-                                            0 if tokens is None else tokens.shape[1], _ptr(lens), _ptr(repetition),
-                                            _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(allowed), ld(allowed),
-                                            _ptr(y), B, V, _stream(dev)), "logits_adjust")
-    return y
+def op_counts(reset=False):
+    """(calls, multiply-accumulates, launches, seconds) of the operators' GPU kernels since the last reset."""
+    if _torch_lib is None:
+        return 0, 0, 0, 0.0
+    n = (ctypes.c_int64 * 4)()
+    _torch_lib.xdna_torch_counts(n, int(reset))
+    return n[0], n[1], n[2], n[3] * 1e-9

@@ -7,8 +7,8 @@
   quantize_w4       a float weight as linear_w4 takes it
 
 Each is also the op torch.ops.xdna.<name>, opaque to torch.compile. Tensors on a GPU go to the HIP
-kernels (kernels.py), on torch's current stream, without synchronizing; a GPU tensor with the library missing raises.
-Host tensors are computed here with plain torch in float32. There is no backward pass: a call that needs a
+kernels (csrc/xdna_torch.cpp checks the arguments there as the functions here do), on torch's current stream, without
+synchronizing; a GPU tensor with the library missing raises. Host tensors are computed here with plain torch in float32. There is no backward pass: a call that needs a
 gradient raises where the gradient is asked for. Wrong arguments raise ValueError or TypeError before anything is
 launched; what lies in GPU memory (lengths, starts, token ids) is not read on the host, and the kernels
 clamp it, so that no value of it reads or writes out of range.
@@ -23,6 +23,11 @@ from . import kernels
 from .runtime import stats
 
 FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _on_gpu(name, *args):
+    kernels.torch_lib()
+    return getattr(torch.ops.xdna, name)(*args)
 
 
 def _floats(name, t):
@@ -71,6 +76,8 @@ def linear_w4(x, qweight, scales, zeros=None, bias=None):
     """y [..., N] = x [..., K] times the transpose of (q - zero) * scale, plus bias [N], summed in float32 and rounded
     once to x's dtype. qweight uint8 [N, K / 2] (the even k of a byte in its low nibble), scales [N, K / G] with G a
     multiple of 32, zeros uint8 [N, K / G] or None for 8; qweight, scales and zeros contiguous."""
+    if x.is_cuda:
+        return _on_gpu("linear_w4", x, qweight, scales, zeros, bias)
     _floats("x", x)
     _floats("scales", scales)
     if qweight.dtype != torch.uint8 or (zeros is not None and zeros.dtype != torch.uint8):
@@ -91,15 +98,11 @@ def linear_w4(x, qweight, scales, zeros=None, bias=None):
         raise ValueError("linear_w4: qweight, scales and zeros must be contiguous")
     _same_device(x, qweight, scales, zeros, bias)
     t0 = time.perf_counter()
-    if x.is_cuda:
-        y = kernels.linear_w4(x.reshape(-1, k), qweight, scales, zeros, bias)
-        stats.launches += 1
-    else:
-        z = 8.0 if zeros is None else zeros.float().unsqueeze(-1)
-        q = torch.stack([qweight & 15, qweight >> 4], dim=-1).view(n, groups, -1).float()
-        y = x.reshape(-1, k).float() @ ((q - z) * scales.float().unsqueeze(-1)).view(n, k).t()
-        y = (y if bias is None else y + bias.float()).to(x.dtype)
-    stats.record("gpu" if x.is_cuda else "cpu", t0, y.shape[0] * n * k)
+    z = 8.0 if zeros is None else zeros.float().unsqueeze(-1)
+    q = torch.stack([qweight & 15, qweight >> 4], dim=-1).view(n, groups, -1).float()
+    y = x.reshape(-1, k).float() @ ((q - z) * scales.float().unsqueeze(-1)).view(n, k).t()
+    y = (y if bias is None else y + bias.float()).to(x.dtype)
+    stats.record("cpu", t0, y.shape[0] * n * k)
     return y.view(*x.shape[:-1], n)
 
 
@@ -148,6 +151,8 @@ def attention_causal(q, k, v, starts, scale=None):
     strides; H a multiple of KV, q head h with kv head h / (H / KV); D a multiple of 8, at most 128). starts int32 [S + 1]: the first
     token of each sequence, ascending, and T. A token sees its own sequence's tokens up to itself. scale: 1 / sqrt(D) if
     None. Float32 sums; the softmax's weights are rounded to q's dtype for their product with v, and the result once."""
+    if q.is_cuda:
+        return _on_gpu("attention_causal", q, k, v, starts, scale)
     if q.dim() != 3 or k.dim() != 3 or tuple(v.shape) != tuple(k.shape):
         raise ValueError(f"attention_causal takes q [T, H, D] and k, v [T, KV, D], got {list(q.shape)}, {list(k.shape)} and "
                          f"{list(v.shape)}")
@@ -159,19 +164,15 @@ def attention_causal(q, k, v, starts, scale=None):
         raise ValueError("starts must be [S + 1], got []")
     _same_device(q, k, v, starts)
     t0 = time.perf_counter()
-    if q.is_cuda:
-        o = kernels.attention_causal(q, k, v, starts.contiguous(), scale)
-        stats.launches += 1
-    else:
-        at = torch.arange(t)
-        seq = torch.searchsorted(starts, at, right=True)
-        seen = (seq[:, None] == seq[None, :]) & (at[None, :] <= at[:, None])
-        kv = k.shape[1]
-        qf, kf, vf = (x.float().transpose(0, 1) for x in (q, k, v))
-        qf = qf.reshape(kv, h // kv, t, d)
-        o = _softmax_v(qf @ kf[:, None].transpose(-1, -2) * scale, seen, vf[:, None])
-        o = o.reshape(h, t, d).transpose(0, 1).contiguous().to(q.dtype)
-    stats.record("gpu" if q.is_cuda else "cpu", t0, t * t * h * d)     # at most: the sequences' lengths are not read
+    at = torch.arange(t)
+    seq = torch.searchsorted(starts, at, right=True)
+    seen = (seq[:, None] == seq[None, :]) & (at[None, :] <= at[:, None])
+    kv = k.shape[1]
+    qf, kf, vf = (x.float().transpose(0, 1) for x in (q, k, v))
+    qf = qf.reshape(kv, h // kv, t, d)
+    o = _softmax_v(qf @ kf[:, None].transpose(-1, -2) * scale, seen, vf[:, None])
+    o = o.reshape(h, t, d).transpose(0, 1).contiguous().to(q.dtype)
+    stats.record("cpu", t0, t * t * h * d)     # at most: the sequences' lengths are not read
     return o
 
 
@@ -179,6 +180,8 @@ def attention_prefix(q, kp, vp, kc, vc, lens, scale=None):
     """One decode step's attention of B sequences that share a prefix: out [B, H, D] of q [B, H, D] (the new tokens'), kp, vp
     [P, KV, D] (the prefix's, held once) and kc, vc [B, S, KV, D], of which sequence b sees the first lens[b] (int32 [B]; clamped to
     0 .. S; the new token's own among them). P and S may be 0. Types, scale and rounding as in attention_causal."""
+    if q.is_cuda:
+        return _on_gpu("attention_prefix", q, kp, vp, kc, vc, lens, scale)
     if q.dim() != 3 or kp.dim() != 3 or kc.dim() != 4 or tuple(vp.shape) != tuple(kp.shape) or tuple(vc.shape) != tuple(kc.shape):
         raise ValueError(f"attention_prefix takes q [B, H, D], kp, vp [P, KV, D] and kc, vc [B, S, KV, D], got {list(q.shape)}, "
                          f"{list(kp.shape)}, {list(vp.shape)}, {list(kc.shape)} and {list(vc.shape)}")
@@ -192,17 +195,13 @@ def attention_prefix(q, kp, vp, kc, vc, lens, scale=None):
     _same_device(q, kp, vp, kc, vc, lens)
     t0 = time.perf_counter()
     n = kc.shape[1]
-    if q.is_cuda:
-        o = kernels.attention_prefix(q, kp, vp, kc, vc, lens.contiguous(), scale)
-        stats.launches += 1
-    else:
-        qf = q.float().view(b, kv, h // kv, d) if q.is_contiguous() else q.float().reshape(b, kv, h // kv, d)
-        k = torch.cat([kp.float().expand(b, p, kv, d), kc.float()], 1).permute(0, 2, 1, 3)
-        v = torch.cat([vp.float().expand(b, p, kv, d), vc.float()], 1).permute(0, 2, 1, 3)
-        seen = torch.arange(p + n)[None, :] < p + lens.clamp(0, n)[:, None]
-        o = _softmax_v(qf @ k.transpose(2, 3) * scale, seen[:, None, None, :].expand(b, kv, h // kv, p + n), v)
-        o = o.reshape(b, h, d).to(q.dtype)
-    stats.record("gpu" if q.is_cuda else "cpu", t0, 2 * b * (p + n) * h * d)
+    qf = q.float().reshape(b, kv, h // kv, d)
+    k = torch.cat([kp.float().expand(b, p, kv, d), kc.float()], 1).permute(0, 2, 1, 3)
+    v = torch.cat([vp.float().expand(b, p, kv, d), vc.float()], 1).permute(0, 2, 1, 3)
+    seen = torch.arange(p + n)[None, :] < p + lens.clamp(0, n)[:, None]
+    o = _softmax_v(qf @ k.transpose(2, 3) * scale, seen[:, None, None, :].expand(b, kv, h // kv, p + n), v)
+    o = o.reshape(b, h, d).to(q.dtype)
+    stats.record("cpu", t0, 2 * b * (p + n) * h * d)
     return o
 
 
@@ -214,6 +213,8 @@ def logits_adjust(logits, tokens=None, lens=None, repetition=None, presence=None
     tokens int32 or int64 [B, L] with lens int32 [B] (clamped to 0 .. L; ids outside 0 .. V - 1 count nowhere); repetition,
     presence, frequency float32 [B]; bias float32 [V] or [B, V]; allowed int32 [B, ceil(V / 32)], token v at bit v % 32 of
     word v / 32. Each may be None."""
+    if logits.is_cuda:
+        return _on_gpu("logits_adjust", logits, tokens, lens, repetition, presence, frequency, bias, allowed)
     _floats("logits", logits)
     if logits.dim() != 2:
         raise ValueError(f"logits must be [B, V], got {list(logits.shape)}")
@@ -237,10 +238,7 @@ def logits_adjust(logits, tokens=None, lens=None, repetition=None, presence=None
         _whole("allowed", allowed, 2, "[B, ceil(V / 32)]")
         _shape("allowed", allowed, (b, -(-v // 32)))
     _same_device(logits, tokens, lens, repetition, presence, frequency, bias, allowed)
-    if logits.is_cuda:
-        y = kernels.logits_adjust(logits, tokens, lens, repetition, presence, frequency, bias, allowed)
-        stats.launches += 1
-        return y
+    t0 = time.perf_counter()
     x = logits.float()
     if tokens is not None:
         t = tokens.long()
@@ -259,4 +257,5 @@ def logits_adjust(logits, tokens=None, lens=None, repetition=None, presence=None
     if allowed is not None:
         ok = (allowed.unsqueeze(-1) >> torch.arange(32, dtype=torch.int32)) & 1
         x = x.masked_fill(ok.view(b, -1)[:, :v] == 0, -math.inf)
+    stats.record("cpu", t0, 0)
     return x.to(logits.dtype)

@@ -10,12 +10,13 @@ torch.compile each op is opaque with a shape function; Inductor compiles everyth
 calls it as an extern kernel.
 """
 
+import os
 from typing import Optional
 
 import torch
 import torch._dynamo
 
-from . import conv, lm, runtime, stack
+from . import conv, kernels, lm, runtime, stack
 
 try:    # what custom_op registers for autograd (below)
     from torch._library.autograd import make_autograd_impl as _make_autograd_impl
@@ -234,8 +235,9 @@ if hasattr(linear, "_opoverload"):
     _direct(conv3x3_fused, lambda x, w, b, relu, cid: conv.conv3x3_fused(_configs[cid], x, w, b, relu), _lib)
     _direct(conv3x3_chain, lambda x, ws, bs, relus, after, pools, cid: conv.conv3x3_chain(
         _configs[cid], cid, x, list(ws), list(bs), list(relus), list(after), list(pools)), _lib)
-    _direct(linear_w4, lm.linear_w4, _lib)
-    _direct(attention_causal, lm.attention_causal, _lib)
-    _direct(attention_prefix, lm.attention_prefix, _lib)
-    _direct(logits_adjust, lm.logits_adjust, _lib)
     _direct(qwen3_stack, lambda x, mask, sid, cid: stack.run(_configs[cid], sid, x, mask), _lib)
+
+# The language model operators' GPU kernels and their way past autograd are C++ (csrc/xdna_torch.cpp). Without the library
+# their GPU calls reach the functions above, which raise.
+if os.path.exists(kernels.TORCH_LIB_PATH):
+    kernels.torch_lib()

@@ -48,6 +48,7 @@ class Stats:
         self.fallbacks = []             # (shape or layer, error text)
         self.stacks = Counter()         # (stack name, "gpu" fused / "cpu" plain graph) -> graph calls
         self.checks = []                # (stack, relative error) of first fused calls
+        kernels.op_counts(reset=True)
 
     def record(self, device, since, macs):
         """One op call on `device` that started at perf_counter() value `since`."""
@@ -57,10 +58,16 @@ class Stats:
 
     def as_dict(self):
         ok, why = kernels.available(), kernels.unavailable_reason()
-        d = {"calls": dict(self.calls),
-             "seconds": {dev: round(t, 4) for dev, t in self.seconds.items()},
-             "gmacs": {dev: round(m / 1e9, 3) for dev, m in self.macs.items()},
-             "gpu_launches": self.launches, "fallbacks": list(self.fallbacks),
+        calls, seconds, macs, launches = dict(self.calls), dict(self.seconds), dict(self.macs), self.launches
+        n, m, started, t = kernels.op_counts()          # of the operators that count for themselves
+        if n:
+            for total, part in ((calls, n), (seconds, t), (macs, m)):
+                total["gpu"] = total.get("gpu", 0) + part
+            launches += started
+        d = {"calls": calls,
+             "seconds": {dev: round(t, 4) for dev, t in seconds.items()},
+             "gmacs": {dev: round(m / 1e9, 3) for dev, m in macs.items()},
+             "gpu_launches": launches, "fallbacks": list(self.fallbacks),
              "stacks": {f"{name} on {dev}": n for (name, dev), n in self.stacks.items()},
              "checks": list(self.checks),
              "decisions": {"x".join(str(p) for p in key): v for key, v in decisions.items()},
