@@ -164,220 +164,163 @@ __device__ __forceinline__ void add_not_finite(f32x16a (&o)[D / 32], const float
   }
 }
 
-// LDS bytes of a workgroup: K and V of ST tiles of KT keys for each of KW groups of waves
-template <int D, int KW, int KT, int ST>
-constexpr int LDS_BYTES = KW * ST * 2 * KT * 2 * D;
-
-// Attention of QW x KW waves: wave w has the 32 rows w % QW (fragments qf, in the MFMA's order) and the tiles
-// kg, kg + KW, ... of group kg = w / QW; the groups meet in LDS. ST == 2: tile t + 1 loads while t is used, one workgroup barrier a tile.
-// ST == 1 (QW == 1, a group's LDS is its wave's own): K of the next tile loads once S is done, V after the tile.
-// store(chunk, o, m, l) receives dims 8 (chunk % 4) + 32 (chunk / 4) + 4 (lane / 32) .. + 3 of the lane's row: the sum
-// of p v, the maximum and the sum of p.
-template <int DT, int D, int QW, int KW, int KT, int ST, bool CAUSAL, class Store>
-__device__ __forceinline__ void attend(int8_t* lds_all, float* ml, const Keys& ks, int d, const i32x4 (&qf)[D / 16],
-                                       const Seen& seen, float c, Store&& store) {
-  static_assert(ST == 2 || (QW == 1 && KT == 32), "a single stage is one wave's own and one block of keys");
-  constexpr int RB = 2 * D, KB = KT * RB, STAGE = 2 * KB, NB = KT / 32, DB = D / 32;
-  constexpr int CH = D / 8, RPL = 64 / CH;    // 16-byte chunks of a row, rows of one 1 KB load
-  constexpr int NI = KB / 1024 / QW;          // 1 KB loads of K, and of V, per wave and tile
+// Attention of 32 rows by KW waves: wave w has the tiles w, w + KW, ... of 32 keys, in LDS of its own (kl_, vl_: KW tiles of
+// K, and of V, each an array, so that the compiler knows which loads a read has to wait for), and the waves meet in LDS at
+// the end (meet: KW x 32 x D float32, which may lie over the tiles; ml: 2 KW x 64). No barriers before that: K of a wave's next
+// tile loads once its scores are done, V after its products. store(chunk, o, m, l) receives dims 8 (chunk % 4) + 32 (chunk / 4) +
+// 4 (lane / 32) .. + 3 of the lane's row: the sum of p v, the maximum and the sum of p.
+template <int DT, int D, int KW, bool CAUSAL, class Store>
+__device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml, const Keys& ks, int d, const i32x4 (&qf)[D / 16],
+                                             const Seen& seen, float c, Store&& store) {
+  constexpr int KT = 32, RB = 2 * D, KB = KT * RB, DB = D / 32, CH = D / 8, RPL = 64 / CH, NI = KB / 1024;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kg = wave / QW, qw = wave - kg * QW;
-  int8_t* const lds = lds_all + kg * (ST * STAGE);
-  // this lane's share of load j: row lrow + j * RPL of the tile, chunk lane % CH of its LDS row
-  int lrow[NI];
-  uint32_t kc[NI], vc[NI];
-#pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    lrow[j] = (qw * NI + j) * RPL + lane / CH;
-    kc[j] = (uint32_t)(((lane % CH) ^ k_swizzle<D>(lrow[j])) * 16);
-    vc[j] = (uint32_t)(((lane % CH) ^ (v_swizzle<D>(lrow[j]) * 4)) * 16);
-  }
-  const int t1 = (int)cdiv(ks.n, KT), tiles = t1 + (int)cdiv(ks.n2, KT), nt = (int)cdiv(tiles, KW);
-  auto load = [&](bool v, int tile, int8_t* dst) {
+  const int base = wave * KB;
+  const int t1 = (int)cdiv(ks.n, KT), tiles = t1 + (int)cdiv(ks.n2, KT);
+  // load j: rows j RPL + lane / CH, chunk lane % CH of the LDS row; a tile past the last loads nothing (the bounds check), so that
+  // the loads under way are always as many
+  auto load = [&](bool v, int tile) {
     const bool two = tile >= t1;
-    const int k0 = (two ? tile - t1 : tile) * KT, left = (two ? ks.n2 : ks.n) - k0;
+    const int k0 = (two ? tile - t1 : tile) * KT, left = min((two ? ks.n2 : ks.n) - k0, KT) - 1;
     const int64_t pitch = v ? (two ? ks.vp2 : ks.vp) : (two ? ks.kp2 : ks.kp);
-    const char* base = (v ? (two ? ks.v2 : ks.v) : (two ? ks.k2 : ks.k)) + k0 * pitch;
-    const auto r = make_rsrc(base, left > 0 ? (uint32_t)(min(left, KT) - 1) * (uint32_t)pitch + 2u * d : 0u);
+    const char* from = (v ? (two ? ks.v2 : ks.v) : (two ? ks.k2 : ks.k)) + k0 * pitch;
+    const auto r = make_rsrc(from, tile < tiles && left >= 0 ? (uint32_t)left * (uint32_t)pitch + 2u * d : 0u);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const uint32_t at = v ? vc[j] : kc[j];
-      const uint32_t off = at < 2u * d ? (uint32_t)lrow[j] * (uint32_t)pitch + at : OOB;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void)(dst + ((qw * NI + j) << 10)), 16, (int)off, 0, 0, 0);
+      const int lrow = j * RPL + lane / CH;
+      const uint32_t at = (uint32_t)(((lane % CH) ^ (v ? v_swizzle<D>(lrow) * 4 : k_swizzle<D>(lrow))) * 16);
+      const uint32_t off = at < 2u * d ? (uint32_t)lrow * (uint32_t)pitch + at : OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void)((v ? vl_ : kl_) + (base + (j << 10))), 16, (int)off, 0, 0, 0);
     }
   };
   f32x16a o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16a{};
   float m = -INFINITY, l = 0.0f;
-  const int krd = row * RB, kx = k_swizzle<D>(row);
-  const int vkey = 4 * half + ((lane & 15) >> 2);      // of each 8 keys
-  const int vrd = vkey * RB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3), vx = v_swizzle<D>(vkey);
-  // the V^T fragment of step u and dims 32 db .. + 31 of a block of 32 keys
-  auto v_frag = [&](const int8_t* vb, int u, int db) {
-    const int8_t* at = vb + vrd + ((db ^ vx) << 6) + u * 16 * RB;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * RB));
+  // each read one index from its array: through a chain of offsets the compiler loses sight of which array it is
+  const int vkey = 4 * half + ((lane & 15) >> 2);
+  int voff[DB], koff[D / 16];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    voff[db] = base + vkey * RB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + ((db ^ v_swizzle<D>(vkey)) << 6);
+    asm volatile("" : "+v"(voff[db]));
+  }
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    koff[s] = base + row * RB + (((2 * s + half) ^ k_swizzle<D>(row)) << 4);
+    asm volatile("" : "+v"(koff[s]));
+  }
+  auto v_frag = [&](int u, int db) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vl_ + (voff[db] + u * 16 * RB)));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vl_ + (voff[db] + u * 16 * RB + 8 * RB)));
     const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
     return i32x4{(int)x.x, (int)x.y, (int)y.x, (int)y.y};
   };
-  if (kg < tiles) {
-    load(false, kg, lds);
-    load(true, kg, lds + KB);
-  }
-  for (int t = 0; t < nt; ++t) {
-    const int tile = t * KW + kg, next = tile + KW;
-    int8_t* const cur = lds + (ST == 2 ? (t & 1) * STAGE : 0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    if constexpr (ST == 2) {
-      __builtin_amdgcn_s_barrier();          // tile t is whole; every wave is done with tile t - 1
-      __builtin_amdgcn_sched_barrier(0);
-      if (next < tiles) {
-        load(false, next, lds + ((t + 1) & 1) * STAGE);
-        load(true, next, lds + ((t + 1) & 1) * STAGE + KB);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (tile >= tiles) continue;             // uniform over the group, at its last tile
+  load(false, wave);
+  load(true, wave);
+#pragma unroll 1
+  for (int tile = wave; tile < tiles; tile += KW) {
     const int k0 = (tile >= t1 ? tile - t1 : tile) * KT, left = (tile >= t1 ? ks.n2 : ks.n) - k0;
-    if (CAUSAL && (k0 > seen.last || k0 + KT - 1 < seen.first)) {        // no row of this wave sees a key of the tile
-      if constexpr (ST == 1) {
-        if (next < tiles) {
-          load(false, next, cur);
-          load(true, next, cur + KB);
-        }
-      }
-      continue;
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NI) : "memory");      // K is here, V need not be
+    f32x16a sc = f32x16a{};
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      sc = mfma32<DT>(*reinterpret_cast<const i32x4*>(kl_ + koff[s]), qf[s], sc);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    load(false, tile + KW);
+    __builtin_amdgcn_sched_barrier(0);
+    auto visible = [&](int k) { return CAUSAL ? k0 + k >= seen.lo && k0 + k <= seen.hi : k < left; };
+    const bool part = CAUSAL ? k0 < seen.from_all || k0 + KT - 1 > seen.to_all : left < KT;      // uniform over the wave
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!visible(8 * (e >> 2) + 4 * half + (e & 3))) sc[e] = -INFINITY;
     }
-    const bool part = CAUSAL ? (k0 < seen.from_all || k0 + KT - 1 > seen.to_all) : left < KT;   // uniform over the wave
+    float mx = sc[0];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int8_t* const kb = cur + b * 32 * RB;
-      const int8_t* const vb = cur + KB + b * 32 * RB;
-      f32x16a sc = f32x16a{};
-      __builtin_amdgcn_s_setprio(1);
+    for (int e = 1; e < 15; e += 2) mx = __builtin_elementwise_maximum(mx, __builtin_elementwise_maximum(sc[e], sc[e + 1]));
+    mx = pair_max(__builtin_elementwise_maximum(mx, sc[15]));
+    // the running maximum follows: at few tiles a wave that is as good as not asking whether it has to
+    const float mn = mx > m ? mx : m;
+    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+    l = m == -INFINITY ? l : l * alpha;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-        sc = mfma32<DT>(*reinterpret_cast<const i32x4*>(kb + krd + (((2 * s + half) ^ kx) << 4)), qf[s], sc);
-      if constexpr (ST == 1) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        if (next < tiles) load(false, next, cur);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      auto visible = [&](int e) {
-        const int key = k0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3);
-        return CAUSAL ? key >= seen.lo && key <= seen.hi : key - k0 < left;
-      };
-      if (part) {
+    for (int db = 0; db < DB; ++db) o[db] *= alpha;
+    m = mn;
+    const float mc = (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
+    i32x4 pf[2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!visible(e)) sc[e] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; e += 2)
-        mx = __builtin_elementwise_maximum(mx, __builtin_elementwise_maximum(sc[e], sc[e + 1]));
-      mx = pair_max(mx);
-      const bool grow = mx > m;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float mn = grow ? mx : m;
-        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
-        l *= alpha;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] *= alpha;
-        m = mn;
-      }
-      const float mc = (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
-      float p[16], ps[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc));     // unseen: 2^-inf, c > 0
-      }
-      i32x4 pf[2];
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        ps[0] += p[e];
-        ps[1] += p[e + 1];
-        pf[e >> 3][(e & 7) >> 1] = (int)pack2<DT>(p[e], p[e + 1]);
-      }
-      l += ps[0] + ps[1];
-      bool odd = false;
-      if (CAUSAL && part) odd = not_finite<DT, DB>([&](int u, int db) { return v_frag(vb, u, db); });
-      if (CAUSAL && odd) {
-        add_not_finite<DT, D>(o, p, pf, vb, [&](int u, int db) { return v_frag(vb, u, db); }, [&](int kk) {
-          const int key = k0 + 32 * b + kk;
-          return key >= seen.lo && key <= seen.hi;
-        });
-      } else {
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) o[db] = mfma32<DT>(v_frag(vb, u, db), pf[u], o[db]);
-        __builtin_amdgcn_s_setprio(0);
-      }
+    for (int e = 0; e < 16; e += 2) {
+      const uint32_t w = pack2<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc)),
+                                   __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], c, -mc)));
+      pf[e >> 3][(e & 7) >> 1] = (int)w;
+      l = dot_ones<DT>(w, l);
     }
-    if constexpr (ST == 1) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      if (next < tiles) load(true, next, cur + KB);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");                 // V is here, the next K need not be
+    bool odd = false;
+    if (CAUSAL && part) odd = not_finite<DT, DB>(v_frag);
+    if (CAUSAL && odd) {
+      float p[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], c, -mc));
+      add_not_finite<DT, D>(o, p, pf, vl_ + base, v_frag, visible);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = mfma32<DT>(v_frag(u, db), pf[u], o[db]);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    load(true, tile + KW);
+    __builtin_amdgcn_sched_barrier(0);
   }
   l = pair_sum(l);
-  if constexpr (KW == 1) {
+  // each wave leaves its m, l and O where its tiles were (half of O in K's place, half in V's); wave w then joins chunks w, w + KW, ..
+  constexpr int OB = 32 * D * 2, NC = 4 * DB;      // bytes of half a wave's O, chunks
+  static_assert(OB == KB, "half of O takes a tile of K");
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  ml[wave * 64 + lane] = m;
+  ml[(KW + wave) * 64 + lane] = l;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+  for (int i = 0; i < NC; ++i)
+    *reinterpret_cast<f32x4*>(i < NC / 2 ? kl_ + (base + i * 1024 + lane * 16) : vl_ + (base + (i - NC / 2) * 1024 + lane * 16)) =
+        f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+  __syncthreads();
+  float mt = -INFINITY, lt = 0.0f, w[KW];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store(4 * db + g, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]}, m, l);
-  } else {
-    // each wave leaves its m, l and O; wave (kg, qw) then joins chunks kg, kg + KW, ... of the 32 rows of qw
-    constexpr int OB = 32 * D * 4;           // bytes of a wave's O
-    static_assert(QW * KW * OB <= LDS_BYTES<D, KW, KT, ST>, "the outputs meet where the tiles were");
-    __syncthreads();
-    ml[wave * 64 + lane] = m;
-    ml[(QW * KW + wave) * 64 + lane] = l;
+  for (int g = 0; g < KW; ++g) mt = fmaxf(mt, ml[g * 64 + lane]);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+  for (int g = 0; g < KW; ++g) {
+    const float mg = ml[g * 64 + lane], lg = ml[(KW + g) * 64 + lane];
+    w[g] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mg - mt) * c);     // a wave without keys: nothing
+    lt += mg == -INFINITY ? lg : lg * w[g];              // lg is 0 then, or NaN
+  }
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(lds_all + wave * OB + (db * 4 + g) * 1024 + lane * 16) =
-            f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-    __syncthreads();
-    float mt = -INFINITY, lt = 0.0f, w[KW];
-#pragma unroll
-    for (int g = 0; g < KW; ++g) mt = fmaxf(mt, ml[(g * QW + qw) * 64 + lane]);
+  for (int i = 0; i < (NC + KW - 1) / KW; ++i) {
+    const int chunk = wave + i * KW;
+    if (NC % KW && chunk >= NC) break;
+    const int8_t* const from = chunk < NC / 2 ? kl_ + chunk * 1024 : vl_ + (chunk - NC / 2) * 1024;
+    f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int g = 0; g < KW; ++g) {
-      const float mg = ml[(g * QW + qw) * 64 + lane];
-      w[g] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mg - mt) * c);     // a group without keys: nothing
-      const float lg = ml[(QW * KW + g * QW + qw) * 64 + lane];
-      lt += mg == -INFINITY ? lg : lg * w[g];            // lg is 0 then, or NaN
+      const f32x4 x = *reinterpret_cast<const f32x4*>(from + g * KB + lane * 16);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += x[r] * w[g];
     }
-#pragma unroll
-    for (int i = 0; i < 4 * DB / KW; ++i) {
-      const int chunk = kg + i * KW;
-      f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int g = 0; g < KW; ++g) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(lds_all + (g * QW + qw) * OB + chunk * 1024 + lane * 16);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += x[r] * w[g];
-      }
-      store(chunk, v, mt, lt);
-    }
+    store(chunk, v, mt, lt);
   }
 }
 
-// The same for four waves of 32 rows that share every tile of 64 keys: the form for many rows. K and V of two tiles have
+// Four waves of 32 rows that share every tile of 64 keys: the form for many rows. Waves without rows (idle) only load. K and V of two tiles have
 // an LDS array each, so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way while
 // tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
 // go by one copy of the masked one.
 template <int DT, int D, bool CAUSAL, class Store>
 __device__ __forceinline__ void attend_wide(int8_t* k0_, int8_t* v0_, int8_t* k1_, int8_t* v1_, const Keys& ks, int d,
-                                            const i32x4 (&qf)[D / 16], const Seen& seen, float c, Store&& store) {
+                                            const i32x4 (&qf)[D / 16], const Seen& seen, bool idle, float c,
+                                            Store&& store) {
   constexpr int QW = 4, KT = 64, RB = 2 * D, KB = KT * RB, DB = D / 32;
   constexpr int CH = D / 8, RPL = 64 / CH, NI = KB / 1024 / QW;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
@@ -562,9 +505,14 @@ __device__ __forceinline__ void attend_wide(int8_t* k0_, int8_t* v0_, int8_t* k1
   };
   // The tiles that every row of this wave sees whole are a run of them; its pairs of an even tile and the next take the short
   // path. Waves may disagree on it: each passes one barrier a tile in any case.
+  if (tiles > 0) load(0, k0_, v0_);
+  if (idle) {
+    for (int t = 0; t < tiles; ++t) arrive(t, t & 1 ? k0_ : k1_, t & 1 ? v0_ : v1_);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return;
+  }
   const int all0 = CAUSAL ? (int)(cdiv(seen.from_all, 2 * KT) * 2) : 0;
   const int all1 = max(all0, (CAUSAL ? (seen.to_all + 1) / (2 * KT) : ks.n / (2 * KT)) * 2);
-  if (tiles > 0) load(0, k0_, v0_);
   masked(0, min(all0, tiles));
   for (int t = all0; t < all1; t += 2) {
     arrive(t, k1_, v1_);
@@ -679,11 +627,12 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
     __shared__ __attribute__((aligned(1024))) int8_t v0[128 * D];
     __shared__ __attribute__((aligned(1024))) int8_t k1[128 * D];
     __shared__ __attribute__((aligned(1024))) int8_t v1[128 * D];
-    attend_wide<DT, D, true>(k0, v0, k1, v1, ks, a.d, qf, seen, a.c, store);
+    attend_wide<DT, D, true>(k0, v0, k1, v1, ks, a.d, qf, seen, row0 + 32 * wave >= nrows, a.c, store);
   } else {
-    __shared__ __attribute__((aligned(1024))) int8_t lds[LDS_BYTES<D, 4, 32, 1>];
+    __shared__ __attribute__((aligned(1024))) int8_t kl[4 * 64 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t vl[4 * 64 * D];
     __shared__ float ml[2 * 4 * 64];
-    attend<DT, D, 1, 4, 32, 1, true>(lds, ml, ks, a.d, qf, seen, a.c, store);
+    attend_split<DT, D, 4, true>(kl, vl, ml, ks, a.d, qf, seen, a.c, store);
   }
 }
 
@@ -712,15 +661,17 @@ struct PrefixArgs {
   uint16_t* out;
 };
 
-// Workgroups 0 .. nkv rblocks np - 1 take a part of the prefix for the rows (sequence, q head) of a kv head, 32 QW at a
-// time; the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a workgroup
-// takes all the keys of its (sequence, kv head) and writes the output itself.
-template <int DT, int D, int QW, int KW>
-__global__ __launch_bounds__(256, 2) void prefix_kernel(PrefixArgs a) {
-  constexpr int KT = KW == 1 ? 64 : 32, ST = QW == 1 ? 1 : 2;
-  __shared__ __attribute__((aligned(1024))) int8_t
-      lds[LDS_BYTES<D, KW, KT, ST> > LDS_BYTES<D, 4, 32, 1> ? LDS_BYTES<D, KW, KT, ST> : LDS_BYTES<D, 4, 32, 1>];
-  __shared__ float ml[2 * 4 * 64];
+// Workgroups 0 .. nkv rblocks np - 1 take a part of the prefix for the rows (sequence, q head) of a kv head, 32 at a time, or
+// 128 (WIDE); the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a workgroup
+// takes all the keys of its (sequence, kv head) and writes the output itself. KW: waves that share out keys.
+template <int DT, int D, bool WIDE, int KW>
+__global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
+  static_assert(!WIDE || KW == 4, "four waves in the wide form");
+  constexpr int QW = WIDE ? 4 : 1;
+  // the wide form's second pair of tiles, and the split form's K and V, by halves
+  __shared__ __attribute__((aligned(1024))) int8_t lds_k[KW * 64 * D];
+  __shared__ __attribute__((aligned(1024))) int8_t lds_v[KW * 64 * D];
+  __shared__ float ml[2 * KW * 64];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.nh / a.nkv;
@@ -756,8 +707,14 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(PrefixArgs a) {
     ks.k = reinterpret_cast<const char*>(a.kp + k0 * a.kpt + kvh * a.kph);
     ks.v = reinterpret_cast<const char*>(a.vp + k0 * a.vpt + kvh * a.vph);
     ks.n = max(0, min(a.pkeys, a.P - k0));
-    attend<DT, D, QW, KW, KT, ST, false>(lds, ml, ks, a.d, qf, seen, a.c,
-                                         write(part, (int64_t)b * a.nh + head, want < nrows));
+    const auto out = write(part, (int64_t)b * a.nh + head, want < nrows);
+    if constexpr (WIDE) {
+      __shared__ __attribute__((aligned(1024))) int8_t k0[128 * D];
+      __shared__ __attribute__((aligned(1024))) int8_t v0[128 * D];
+      attend_wide<DT, D, false>(k0, v0, lds_k, lds_v, ks, a.d, qf, seen, rb * 128 + 32 * wave >= nrows, a.c, out);
+    } else {
+      attend_split<DT, D, KW, false>(lds_k, lds_v, ml, ks, a.d, qf, seen, a.c, out);
+    }
     return;
   }
   // rows: the q heads of one (sequence, kv head), 32 at a time
@@ -786,36 +743,47 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(PrefixArgs a) {
     ks.vp = 2 * a.vct;
     ks.n = (int)max<int64_t>(0, min<int64_t>(a.okeys, len - k0));
   }
-  attend<DT, D, 1, 4, 32, 1, false>(lds, ml, ks, a.d, qf, seen, a.c,
-                                    write(all ? -1 : a.np + part, (int64_t)b * a.nh + head, want < grp));
+  attend_split<DT, D, KW, false>(lds_k, lds_v, ml, ks, a.d, qf, seen, a.c,
+                                 write(all ? -1 : a.np + part, (int64_t)b * a.nh + head, want < grp));
 }
 
-// The parts of a row joined, in their order: a wave per row, lane l dims 2 l, 2 l + 1.
+// The parts of a row joined: a workgroup per row, wave w the parts w, w + 4, .., then the waves in their order; lane l dims
+// 2 l, 2 l + 1.
 template <int DT>
 __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restrict__ po, const float* __restrict__ pml,
                                                           int parts, int64_t rows, int d, float c,
                                                           uint16_t* __restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  __shared__ float2 ov[4][64];
+  __shared__ float lv[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = blockIdx.x;
   float mt = -INFINITY;
   for (int i = lane; i < parts; i += 64) mt = fmaxf(mt, pml[(i * rows + row) * 2]);
   mt = wave_max(mt);
   float l = 0.0f, x = 0.0f, y = 0.0f;
-  const bool mine = 2 * lane < d;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
+  const int at = min(2 * lane, d - 2);
+#pragma unroll 8
+  for (int i = wave; i < parts; i += 4) {
     const float2 p = *reinterpret_cast<const float2*>(pml + (i * rows + row) * 2);
+    const float2 v = *reinterpret_cast<const float2*>(po + (i * rows + row) * d + at);
     const float w = p.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((p.x - mt) * c);
     l += p.x == -INFINITY ? p.y : p.y * w;
-    if (mine) {
-      const float2 v = *reinterpret_cast<const float2*>(po + (i * rows + row) * d + 2 * lane);
-      x += v.x * w;
-      y += v.y * w;
-    }
+    x += v.x * w;
+    y += v.y * w;
+  }
+  ov[wave][lane] = make_float2(x, y);
+  if (lane == 0) lv[wave] = l;
+  __syncthreads();
+  if (wave || 2 * lane >= d) return;
+  l = lv[0];
+#pragma unroll
+  for (int g = 1; g < 4; ++g) {
+    l += lv[g];
+    x += ov[g][lane].x;
+    y += ov[g][lane].y;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (mine) *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack2<DT>(x * inv, y * inv);
+  *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack2<DT>(x * inv, y * inv);
 }
 
 // How a call is split: two workgroups a CU where there are keys enough, no part under 256 keys (128 of a sequence's
@@ -823,7 +791,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
 void prefix_plan(PrefixArgs& a) {
   const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), want = 2 * device_cus();
   const int64_t rows = a.B * grp;
-  a.rblocks = (int)cdiv(rows, rows <= 32 ? 32 : rows <= 64 ? 64 : 128);
+  a.rblocks = (int)cdiv(rows, rows <= 32 ? 32 : 128);
   if ((int64_t)a.P + a.S <= 1024) {
     a.np = a.no = 0;
     a.pkeys = a.okeys = 0;
@@ -841,12 +809,11 @@ template <int DT, int D>
 int prefix_go(const PrefixArgs& a, hipStream_t st) {
   const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), rows = a.B * grp;
   const int64_t grid = (a.np * (int64_t)a.rblocks + a.B * hb * std::max(1, a.no)) * a.nkv;
-  if (rows <= 32 || a.np == 0) prefix_kernel<DT, D, 1, 4><<<(unsigned)grid, 256, 0, st>>>(a);
-  else if (rows <= 64) prefix_kernel<DT, D, 2, 2><<<(unsigned)grid, 256, 0, st>>>(a);
-  else prefix_kernel<DT, D, 4, 1><<<(unsigned)grid, 256, 0, st>>>(a);
+  if (a.np + a.no == 0) prefix_kernel<DT, D, false, 8><<<(unsigned)grid, 512, 0, st>>>(a);
+  else if (rows <= 32 || a.np == 0) prefix_kernel<DT, D, false, 4><<<(unsigned)grid, 256, 0, st>>>(a);
+  else prefix_kernel<DT, D, true, 4><<<(unsigned)grid, 256, 0, st>>>(a);
   if (a.np + a.no > 0)
-    prefix_join_kernel<DT><<<(unsigned)cdiv((int64_t)a.B * a.nh, 4), 256, 0, st>>>(
-        a.po, a.pml, a.np + a.no, (int64_t)a.B * a.nh, a.d, a.c, a.out);
+    prefix_join_kernel<DT><<<(unsigned)((int64_t)a.B * a.nh), 256, 0, st>>>(a.po, a.pml, a.np + a.no, (int64_t)a.B * a.nh, a.d, a.c, a.out);
   return launch_status("attention_prefix");
 }
 
