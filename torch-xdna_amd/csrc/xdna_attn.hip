@@ -313,19 +313,19 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
   }
 }
 
-// Four waves of 32 rows that share every tile of 64 keys: the form for many rows. Waves without rows (idle) only load. K and V of two tiles have
-// an LDS array each, so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way while
-// tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
+// Four waves of 32 rows that share every tile of 64 keys: the form for many rows. Waves without rows (idle) only load. Two tiles have
+// an LDS array each (K, then V), so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way
+// while tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
 // go by one copy of the masked one.
 template <int DT, int D, bool CAUSAL, class Store>
-__device__ __forceinline__ void attend_wide(int8_t* k0_, int8_t* v0_, int8_t* k1_, int8_t* v1_, const Keys& ks, int d,
-                                            const i32x4 (&qf)[D / 16], const Seen& seen, bool idle, float c,
+__device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Keys& ks, int d, const i32x4 (&qf)[D / 16], const Seen& seen, bool idle, float c,
                                             Store&& store) {
   constexpr int QW = 4, KT = 64, RB = 2 * D, KB = KT * RB, DB = D / 32;
   constexpr int CH = D / 8, RPL = 64 / CH, NI = KB / 1024 / QW;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (int)cdiv(ks.n, KT);
+  int8_t *const k0_ = lds0, *const v0_ = lds0 + KB, *const k1_ = lds1, *const v1_ = lds1 + KB;
   // this lane's share of load j: row (4 NI wave + j) RPL + lane / CH of the tile, chunk lane % CH of its LDS row. V's chunk
   // is the same for every j (a multiple of 4 rows apart).
   uint32_t ko[NI], vo[NI];
@@ -623,11 +623,9 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
     if (mine && dim < a.d) store4<DT>(orow + dim, o, l == 0.0f ? 0.0f : 1.0f / l);
   };
   if constexpr (WIDE) {
-    __shared__ __attribute__((aligned(1024))) int8_t k0[128 * D];
-    __shared__ __attribute__((aligned(1024))) int8_t v0[128 * D];
-    __shared__ __attribute__((aligned(1024))) int8_t k1[128 * D];
-    __shared__ __attribute__((aligned(1024))) int8_t v1[128 * D];
-    attend_wide<DT, D, true>(k0, v0, k1, v1, ks, a.d, qf, seen, row0 + 32 * wave >= nrows, a.c, store);
+    __shared__ __attribute__((aligned(1024))) int8_t lds0[256 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t lds1[256 * D];
+    attend_wide<DT, D, true>(lds0, lds1, ks, a.d, qf, seen, row0 + 32 * wave >= nrows, a.c, store);
   } else {
     __shared__ __attribute__((aligned(1024))) int8_t kl[4 * 64 * D];
     __shared__ __attribute__((aligned(1024))) int8_t vl[4 * 64 * D];
@@ -668,7 +666,7 @@ template <int DT, int D, bool WIDE, int KW>
 __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
   static_assert(!WIDE || KW == 4, "four waves in the wide form");
   constexpr int QW = WIDE ? 4 : 1;
-  // the wide form's second pair of tiles, and the split form's K and V, by halves
+  // K and V of the split form; a tile each of the wide one
   __shared__ __attribute__((aligned(1024))) int8_t lds_k[KW * 64 * D];
   __shared__ __attribute__((aligned(1024))) int8_t lds_v[KW * 64 * D];
   __shared__ float ml[2 * KW * 64];
@@ -709,9 +707,7 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
     ks.n = max(0, min(a.pkeys, a.P - k0));
     const auto out = write(part, (int64_t)b * a.nh + head, want < nrows);
     if constexpr (WIDE) {
-      __shared__ __attribute__((aligned(1024))) int8_t k0[128 * D];
-      __shared__ __attribute__((aligned(1024))) int8_t v0[128 * D];
-      attend_wide<DT, D, false>(k0, v0, lds_k, lds_v, ks, a.d, qf, seen, rb * 128 + 32 * wave >= nrows, a.c, out);
+      attend_wide<DT, D, false>(lds_k, lds_v, ks, a.d, qf, seen, rb * 128 + 32 * wave >= nrows, a.c, out);
     } else {
       attend_split<DT, D, KW, false>(lds_k, lds_v, ml, ks, a.d, qf, seen, a.c, out);
     }
