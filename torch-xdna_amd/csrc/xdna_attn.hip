@@ -782,19 +782,22 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
   *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack2<DT>(x * inv, y * inv);
 }
 
-// How a call is split: two workgroups a CU where there are keys enough, no part under 256 keys (128 of a sequence's
-// own). One part of both and few keys: a workgroup for each (sequence, kv head), one launch.
+// How a call is split. Up to 512 keys for few sequences: a workgroup of eight waves for each (sequence, kv head), one launch and
+// nothing to join (4 sequences, 8 kv heads, 264 + 64 keys 9.3 us, in parts 10.7; 64 sequences, 500 + 100: 20.5 / 16.5). Else the
+// prefix in parts that make a workgroup a CU in the 32-row form, two in the 128-row one, none under 256 keys, and own keys
+// in parts of 128 at least as far as two workgroups a CU take them (1 sequence, 32768 keys, 8 kv heads: 16 / 32 / 64 parts 29.1 /
+// 28.0 / 30.7 us; 24 x 32 heads over 100000: 32 / 64 / 128 parts 50.2 / 46.3 / 53.1; 16 sequences of 1000 own keys, 2 kv heads:
+// 1 / 2 / 4 / 8 parts 16.7 / 13.7 / 11.8 / 11.1).
 void prefix_plan(PrefixArgs& a) {
-  const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), want = 2 * device_cus();
-  const int64_t rows = a.B * grp;
+  const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), cus = device_cus(), rows = a.B * grp;
   a.rblocks = (int)cdiv(rows, rows <= 32 ? 32 : 128);
-  if ((int64_t)a.P + a.S <= 1024) {
+  if ((int64_t)a.P + a.S <= 512 && a.B * hb * a.nkv <= cus) {
     a.np = a.no = 0;
     a.pkeys = a.okeys = 0;
     return;
   }
-  const int64_t np = std::max<int64_t>(1, std::min(want / (a.rblocks * a.nkv), cdiv(a.P, 256)));
-  const int64_t no = std::max<int64_t>(1, std::min(want / (a.B * hb * a.nkv), cdiv(a.S, 128)));
+  const int64_t np = std::max<int64_t>(1, std::min((rows <= 32 ? cus : 2 * cus) / (a.rblocks * a.nkv), cdiv(a.P, 256)));
+  const int64_t no = std::max<int64_t>(1, std::min(2 * cus / (a.B * hb * a.nkv), cdiv(a.S, 128)));
   a.pkeys = (int)(cdiv(cdiv(a.P, np), 64) * 64);
   a.okeys = (int)(cdiv(cdiv(a.S, no), 32) * 32);
   a.np = a.P ? (int)cdiv(a.P, a.pkeys) : 0;
