@@ -60,6 +60,28 @@ def test_causal_many_rows(gpu, lens, h, kv, d, dtype):
     _within(lm.attention_causal(q, k, v, starts), causal_reference(q, k, v, lens, d ** -0.5))
 
 
+@pytest.mark.parametrize("lens,h,kv,d,dtype", [([1600], 16, 8, 128, "bf16"), ([1057, 1300], 12, 12, 64, "f16"), ([1100], 28, 28, 72, "bf16"),
+                                               ([2049, 1], 16, 8, 64, "bf16"), ([4000], 1, 1, 128, "f16"), ([7000], 7, 1, 64, "bf16")])
+def test_causal_long_rows(gpu, lens, h, kv, d, dtype):
+    """Few long sequences: keys shared out between two groups of waves."""
+    q, k, v, starts = causal_case(lens, h, kv, d, dtype, seed=4, dev=gpu)
+    _within(lm.attention_causal(q, k, v, starts), causal_reference(q, k, v, lens, d ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_causal_not_finite_long_rows(gpu, dtype):
+    """As test_causal_not_finite, where two groups of waves share out the keys."""
+    q, k, v, starts = causal_case([1600], 16, 8, 128, dtype, seed=9, dev=gpu)
+    want = lm.attention_causal(q, k, v, starts)
+    for at, value in ((1500, math.nan), (1599, math.inf), (70, math.nan)):
+        v2 = v.clone()
+        v2[at, 2, 9] = value
+        got = lm.attention_causal(q, k, v2, starts)
+        assert torch.equal(got[:at], want[:at])
+        assert torch.equal(got[at:, :4], want[at:, :4]) and torch.equal(got[at:, 6:], want[at:, 6:])
+        assert not bool(got[at:, 4:6, 9].isfinite().any())
+
+
 @pytest.mark.parametrize("t", [100, 2100])
 def test_causal_strides(gpu, t):
     """Views of a fused projection, heads outermost, an expanded head, unaligned and reversed-stride layouts."""

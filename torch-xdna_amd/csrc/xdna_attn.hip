@@ -317,14 +317,18 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
 // an LDS array each (K, then V), so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way
 // while tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
 // go by one copy of the masked one.
-template <int DT, int D, bool CAUSAL, class Store>
+// KG == 2: eight waves, each group G of four with every other tile in LDS of its own; group 1 leaves its sums there, and group 0
+// joins them.
+template <int DT, int D, bool CAUSAL, int KG, int G, class Store>
 __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Keys& ks, int d, const i32x4 (&qf)[D / 16], const Seen& seen, bool idle, float c,
-                                            Store&& store) {
+                                            Store&& store, float* ml = nullptr, const int8_t* other0 = nullptr,
+                                            const int8_t* other1 = nullptr) {
   constexpr int QW = 4, KT = 64, RB = 2 * D, KB = KT * RB, DB = D / 32;
   constexpr int CH = D / 8, RPL = 64 / CH, NI = KB / 1024 / QW;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (int)cdiv(ks.n, KT);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % QW;
+  const int tiles = (int)cdiv(cdiv(ks.n, KT), KG);      // of a group; tile t of group G starts at key (t KG + G) KT
+  auto first_key = [](int t) { return (t * KG + G) * KT; };
   int8_t *const k0_ = lds0, *const v0_ = lds0 + KB, *const k1_ = lds1, *const v1_ = lds1 + KB;
   // this lane's share of load j: row (4 NI wave + j) RPL + lane / CH of the tile, chunk lane % CH of its LDS row. V's chunk
   // is the same for every j (a multiple of 4 rows apart).
@@ -337,9 +341,9 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
     vo[j] = vc < 2u * d ? (uint32_t)r * (uint32_t)ks.vp + vc : OOB;
   }
   auto load = [&](int tile, int8_t* kd, int8_t* vd) {
-    const int left = min(ks.n - tile * KT, KT) - 1;           // below 0: nothing is read
-    const auto kr = make_rsrc(ks.k + (int64_t)tile * KT * ks.kp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.kp + 2u * d);
-    const auto vr = make_rsrc(ks.v + (int64_t)tile * KT * ks.vp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.vp + 2u * d);
+    const int left = min(ks.n - first_key(tile), KT) - 1;     // below 0: nothing is read
+    const auto kr = make_rsrc(ks.k + (int64_t)first_key(tile) * ks.kp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.kp + 2u * d);
+    const auto vr = make_rsrc(ks.v + (int64_t)first_key(tile) * ks.vp, left < 0 ? 0u : (uint32_t)left * (uint32_t)ks.vp + 2u * d);
 #pragma unroll
     for (int j = 0; j < NI; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void)(kd + ((wave * NI + j) << 10)), 16, (int)ko[j], 0, 0, 0);
@@ -460,7 +464,7 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
   auto tile_part = [&](const int8_t* kt, const int8_t* vt, int tile) {
 #pragma unroll 1
     for (int b = 0; b < 2; ++b) {
-      const int first = tile * KT + 32 * b;
+      const int first = first_key(tile) + 32 * b;
       const int8_t* const vb = vt + b * 32 * RB;
       auto visible = [&](int key) { return CAUSAL ? key >= seen.lo && key <= seen.hi : key < ks.n; };
       f32x16a sc = scores(kt + b * 32 * RB);
@@ -498,7 +502,7 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
     for (int t = from; t < to; ++t) {
       const bool odd = t & 1;
       arrive(t, odd ? k0_ : k1_, odd ? v0_ : v1_);
-      const int k0 = t * KT;
+      const int k0 = first_key(t);
       if (CAUSAL && (k0 > seen.last || k0 + KT - 1 < seen.first)) continue;      // no row of this wave sees a key of it
       tile_part(odd ? k1_ : k0_, odd ? v1_ : v0_, t);
     }
@@ -509,10 +513,15 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
   if (idle) {
     for (int t = 0; t < tiles; ++t) arrive(t, t & 1 ? k0_ : k1_, t & 1 ? v0_ : v1_);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (KG == 2) {
+      __syncthreads();
+      __syncthreads();
+    }
     return;
   }
-  const int all0 = CAUSAL ? (int)(cdiv(seen.from_all, 2 * KT) * 2) : 0;
-  const int all1 = max(all0, (CAUSAL ? (seen.to_all + 1) / (2 * KT) : ks.n / (2 * KT)) * 2);
+  const int from = CAUSAL ? max(0, (int)cdiv((int)cdiv(seen.from_all, KT) - G, KG)) : 0;
+  const int to = max(0, (int)cdiv((CAUSAL ? seen.to_all + 1 : ks.n) / KT - G, KG));
+  const int all0 = (from + 1) & ~1, all1 = max(all0, to & ~1);
   masked(0, min(all0, tiles));
   for (int t = all0; t < all1; t += 2) {
     arrive(t, k1_, v1_);
@@ -523,11 +532,39 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
   masked(min(all1, tiles), tiles);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the load past the end: LDS may be another's soon
   l = pair_sum(l);
+  if constexpr (KG == 1) {
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      store(4 * db + g, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]}, m, l);
+      for (int g = 0; g < 4; ++g)
+        store(4 * db + g, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]}, m, l);
+  } else if constexpr (G == 1) {
+    __syncthreads();
+    float* const at = reinterpret_cast<float*>((wave < 2 ? lds0 : lds1) + (wave & 1) * (128 * D));
+#pragma unroll
+    for (int i = 0; i < 4 * DB; ++i)
+      *reinterpret_cast<f32x4*>(at + i * 256 + lane * 4) =
+          f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+    ml[wave * 64 + lane] = m;
+    ml[(4 + wave) * 64 + lane] = l;
+    __syncthreads();
+  } else {
+    __syncthreads();
+    __syncthreads();
+    const float* const at = reinterpret_cast<const float*>((wave < 2 ? other0 : other1) + (wave & 1) * (128 * D));
+    const float m1 = ml[wave * 64 + lane], l1 = ml[(4 + wave) * 64 + lane], mt = fmaxf(m, m1);
+    const float w0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mt) * c);
+    const float w1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m1 - mt) * c);
+    const float lt = (m == -INFINITY ? l : l * w0) + (m1 == -INFINITY ? l1 : l1 * w1);     // 0 or NaN where there is no maximum
+#pragma unroll
+    for (int i = 0; i < 4 * DB; ++i) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(at + i * 256 + lane * 4);
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = o[i / 4][4 * (i % 4) + r] * w0 + x[r] * w1;
+      store(i, v, mt, lt);
+    }
+  }
 }
 
 // A row's q in the MFMA's order, its sign bits flipped where the scale is negative, zeros past the head's dims.
@@ -583,10 +620,10 @@ struct CausalArgs {
 // Tiles of 32 QW rows over all tokens, whatever sequences they fall into: a tile's keys run from the first token of
 // its first row's sequence to its last row's token, and each row's mask does the rest. Last tiles first: in
 // a long prompt they are the longest.
-// WIDE: 128 rows by attend_wide, else 32 rows whose keys four waves share out.
-template <int DT, int D, bool WIDE>
-__global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
-  constexpr int QW = WIDE ? 4 : 1;
+// KG: groups of waves in the wide form (128 rows by attend_wide); 0: 32 rows whose keys four waves share out.
+template <int DT, int D, int KG>
+__global__ __launch_bounds__(KG == 2 ? 512 : 256, KG == 2 ? 1 : 2) void causal_kernel(CausalArgs a) {
+  constexpr int QW = KG ? 4 : 1;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.nh / a.nkv, nrows = a.T * grp;
@@ -622,10 +659,19 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
     const int dim = 8 * chunk + 4 * half;
     if (mine && dim < a.d) store4<DT>(orow + dim, o, l == 0.0f ? 0.0f : 1.0f / l);
   };
-  if constexpr (WIDE) {
+  const bool idle = row0 + 32 * (wave % QW) >= nrows;
+  if constexpr (KG == 1) {
     __shared__ __attribute__((aligned(1024))) int8_t lds0[256 * D];
     __shared__ __attribute__((aligned(1024))) int8_t lds1[256 * D];
-    attend_wide<DT, D, true>(lds0, lds1, ks, a.d, qf, seen, row0 + 32 * wave >= nrows, a.c, store);
+    attend_wide<DT, D, true, 1, 0>(lds0, lds1, ks, a.d, qf, seen, idle, a.c, store);
+  } else if constexpr (KG == 2) {
+    __shared__ __attribute__((aligned(1024))) int8_t lds0[256 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t lds1[256 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t lds2[256 * D];
+    __shared__ __attribute__((aligned(1024))) int8_t lds3[256 * D];
+    __shared__ float ml[2 * 4 * 64];
+    if (wave < 4) attend_wide<DT, D, true, 2, 0>(lds0, lds1, ks, a.d, qf, seen, idle, a.c, store, ml, lds2, lds3);
+    else attend_wide<DT, D, true, 2, 1>(lds2, lds3, ks, a.d, qf, seen, idle, a.c, store, ml);
   } else {
     __shared__ __attribute__((aligned(1024))) int8_t kl[4 * 64 * D];
     __shared__ __attribute__((aligned(1024))) int8_t vl[4 * 64 * D];
@@ -634,13 +680,20 @@ __global__ __launch_bounds__(256, 2) void causal_kernel(CausalArgs a) {
   }
 }
 
+// 128 rows to a workgroup once that makes three for four CUs, below it 32 rows with their keys shared out (1024 tokens, 16 / 8
+// heads of 128: 21.8 us shared out, 31.3 with 128 rows; 2048 tokens 49.9 / 52.6). Up to two workgroups a CU two groups of waves share out
+// the keys of the 128 rows, where the sequences are long (the host knows their mean): a CU's workgroups all
+// run at once then, and the longest row's chain of tiles is what takes the time (2048 tokens 44.3 us against 52.6 with one group, 4096
+// 97.0 / 111.6; 8192 323 / 318; forty of 100 33.6 / 24.4; 4096 / 1500 / 700, 12 heads of 64: 69.5 / 70.0).
 template <int DT, int D>
 int causal_go(const CausalArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.T * (a.nh / a.nkv);
-  const bool wide = 4 * cdiv(rows, 128) * a.nkv >= 3 * (int64_t)device_cus();
-  const int64_t grid = cdiv(rows, wide ? 128 : 32) * a.nkv;
-  if (wide) causal_kernel<DT, D, true><<<(unsigned)grid, 256, 0, st>>>(a);
-  else causal_kernel<DT, D, false><<<(unsigned)grid, 256, 0, st>>>(a);
+  const int64_t rows = (int64_t)a.T * (a.nh / a.nkv), cus = device_cus();
+  const int64_t wgs = cdiv(rows, 128) * a.nkv;
+  const int kg = 4 * wgs < 3 * cus ? 0 : wgs <= 2 * cus && a.T >= 1024ll * (a.nstarts - 1) ? 2 : 1;
+  const unsigned grid = (unsigned)(kg ? wgs : cdiv(rows, 32) * a.nkv);
+  if (kg == 0) causal_kernel<DT, D, 0><<<grid, 256, 0, st>>>(a);
+  else if (kg == 1) causal_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a);
+  else causal_kernel<DT, D, 2><<<grid, 512, 0, st>>>(a);
   return launch_status("attention_causal");
 }
 
@@ -707,7 +760,7 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
     ks.n = max(0, min(a.pkeys, a.P - k0));
     const auto out = write(part, (int64_t)b * a.nh + head, want < nrows);
     if constexpr (WIDE) {
-      attend_wide<DT, D, false>(lds_k, lds_v, ks, a.d, qf, seen, rb * 128 + 32 * wave >= nrows, a.c, out);
+      attend_wide<DT, D, false, 1, 0>(lds_k, lds_v, ks, a.d, qf, seen, rb * 128 + 32 * wave >= nrows, a.c, out);
     } else {
       attend_split<DT, D, KW, false>(lds_k, lds_v, ml, ks, a.d, qf, seen, a.c, out);
     }
