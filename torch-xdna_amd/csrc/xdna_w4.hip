@@ -555,7 +555,13 @@ __global__ __launch_bounds__(256) void w4_join_kernel(const float* __restrict__ 
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= MN) return;
   float v = 0.0f;
-  for (int p = 0; p < parts; ++p) v += part[p * MN + i];
+  for (int p0 = 0; p0 < parts; p0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = part[min(p0 + j, parts - 1) * MN + i];      // all on their way at once
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v += p0 + j < parts ? x[j] : 0.0f;
+  }
   if (bias) v += load_any(bias, i % N, bias_dt);
   store_from_f32<DT>(y, i, v);
 }
