@@ -726,8 +726,19 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.nh / a.nkv;
-  const int kvh = blockIdx.x % a.nkv;
-  const int rest = blockIdx.x / a.nkv;
+  // The blocks of rows that read the same keys run on one XCD (workgroups go round the eight), next to each other in time, so that its L2 has
+  // the keys for all but the first: items (part, kv head) in eights, their blocks 8 apart.
+  const int items = a.np * a.nkv, pre = items * a.rblocks;
+  int b0 = blockIdx.x, rb = 0;
+  if (b0 < pre) {
+    const int eights = items / 8 * 8, whole = eights * a.rblocks, left = items - eights;
+    const int i = b0 < whole ? b0 % 8 : (b0 - whole) % left, j = b0 < whole ? b0 / 8 : (b0 - whole) / left;
+    rb = j % a.rblocks;
+    b0 = (b0 < whole ? j / a.rblocks * 8 : eights) + i;
+  } else {
+    b0 -= pre;
+  }
+  const int kvh = b0 % a.nkv, rest = b0 / a.nkv;
   Keys ks;
   ks.kp = 2 * a.kpt;
   ks.vp = 2 * a.vpt;
@@ -749,8 +760,8 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
       }
     };
   };
-  if (rest < a.rblocks * a.np) {
-    const int rb = rest % a.rblocks, part = rest / a.rblocks, nrows = a.B * grp;
+  if ((int)blockIdx.x < pre) {
+    const int part = rest, nrows = a.B * grp;
     const int want = rb * (32 * QW) + 32 * (wave % QW) + (lane & 31), idx = min(want, nrows - 1);
     const int b = idx / grp, head = kvh * grp + idx - b * grp;
     load_q<D>(qf, a.q + b * a.qb + head * a.qh, half, a.d, a.sign);
@@ -767,7 +778,7 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
     return;
   }
   // rows: the q heads of one (sequence, kv head), 32 at a time
-  const int hb = (grp + 31) / 32, own = rest - a.rblocks * a.np, parts = max(1, a.no);
+  const int hb = (grp + 31) / 32, own = rest, parts = max(1, a.no);
   const int b = own / (hb * parts), at = own - b * (hb * parts), part = at / hb, want = (at - part * hb) * 32 + (lane & 31);
   const int head = kvh * grp + min(want, grp - 1);
   load_q<D>(qf, a.q + b * a.qb + head * a.qh, half, a.d, a.sign);
