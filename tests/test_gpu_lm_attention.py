@@ -244,3 +244,21 @@ def test_prefix_scales_stream_and_graph(gpu, p, scale):
     want = lm.attention_prefix(*args, scale)
     _within(want, prefix_reference(*args, scale))
     _replays(lambda: lm.attention_prefix(*args, scale), want)
+
+
+def test_prefix_offsets_past_32_bits(gpu):
+    """Caches whose tokens, and whose sequences, lie so far apart that byte offsets pass 32 bits."""
+    p, s, kv, d = 700, 300, 2, 64
+    q, kp, vp, kc, vc, lens = prefix_case(2, p, s, 4, kv, d, "bf16", seed=16, dev=gpu)
+    want = lm.attention_prefix(q, kp, vp, kc, vc, lens)
+    far = torch.empty(p, 1 << 22, dtype=q.dtype, device=gpu)                      # 8 MB from token to token: 5.9 GB
+    kf, vf = far[:, :kv * d].view(p, kv, d), far[:, kv * d:2 * kv * d].view(p, kv, d)
+    kf.copy_(kp), vf.copy_(vp)
+    apart = far.view(-1)[5 << 20:].as_strided((2, s, kv, d), ((p // 2) << 22, 1024, 256, 1))     # 2.9 GB from sequence to sequence
+    apart.copy_(kc)
+    kf.copy_(kp), vf.copy_(vp)
+    assert torch.equal(lm.attention_prefix(q, kf, vf, apart, vc, lens), want)    # the views do not overlap
+    assert torch.equal(lm.attention_prefix(q, kf, vf, kc, vc, lens), want)
+    c = causal_case([p - 200, 200], 4, kv, d, "bf16", seed=17, dev=gpu)
+    kf.copy_(c[1])
+    assert torch.equal(lm.attention_causal(c[0], kf, c[2], c[3]), lm.attention_causal(*c))

@@ -14,8 +14,9 @@
 // share their loads. MFMA 32x32x16 (srcA = X, srcB = Y) gives lane l row l % 32 of Y and, in element 4 g + r, row
 // 8 g + 4 (l / 32) + r of X; lane l supplies values 8 (l / 32) .. + 7 of the 16-deep step of its operand's row l % 32.
 // S = K Q^T leaves in a lane 16 of 32 keys of its row, and these are, 8 at a time, what O^T = V^T P^T takes from that
-// lane if step u's k slot 8 h + i stands for key 16 u + 8 (i / 4) + 4 h + i % 4. V keeps its rows of one key each: the transposed
-// LDS read (16 lanes, 4 rows of 16 values: lane i gets column i) makes the V^T fragments in that order.
+// lane if step u's k slot 8 h + i stands for key 16 u + 8 (i / 4) + 4 h + i % 4. V keeps its rows of one key each:
+// the transposed LDS read (16 lanes, 4 rows of 16 values: lane i gets column i) makes the V^T fragments in that
+// order.
 //
 // Tiles of KT keys come into LDS by the DMA form of the buffer load, whose bounds check fills keys past the end, and
 // dims past the head's, with zeros. A 16-byte chunk's place in its row is XORed with the row so that the lanes that
@@ -164,11 +165,12 @@ __device__ __forceinline__ void add_not_finite(f32x16a (&o)[D / 32], const float
   }
 }
 
-// Attention of 32 rows by KW waves: wave w has the tiles w, w + KW, ... of 32 keys, in LDS of its own (kl_, vl_: KW tiles of
-// K, and of V, each an array, so that the compiler knows which loads a read has to wait for), and the waves meet in LDS at
-// the end (meet: KW x 32 x D float32, which may lie over the tiles; ml: 2 KW x 64). No barriers before that: K of a wave's next
-// tile loads once its scores are done, V after its products. store(chunk, o, m, l) receives dims 8 (chunk % 4) + 32 (chunk / 4) +
-// 4 (lane / 32) .. + 3 of the lane's row: the sum of p v, the maximum and the sum of p.
+// Attention of 32 rows by KW waves: wave w has the tiles w, w + KW, ... of 32 keys, in LDS of its own (kl_, vl_: KW
+// tiles of K, and of V, each an array, so that the compiler knows which loads a read has to wait for), and the waves
+// meet in LDS at the end (meet: KW x 32 x D float32, which may lie over the tiles; ml: 2 KW x 64). No barriers before
+// that: K of a wave's next tile loads once its scores are done, V after its products. store(chunk, o, m, l) receives
+// dims 8 (chunk % 4) + 32 (chunk / 4) + 4 (lane / 32) .. + 3 of the lane's row: the sum of p v, the maximum and the
+// sum of p.
 template <int DT, int D, int KW, bool CAUSAL, class Store>
 __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml, const Keys& ks, int d, const i32x4 (&qf)[D / 16],
                                              const Seen& seen, float c, Store&& store) {
@@ -177,8 +179,8 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int base = wave * KB;
   const int t1 = (int)cdiv(ks.n, KT), tiles = t1 + (int)cdiv(ks.n2, KT);
-  // load j: rows j RPL + lane / CH, chunk lane % CH of the LDS row; a tile past the last loads nothing (the bounds check), so that
-  // the loads under way are always as many
+  // load j: rows j RPL + lane / CH, chunk lane % CH of the LDS row; a tile past the last loads nothing (the bounds
+  // check), so that the loads under way are always as many
   auto load = [&](bool v, int tile) {
     const bool two = tile >= t1;
     const int k0 = (two ? tile - t1 : tile) * KT, left = min((two ? ks.n2 : ks.n) - k0, KT) - 1;
@@ -277,7 +279,8 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
     __builtin_amdgcn_sched_barrier(0);
   }
   l = pair_sum(l);
-  // each wave leaves its m, l and O where its tiles were (half of O in K's place, half in V's); wave w then joins chunks w, w + KW, ..
+  // each wave leaves its m, l and O where its tiles were (half of O in K's place, half in V's); wave w then joins
+  // chunks w, w + KW, ..
   constexpr int OB = 32 * D * 2, NC = 4 * DB;      // bytes of half a wave's O, chunks
   static_assert(OB == KB, "half of O takes a tile of K");
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -313,12 +316,19 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
   }
 }
 
-// Four waves of 32 rows that share every tile of 64 keys: the form for many rows. Waves without rows (idle) only load. Two tiles have
-// an LDS array each (K, then V), so that the compiler knows which loads a read has to wait for: tile t + 1 is on its way
-// while tile t is used. Tiles that all rows see whole take the short path (tile_all); the others, at the ends of a prompt's keys,
-// go by one copy of the masked one.
-// KG == 2: eight waves, each group G of four with every other tile in LDS of its own; group 1 leaves its sums there, and group 0
-// joins them.
+// Four waves of 32 rows that share every tile of 64 keys: the form for many rows. Waves without rows (idle) only
+// load. Two tiles have an LDS array each (K, then V), so that the compiler knows which loads a read has to wait for:
+// tile t + 1 is on its way while tile t is used. Tiles that all rows see whole take the short path (tile_all); the
+// others, at the ends of a prompt's keys, go by one copy of the masked one.
+//
+// What bounds it: a tile is 32 MFMAs (1024 cycles; heads of 64: 512) and about 130 vector instructions, 32 exps among
+// them, for a wave. Heads of 128: the card's power (1 x 16384, 16 / 8 heads: 1020 us, 1080 TFLOP/s, MFMA busy 57% at
+// 1.76 GHz); heads of 64 the vector units (8192, 16 / 8 heads: 199 us, 690 TFLOP/s). The maximum follows once a tile;
+// l sums the p that are rounded, two at a time by a dot product with ones. With the masked tiles in the same loop the
+// compiler kept two sets of O (64 moves a tile: 1160 us).
+//
+// KG == 2: eight waves, each group G of four with every other tile in LDS of its own; group 1 leaves its sums there,
+// and group 0 joins them.
 template <int DT, int D, bool CAUSAL, int KG, int G, class Store>
 __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Keys& ks, int d, const i32x4 (&qf)[D / 16], const Seen& seen, bool idle, float c,
                                             Store&& store, float* ml = nullptr, const int8_t* other0 = nullptr,
@@ -330,8 +340,8 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
   const int tiles = (int)cdiv(cdiv(ks.n, KT), KG);      // of a group; tile t of group G starts at key (t KG + G) KT
   auto first_key = [](int t) { return (t * KG + G) * KT; };
   int8_t *const k0_ = lds0, *const v0_ = lds0 + KB, *const k1_ = lds1, *const v1_ = lds1 + KB;
-  // this lane's share of load j: row (4 NI wave + j) RPL + lane / CH of the tile, chunk lane % CH of its LDS row. V's chunk
-  // is the same for every j (a multiple of 4 rows apart).
+  // this lane's share of load j: row (4 NI wave + j) RPL + lane / CH of the tile, chunk lane % CH of its LDS row. V's
+  // chunk is the same for every j (a multiple of 4 rows apart).
   uint32_t ko[NI], vo[NI];
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
@@ -355,8 +365,8 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16a{};
   float m = -INFINITY, l = 0.0f;
-  // offsets of the lane's K fragments in their block of 32 keys, and of its V fragments'; kept out of the compiler's sight, which
-  // would hold a set of them for each array
+  // offsets of the lane's K fragments in their block of 32 keys, and of its V fragments'; kept out of the compiler's
+  // sight, which would hold a set of them for each array
   uint32_t koff[D / 16], voff[DB];
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
@@ -413,8 +423,8 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
       l = dot_ones<DT>(w, l);
     }
   };
-  // The reads of K run six ahead of their products, those of V's first half go out before the softmax and the second half's under
-  // the first half's products: with two waves a SIMD little else hides a trip to LDS.
+  // The reads of K run six ahead of their products, those of V's first half go out before the softmax and the second
+  // half's under the first half's products: with two waves a SIMD little else hides a trip to LDS.
   auto tile_all = [&](const int8_t* kt, const int8_t* vt) {
     f32x16a sc[2];
     i32x4 pf[2][2], vf[2][2][DB];
@@ -507,8 +517,8 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
       tile_part(odd ? k1_ : k0_, odd ? v1_ : v0_, t);
     }
   };
-  // The tiles that every row of this wave sees whole are a run of them; its pairs of an even tile and the next take the short
-  // path. Waves may disagree on it: each passes one barrier a tile in any case.
+  // The tiles that every row of this wave sees whole are a run of them; its pairs of an even tile and the next take
+  // the short path. Waves may disagree on it: each passes one barrier a tile in any case.
   if (tiles > 0) load(0, k0_, v0_);
   if (idle) {
     for (int t = 0; t < tiles; ++t) arrive(t, t & 1 ? k0_ : k1_, t & 1 ? v0_ : v1_);
@@ -680,11 +690,12 @@ __global__ __launch_bounds__(KG == 2 ? 512 : 256, KG == 2 ? 1 : 2) void causal_k
   }
 }
 
-// 128 rows to a workgroup once that makes three for four CUs, below it 32 rows with their keys shared out (1024 tokens, 16 / 8
-// heads of 128: 21.8 us shared out, 31.3 with 128 rows; 2048 tokens 49.9 / 52.6). Up to two workgroups a CU two groups of waves share out
-// the keys of the 128 rows, where the sequences are long (the host knows their mean): a CU's workgroups all
-// run at once then, and the longest row's chain of tiles is what takes the time (2048 tokens 44.3 us against 52.6 with one group, 4096
-// 97.0 / 111.6; 8192 323 / 318; forty of 100 33.6 / 24.4; 4096 / 1500 / 700, 12 heads of 64: 69.5 / 70.0).
+// 128 rows to a workgroup once that makes three for four CUs, below it 32 rows with their keys shared out (1024
+// tokens, 16 / 8 heads of 128: 21.8 us shared out, 31.3 with 128 rows; 2048 tokens 49.9 / 52.6). Up to two workgroups
+// a CU two groups of waves share out the keys of the 128 rows, where the sequences are long (the host knows their
+// mean): a CU's workgroups all run at once then, and the longest row's chain of tiles is what takes the time (2048
+// tokens 44.3 us against 52.6 with one group, 4096 97.0 / 111.6; 8192 323 / 318; forty of 100 33.6 / 24.4; 4096 /
+// 1500 / 700, 12 heads of 64: 69.5 / 70.0).
 template <int DT, int D>
 int causal_go(const CausalArgs& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.T * (a.nh / a.nkv), cus = device_cus();
@@ -712,9 +723,12 @@ struct PrefixArgs {
   uint16_t* out;
 };
 
-// Workgroups 0 .. nkv rblocks np - 1 take a part of the prefix for the rows (sequence, q head) of a kv head, 32 at a time, or
-// 128 (WIDE); the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a workgroup
-// takes all the keys of its (sequence, kv head) and writes the output itself. KW: waves that share out keys.
+// Workgroups 0 .. nkv rblocks np - 1 take a part of the prefix for the rows (sequence, q head) of a kv head, 32 at a
+// time, or 128 (WIDE); the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a
+// workgroup takes all the keys of its (sequence, kv head) and writes the output itself. KW: waves that share out
+// keys. Measured, with the join: 48 rows of 2 / 1 heads of 128 on 8 kv heads over 4096 shared keys and up to 700 own
+// ones 25.6 us (86 MB, 3.4 TB/s); 24 rows of 8 / 1 heads of 64 on 4 over 100000 43 us (107 MB, 2.5 TB/s), bound by
+// the softmax's vector instructions and by six waves on four SIMDs.
 template <int DT, int D, bool WIDE, int KW>
 __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
   static_assert(!WIDE || KW == 4, "four waves in the wide form");
@@ -726,8 +740,8 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.nh / a.nkv;
-  // The blocks of rows that read the same keys run on one XCD (workgroups go round the eight), next to each other in time, so that its L2 has
-  // the keys for all but the first: items (part, kv head) in eights, their blocks 8 apart.
+  // The blocks of rows that read the same keys run on one XCD (workgroups go round the eight), next to each other in
+  // time, so that its L2 has the keys for all but the first: items (part, kv head) in eights, their blocks 8 apart.
   const int items = a.np * a.nkv, pre = items * a.rblocks;
   int b0 = blockIdx.x, rb = 0;
   if (b0 < pre) {
@@ -807,8 +821,8 @@ __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
                                  write(all ? -1 : a.np + part, (int64_t)b * a.nh + head, want < grp));
 }
 
-// The parts of a row joined: a workgroup per row, wave w the parts w, w + 4, .., then the waves in their order; lane l dims
-// 2 l, 2 l + 1.
+// The parts of a row joined: a workgroup per row, wave w the parts w, w + 4, .., then the waves in their order; lane
+// l dims 2 l, 2 l + 1.
 template <int DT>
 __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restrict__ po, const float* __restrict__ pml,
                                                           int parts, int64_t rows, int d, float c,
@@ -846,12 +860,12 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
   *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack2<DT>(x * inv, y * inv);
 }
 
-// How a call is split. Up to 512 keys for few sequences: a workgroup of eight waves for each (sequence, kv head), one launch and
-// nothing to join (4 sequences, 8 kv heads, 264 + 64 keys 9.3 us, in parts 10.7; 64 sequences, 500 + 100: 20.5 / 16.5). Else the
-// prefix in parts that make a workgroup a CU in the 32-row form, two in the 128-row one, none under 256 keys, and own keys
-// in parts of 128 at least as far as two workgroups a CU take them (1 sequence, 32768 keys, 8 kv heads: 16 / 32 / 64 parts 29.1 /
-// 28.0 / 30.7 us; 24 x 32 heads over 100000: 32 / 64 / 128 parts 50.2 / 46.3 / 53.1; 16 sequences of 1000 own keys, 2 kv heads:
-// 1 / 2 / 4 / 8 parts 16.7 / 13.7 / 11.8 / 11.1).
+// How a call is split. Up to 512 keys for few sequences: a workgroup of eight waves for each (sequence, kv head), one
+// launch and nothing to join (4 sequences, 8 kv heads, 264 + 64 keys 9.3 us, in parts 10.7; 64 sequences, 500 + 100:
+// 20.5 / 16.5). Else the prefix in parts that make a workgroup a CU in the 32-row form, two in the 128-row one, none
+// under 256 keys, and own keys in parts of 128 at least as far as two workgroups a CU take them (1 sequence, 32768
+// keys, 8 kv heads: 16 / 32 / 64 parts 29.1 / 28.0 / 30.7 us; 24 x 32 heads over 100000: 32 / 64 / 128 parts 50.2 /
+// 46.3 / 53.1; 16 sequences of 1000 own keys, 2 kv heads: 1 / 2 / 4 / 8 parts 16.7 / 13.7 / 11.8 / 11.1).
 void prefix_plan(PrefixArgs& a) {
   const int64_t grp = a.nh / a.nkv, hb = cdiv(grp, 32), cus = device_cus(), rows = a.B * grp;
   a.rblocks = (int)cdiv(rows, rows <= 32 ? 32 : 128);

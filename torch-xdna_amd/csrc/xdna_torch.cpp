@@ -1,10 +1,10 @@
-// The language model operators' GPU kernels of torch.ops.xdna.*, from the dispatcher to the library's C ABI without a trip
-// through Python: the checks, the output, the workspace, the stream. A small call is all host time: one row through 1024 x
-// 4096 4-bit weights takes 4.5 us on the GPU, and took 15 to issue from Python.
+// The language model operators' GPU kernels of torch.ops.xdna.*, from the dispatcher to the library's C ABI without a
+// trip through Python: the checks, the output, the workspace, the stream. A small call is all host time: one row
+// through 1024 x 4096 4-bit weights takes 4.5 us on the GPU, and took 15 to issue from Python.
 //
-// Registered for CUDA (the work) and AutogradCUDA (nothing but the dispatch below it; outputs of inputs that need a gradient
-// get a node that raises when it is asked for). Python's registrations of the ops give them their schemas, their host
-// kernels and their shapes under fake tensors.
+// Registered for CUDA (the work) and AutogradCUDA (nothing but the dispatch below it; outputs of inputs that need a
+// gradient get a node that raises when it is asked for). Python's registrations of the ops give them their schemas,
+// their host kernels and their shapes under fake tensors.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -142,9 +142,9 @@ double attention_args(const char* name, const Tensor& q, std::initializer_list<c
   return scale ? *scale : 1.0 / std::sqrt((double)d);
 }
 
-// t [.., heads, d] as the library reads it, and its strides but the last's (of dims of one, any will do): itself where the
-// last dim is dense, it starts on 16 bytes, no token's values overlap the next one's and the strides are multiples of 8
-// that fit the kernels' offsets; else a copy.
+// t [.., heads, d] as the library reads it, and its strides but the last's (of dims of one, any will do): itself
+// where the last dim is dense, it starts on 16 bytes, no token's values overlap the next one's and the strides are
+// multiples of 8 that fit the kernels' offsets; else a copy.
 Tensor heads(Tensor t, int64_t* st) {
   const int64_t n = t.dim() - 1, d = t.size(n);
   for (int pass = 0; pass < 2; ++pass) {

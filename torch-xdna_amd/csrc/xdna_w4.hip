@@ -7,16 +7,17 @@
 // The weights are whole numbers until their group's sum is done, so nothing is rounded before the float32 sums: x is
 // multiplied by q - z (or by 128 + q, below), the float32 sum takes the group's scale as one fma.
 //
-// Unpacking: byte p of a word and of the word shifted by 4, put side by side by one byte permute, have q[2p] and q[2p + 1]
-// in the low bits of their halves; masked and with the bits of 128 (bfloat16) or 1024 (float16) ORed in they are two
-// floats of value 128 + q or 1024 + q. float16 subtracts 1024 + z at once (exact, packed). bfloat16 has no packed
-// add here: the sum over 128 + q stays, and (128 + z) times the group's sum of x is taken off in float32. The sums are
-// then up to 30 times the result's own size, 2^-19 in the float32 sums against the output's 2^-9. Where x is not
-// finite that difference is not what the formula says (inf - inf), so such sums are formed again, value by value. float32
-// x meets weights converted one by one, q - z; for the matrix units it is cut into three bfloat16 numbers that add up
-// to it exactly.
+// Unpacking: byte p of a word and of the word shifted by 4, put side by side by one byte permute, have q[2p] and q[2p
+// + 1] in the low bits of their halves; masked and with the bits of 128 (bfloat16) or 1024 (float16) ORed in they are
+// two floats of value 128 + q or 1024 + q. float16 subtracts 1024 + z at once (exact, packed). bfloat16 has no packed
+// add here: the sum over 128 + q stays, and (128 + z) times the group's sum of x is taken off in float32. The sums
+// are then up to 30 times the result's own size, 2^-19 in the float32 sums against the output's 2^-9. Where x is not
+// finite that difference is not what the formula says (inf - inf), so such sums are formed again, value by value.
+// float32 x meets weights converted one by one, q - z; for the matrix units it is cut into three bfloat16 numbers
+// that add up to it exactly.
 //
-// One row (a decode step), and up to four where the weights are few, are dot products on the vector units: w4_row_kernel. More go to the matrix units, x through LDS: w4_tile_kernel.
+// One row (a decode step), and up to four where the weights are few, are dot products on the vector units:
+// w4_row_kernel. More go to the matrix units, x through LDS: w4_tile_kernel.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -98,8 +99,8 @@ __device__ __forceinline__ void split3(const uint32_t (&v)[8], i32x4 (&p)[3]) {
     for (int e = 0; e < 4; ++e) p[i][e] = (int)((h[i][2 * e] >> 16) | (h[i][2 * e + 1] & 0xffff0000u));
 }
 
-// The words of a load, taken apart here and not before: the compiler would otherwise copy them to registers of their own, and
-// wait for the load, right where it is issued.
+// The words of a load, taken apart here and not before: the compiler would otherwise copy them to registers of their
+// own, and wait for the load, right where it is issued.
 __device__ __forceinline__ void words(const uint4& v, uint32_t (&w)[4]) {
   i32x4 t = {(int)v.x, (int)v.y, (int)v.z, (int)v.w};
   asm volatile("" : "+v"(t));
@@ -144,9 +145,9 @@ constexpr int W4_ROW_GROUPS = 4096;   // scales and zero points of a workgroup
 // A wave has 64 / KL columns; a lane's 16-byte load is 32 consecutive weights of one column, KL lanes side by side read
 // 16 KL bytes of it. a.per waves share a set of columns, the blocks of 32 KL weights dealt out to them; lanes meet by
 // shuffles, waves in LDS, both in a fixed order.
-// What a CU's address unit can take bounds such a kernel as much as the memory: a load costs it 16 cycles at least, however
-// little it fetches. So x, the scales and the zero points come into LDS once per workgroup, line by line, by pieces of PB
-// blocks (with a lane's own loads of them 1 x 4096 -> 14336 takes 24 us, so 15).
+// What a CU's address unit can take bounds such a kernel as much as the memory: a load costs it 16 cycles at least,
+// however little it fetches. So x, the scales and the zero points come into LDS once per workgroup, line by line, by
+// pieces of PB blocks (with a lane's own loads of them 1 x 4096 -> 14336 takes 24 us, so 15).
 template <int DT, bool S4, int KL, int R>
 __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
   constexpr int W = 8, CL = 64 / KL;                    // waves, columns of a load
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
 // scale. A lane's 16-byte load of weights is 32 consecutive ones of its column; the words change quarters so that a
 // step's four quarters are 32 consecutive k. Two tiles' x (DMA into LDS) and weights are on their way while a third is
 // used. Scales and zero points come into LDS for WIN k at a time. FL: steps (32 k each) of a group's sum
-// before its scale: 4 where G % 128 == 0, 2 where G % 64 == 0, else 1.
+// before its scale: 4 where G % 128 == 0, 2 where G % 64 == 0, else 1. Measured with the join: 40 x 14336 -> 4096 in
+// float16 23.3 us (33.6 MB), 8 x 4096 -> 14336 in bfloat16 15 us (33 MB): latency, with two workgroups a CU.
 template <int DT, bool S4, int MT, int FL>
 __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
   constexpr int W = 4;                                  // waves
@@ -382,7 +384,8 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
     xk[i] = row < rows ? k : K;
     xoff[i] = (uint32_t)((row * a.ldx + k) * esz);
   }
-  // k / G (uniform): k < 2^22 and G >= 32, so the product with the reciprocal is off by less than 2^-1 / G of a quotient's step
+  // k / G (uniform): k < 2^22 and G >= 32, so the product with the reciprocal is off by less than 2^-1 / G of a
+  // quotient's step
   const float rg = 1.0f / (float)G;
   auto group_of = [&](int k) { return (int)(((float)min(k, K - 1) + 0.5f) * rg); };
   uint4 ring[D][U];
@@ -572,14 +575,14 @@ struct W4Plan {
   int mt, parts;        // w4_tile_kernel's row blocks of 16 and split of K
 };
 
-// One row: the row kernel, but for 16-bit rows and 32 columns a CU (8192) or more (1 x 4096 -> 14336, bfloat16: row 15.2,
-// tiles 14.0 us; 1 x 512 -> 14336 6.8 / 5.9; 1 x 14336 -> 4096 11.8 / 16.5; 1 x 4096 -> 14336 in float32 12.9 / 36). Two
-// to four rows: where the weights are few (3 x 1504 -> 1001 in float32 9.3 / 14.9 us, 4 x 8192 -> 512 7.4 / 10.1, 4 x 4096 ->
-// 4096 12.4 / 10.0). Its lanes along K: 64, so that long K makes waves enough, or 16 where the columns do (4096 ->
-// 14336 in bfloat16: 15.2 with 16, 19.0 with 64; 14336 -> 4096: 25 / 11.8), and more waves along K below four a CU (14336 -> 64: one
-// wave 9.2 us, four 5.8).
-// Tiles: K in as many parts as make two workgroups a CU, none under 1024 k (40 x 14336 -> 4096: 1 / 2 / 4 / 8 / 16 parts
-// 82.1 / 45.8 / 27.9 / 24.7 / 28.3 us, of which 5 the joining).
+// One row: the row kernel, but for 16-bit rows and 32 columns a CU (8192) or more (1 x 4096 -> 14336, bfloat16: row
+// 15.2, tiles 14.0 us; 1 x 512 -> 14336 6.8 / 5.9; 1 x 14336 -> 4096 11.8 / 16.5; 1 x 4096 -> 14336 in float32 12.9 /
+// 36). Two to four rows: where the weights are few (3 x 1504 -> 1001 in float32 9.3 / 14.9 us, 4 x 8192 -> 512 7.4 /
+// 10.1, 4 x 4096 -> 4096 12.4 / 10.0). Its lanes along K: 64, so that long K makes waves enough, or 16 where the
+// columns do (4096 -> 14336 in bfloat16: 15.2 with 16, 19.0 with 64; 14336 -> 4096: 25 / 11.8), and more waves along
+// K below four a CU (14336 -> 64: one wave 9.2 us, four 5.8). Tiles: K in as many parts as make two workgroups a CU,
+// none under 1024 k (40 x 14336 -> 4096: 1 / 2 / 4 / 8 / 16 parts 82.1 / 45.8 / 27.9 / 24.7 / 28.3 us, of which 5 the
+// joining).
 W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   W4Plan p{};
   const int64_t cus = device_cus();

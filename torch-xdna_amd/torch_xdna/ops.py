@@ -240,4 +240,7 @@ if hasattr(linear, "_opoverload"):
 # The language model operators' GPU kernels and their way past autograd are C++ (csrc/xdna_torch.cpp). Without the library
 # their GPU calls reach the functions above, which raise.
 if os.path.exists(kernels.TORCH_LIB_PATH):
-    kernels.torch_lib()
+    try:
+        kernels.torch_lib()
+    except (OSError, RuntimeError):     # another torch or ABI than it was built for: raised again by the first GPU call
+        pass
