@@ -28,7 +28,8 @@ def _check(args, biased=False):
     (2, 40, 8320, 128, True, True), (3, 77, 4192, 32, False, True), (4, 33, 2048, 64, True, False), (4, 2100, 2048, 128, True, True),
     # tiles: K in one part and in several, windows of scales that end inside a group
     (17, 70, 1376, 32, True, True), (33, 65, 1056, 96, False, False), (64, 130, 4512, 32, True, True), (50, 64, 5120, 160, True, False),
-    (16, 200, 9216, 64, False, True), (47, 300, 2240, 64, True, False), (8, 100, 2176, 128, True, True), (70, 40, 3200, 320, True, True)])
+    (5, 70, 512, 32, True, True), (30, 90, 544, 32, False, True), (64, 100, 640, 128, True, False), (20, 50, 20512, 32, True, True),
+    (33, 17000, 640, 64, True, True), (16, 200, 9216, 64, False, True), (47, 300, 2240, 64, True, False), (8, 100, 2176, 128, True, True), (70, 40, 3200, 320, True, True)])
 def test_w4_forms(gpu, m, n, k, group, zeros, bias, dtype):
     _check(w4_case(m, n, k, group, zeros, bias, dtype, seed=m + k, dev=gpu), biased=dtype == "bf16")
 

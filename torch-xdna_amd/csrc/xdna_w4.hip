@@ -343,9 +343,11 @@ __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
 // step's four quarters are 32 consecutive k. Two tiles' x (DMA into LDS) and weights are on their way while a third is
 // used. Scales and zero points come into LDS for WIN k at a time. FL: steps (32 k each) of a group's sum
 // before its scale: 4 where G % 128 == 0, 2 where G % 64 == 0, else 1. Measured with the join: 40 x 14336 -> 4096 in
-// float16 23.3 us (33.6 MB), 8 x 4096 -> 14336 in bfloat16 15 us (33 MB): latency, with two workgroups a CU.
-template <int DT, bool S4, int MT, int FL>
-__global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
+// float16 23 us (33.6 MB), 8 x 4096 -> 14336 in bfloat16 13.0 us (33 MB): latency, eight waves a CU.
+// KG groups of four waves share out a part's tiles (group GI the GI-th run of them), each with LDS of its own, and meet in
+// LDS at the end: as good as more parts, without their join. All groups pass the same barriers, whatever tiles there are.
+template <int DT, bool S4, int MT, int FL, int KG, int GI>
+__device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
   constexpr int W = 4;                                  // waves
   constexpr int XP = DT == XDNA_F32 ? 3 : 1, GC = 4 / FL, D = 3;
   constexpr uint32_t esz = DT == XDNA_F32 ? 4 : 2;
@@ -361,18 +363,19 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
   __shared__ __attribute__((aligned(1024))) int8_t lds2[TILE];
   __shared__ float sl[GW * COLS];                       // group by group, so that a wave's columns lie side by side
   __shared__ uint8_t zl[GW * COLS];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W, tid = threadIdx.x % (W * 64);
   const int col = lane & 15, quarter = lane >> 4;
   const int64_t N = a.N;
   const int K = a.K, G = a.G, groups = K / G;
   const int64_t w0 = (int64_t)blockIdx.x * COLS, n0 = w0 + wave * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
   const int cols = (int)max<int64_t>(0, min<int64_t>(16, N - n0)), rows = (int)min<int64_t>(16 * MT, a.M - m0);
   const int wcols = (int)min<int64_t>(COLS, N - w0);
-  const int tbeg = blockIdx.z * a.per, tend = min((K + KT - 1) / KT, tbeg + a.per);
+  // tiles tbeg .. tend - 1 are there, tbeg .. tnom - 1 are gone through
+  const int part = blockIdx.z * a.per, last = min((K + KT - 1) / KT, part + a.per), share = (a.per + KG - 1) / KG;
+  const int tbeg = part + GI * share, tend = min(last, tbeg + share), tnom = KG == 1 ? tend : tbeg + share;
   const auto wr = make_rsrc(a.qw + (cols ? n0 : 0) * (K / 2), (uint32_t)cols * (uint32_t)(K / 2));
   const auto xr = make_rsrc(static_cast<const char*>(a.x) + m0 * a.ldx * esz, (uint32_t)(((rows - 1) * a.ldx + K) * esz));
   const uint8_t* const zeros = a.zeros ? a.zeros : static_cast<const uint8_t*>(a.scales);    // read in any case, 8 put in later
-  f32x4 acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // load j: the rows of the tile's KB j, a row's chunk c at place c ^ (row & 15); what lies past K is zeros
@@ -405,13 +408,13 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
       ring[slot][u] = buf_load_u4<true>(wr, in ? (uint32_t)(col * (K / 2) + tile * (KT / 2) + u * 64 + quarter * 16) : OOB);
     }
   };
-  for (int win = tbeg; win < tend; win += WIN / KT) {
-    const int wend = min(tend, win + WIN / KT), g0 = win * KT / G, gn = (min(K, wend * KT) - 1) / G + 1 - g0;
+  for (int win = tbeg; win < tnom; win += WIN / KT) {
+    const int wend = min(tnom, win + WIN / KT), g0 = min(win * KT, K - 1) / G, gn = (min(K, wend * KT) - 1) / G + 1 - g0;
     if (win > tbeg) __syncthreads();
 #pragma unroll
     for (int i = 0; i < D - 1; ++i) fetch(win + i, i);
     const int elems = wcols * gn;
-    for (int i0 = threadIdx.x; i0 < elems; i0 += 8 * W * 64) {     // eight loads of each at a time
+    for (int i0 = tid; i0 < elems; i0 += 8 * W * 64) {     // eight loads of each at a time
       uint32_t sv[8], zv[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -440,6 +443,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (decltype(steady)::value) fetch(tile + D - 1, (d + D - 1) % D);
       __builtin_amdgcn_sched_barrier(0);
+      if (KG > 1 && tile >= tend) return;          // uniform
       const int8_t* const cur = d == 0 ? lds0 : d == 1 ? lds1 : lds2;
       // x's fragments of a chunk are read one chunk ahead of their use, all at once
       constexpr int XR = DT == XDNA_F32 ? 2 : 1;
@@ -537,17 +541,41 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(W4Args a) {
           if (t == (e >> 2) && r == (e & 3) && !(fabsf(acc[t][r]) < INFINITY)) acc[t][r] = v;
     }
   }
-  if (col >= cols) return;
-  const float bias = a.bias && !a.part ? load_any(a.bias, n0 + col, a.bias_dt) : 0.0f;
+}
+
+template <int DT, bool S4, int MT, int FL, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void w4_tile_kernel(W4Args a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x4 acc[MT];
+  if (KG == 1 || wave < 4) w4_tiles<DT, S4, MT, FL, KG, 0>(a, acc);
+  if constexpr (KG == 2) {
+    __shared__ f32x4 red[MT][4][64];
+    if (wave >= 4) {
+      w4_tiles<DT, S4, MT, FL, KG, 1>(a, acc);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) red[t][wave - 4][lane] = acc[t];
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const f32x4 x = red[t][wave][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[t][r] += x[r];
+    }
+  }
+  const int col = lane & 15, quarter = lane >> 4;
+  const int64_t N = a.N, n = (int64_t)blockIdx.x * 64 + wave * 16 + col, m0 = (int64_t)blockIdx.y * (16 * MT);
+  if (n >= N) return;
+  const float bias = a.bias && !a.part ? load_any(a.bias, n, a.bias_dt) : 0.0f;
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * quarter + r;
-      if (row >= rows) continue;
-      const int64_t out = (m0 + row) * N + n0 + col;
-      if (a.part) a.part[blockIdx.z * a.M * N + out] = acc[t][r];
-      else store_from_f32<DT>(a.y, out, a.bias ? acc[t][r] + bias : acc[t][r]);
+      const int64_t row = m0 + 16 * t + 4 * quarter + r;
+      if (row >= a.M) continue;
+      if (a.part) a.part[blockIdx.z * a.M * N + row * N + n] = acc[t][r];
+      else store_from_f32<DT>(a.y, row * N + n, a.bias ? acc[t][r] + bias : acc[t][r]);
     }
 }
 
@@ -572,7 +600,7 @@ __global__ __launch_bounds__(256) void w4_join_kernel(const float* __restrict__ 
 struct W4Plan {
   bool row;             // w4_row_kernel
   int kl, per;          // its lanes and waves along K
-  int mt, parts;        // w4_tile_kernel's row blocks of 16 and split of K
+  int mt, kg, parts;    // w4_tile_kernel's row blocks of 16, groups of waves and split of K
 };
 
 // One row: the row kernel, but for 16-bit rows and 32 columns a CU (8192) or more (1 x 4096 -> 14336, bfloat16: row
@@ -580,9 +608,13 @@ struct W4Plan {
 // 36). Two to four rows: where the weights are few (3 x 1504 -> 1001 in float32 9.3 / 14.9 us, 4 x 8192 -> 512 7.4 /
 // 10.1, 4 x 4096 -> 4096 12.4 / 10.0). Its lanes along K: 64, so that long K makes waves enough, or 16 where the
 // columns do (4096 -> 14336 in bfloat16: 15.2 with 16, 19.0 with 64; 14336 -> 4096: 25 / 11.8), and more waves along
-// K below four a CU (14336 -> 64: one wave 9.2 us, four 5.8). Tiles: K in as many parts as make two workgroups a CU,
-// none under 1024 k (40 x 14336 -> 4096: 1 / 2 / 4 / 8 / 16 parts 82.1 / 45.8 / 27.9 / 24.7 / 28.3 us, of which 5 the
-// joining).
+// K below four a CU (14336 -> 64: one wave 9.2 us, four 5.8).
+//
+// Tiles of 16-bit rows: two groups of waves share out K from 512 k on, unless there are two workgroups a CU without
+// (1 x 4096 -> 14336: one group 16.0 us, two 12.6, four 12.6; 64 x 4096 -> 14336 32.4 / 25.7), and K goes in parts on
+// top until there is a workgroup a CU, none under 512 k, 16 at most (40 x 14336 -> 4096 with two groups: 3 / 4 / 8 parts
+// 29.2 / 23.2 / 26.4 us, of which 3.5 the joining; 2 x 14336 -> 1000: 8 / 16 parts 10.6 / 9.4; 5 x 992 -> 2000: 7.3
+// with one). float32: parts alone, two workgroups a CU, none under 1024 k.
 W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   W4Plan p{};
   const int64_t cus = device_cus();
@@ -597,12 +629,14 @@ W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   } else {
     p.mt = (int)std::min<int64_t>(f32 ? 2 : 4, cdiv(M, 16));
     const int64_t wgs = cdiv(N, 64) * cdiv(M, 16 * p.mt);
-    p.parts = (int)std::max<int64_t>(1, std::min(2 * cus / wgs, K / 1024));
+    p.kg = !f32 && K >= 512 && wgs < 2 * cus ? 2 : 1;
+    p.parts = (int)std::max<int64_t>(
+        1, p.kg == 2 ? std::min<int64_t>({cus / wgs, K / 512, 16}) : std::min(2 * cus / wgs, K / 1024));
   }
   return p;
 }
 
-template <int DT, bool S4, int MT, int FL>
+template <int DT, bool S4, int MT, int FL, int KG>
 int w4_tile_go(W4Args a, int parts, hipStream_t st) {
   // rows of a launch: the grid's y
   const int64_t rows = a.part ? a.M : std::min<int64_t>(65535, cdiv(a.M, 16 * MT)) * (16 * MT), M = a.M;
@@ -613,19 +647,27 @@ int w4_tile_go(W4Args a, int parts, hipStream_t st) {
     b.M = std::min(rows, M - m);
     b.x = static_cast<const char*>(a.x) + m * a.ldx * esz;
     b.y = static_cast<char*>(a.y) + m * a.N * esz;
-    w4_tile_kernel<DT, S4, MT, FL>
-        <<<dim3((unsigned)cdiv(a.N, 64), (unsigned)cdiv(b.M, 16 * MT), (unsigned)parts), 256, 0, st>>>(b);
+    w4_tile_kernel<DT, S4, MT, FL, KG>
+        <<<dim3((unsigned)cdiv(a.N, 64), (unsigned)cdiv(b.M, 16 * MT), (unsigned)parts), 256 * KG, 0, st>>>(b);
   }
   if (a.part)
     w4_join_kernel<DT><<<(unsigned)cdiv(M * a.N, 256), 256, 0, st>>>(a.part, parts, M * a.N, a.N, a.bias, a.bias_dt, a.y);
   return launch_status("linear_w4");
 }
 
-template <int DT, bool S4, int MT>
+template <int DT, bool S4, int MT, int KG>
 int w4_group(const W4Args& a, const W4Plan& p, hipStream_t st) {
-  if (a.G % 128 == 0) return w4_tile_go<DT, S4, MT, 4>(a, p.parts, st);
-  if (a.G % 64 == 0) return w4_tile_go<DT, S4, MT, 2>(a, p.parts, st);
-  return w4_tile_go<DT, S4, MT, 1>(a, p.parts, st);
+  if (a.G % 128 == 0) return w4_tile_go<DT, S4, MT, 4, KG>(a, p.parts, st);
+  if (a.G % 64 == 0) return w4_tile_go<DT, S4, MT, 2, KG>(a, p.parts, st);
+  return w4_tile_go<DT, S4, MT, 1, KG>(a, p.parts, st);
+}
+
+template <int DT, bool S4, int MT>
+int w4_tiles_go(const W4Args& a, const W4Plan& p, hipStream_t st) {
+  if constexpr (DT != XDNA_F32) {
+    if (p.kg == 2) return w4_group<DT, S4, MT, 2>(a, p, st);
+  }
+  return w4_group<DT, S4, MT, 1>(a, p, st);
 }
 
 template <int DT, bool S4, int KL>
@@ -640,9 +682,9 @@ int w4_row_go(W4Args a, const W4Plan& p, hipStream_t st) {
 template <int DT, bool S4>
 int w4_go(const W4Args& a, const W4Plan& p, hipStream_t st) {
   if (p.row) return p.kl == 16 ? w4_row_go<DT, S4, 16>(a, p, st) : w4_row_go<DT, S4, 64>(a, p, st);
-  if (p.mt == 1) return w4_group<DT, S4, 1>(a, p, st);
-  if (DT == XDNA_F32 || p.mt == 2) return w4_group<DT, S4, 2>(a, p, st);
-  if constexpr (DT != XDNA_F32) return p.mt == 3 ? w4_group<DT, S4, 3>(a, p, st) : w4_group<DT, S4, 4>(a, p, st);
+  if (p.mt == 1) return w4_tiles_go<DT, S4, 1>(a, p, st);
+  if (DT == XDNA_F32 || p.mt == 2) return w4_tiles_go<DT, S4, 2>(a, p, st);
+  if constexpr (DT != XDNA_F32) return p.mt == 3 ? w4_tiles_go<DT, S4, 3>(a, p, st) : w4_tiles_go<DT, S4, 4>(a, p, st);
   return XDNA_EUNSUPPORTED;
 }
 
