@@ -614,7 +614,9 @@ struct W4Plan {
 // (1 x 4096 -> 14336: one group 16.0 us, two 12.6, four 12.6; 64 x 4096 -> 14336 32.4 / 25.7), and K goes in parts on
 // top until there is a workgroup a CU, none under 512 k, 16 at most (40 x 14336 -> 4096 with two groups: 3 / 4 / 8 parts
 // 29.2 / 23.2 / 26.4 us, of which 3.5 the joining; 2 x 14336 -> 1000: 8 / 16 parts 10.6 / 9.4; 5 x 992 -> 2000: 7.3
-// with one). float32: parts alone, two workgroups a CU, none under 1024 k.
+// with one). float32, whose tiles take three times the work: parts alone, up to two workgroups a CU and 16 parts, none
+// under 128 k (14 x 1536 -> 138: 1 / 4 / 8 / 12 parts 22.2 / 10.0 / 8.4 / 7.7 us; 8 x 4096 -> 4096 17.0 with
+// 4, 15.1 with 8).
 W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   W4Plan p{};
   const int64_t cus = device_cus();
@@ -631,7 +633,7 @@ W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
     const int64_t wgs = cdiv(N, 64) * cdiv(M, 16 * p.mt);
     p.kg = !f32 && K >= 512 && wgs < 2 * cus ? 2 : 1;
     p.parts = (int)std::max<int64_t>(
-        1, p.kg == 2 ? std::min<int64_t>({cus / wgs, K / 512, 16}) : std::min(2 * cus / wgs, K / 1024));
+        1, p.kg == 2 ? std::min<int64_t>({cus / wgs, K / 512, 16}) : std::min<int64_t>({2 * cus / wgs, K / 128, 16}));
   }
   return p;
 }
