@@ -615,7 +615,7 @@ struct W4Plan {
 // top until there is a workgroup a CU, none under 512 k, 16 at most (40 x 14336 -> 4096 with two groups: 3 / 4 / 8 parts
 // 29.2 / 23.2 / 26.4 us, of which 3.5 the joining; 2 x 14336 -> 1000: 8 / 16 parts 10.6 / 9.4; 5 x 992 -> 2000: 7.3
 // with one). float32, whose tiles take three times the work: parts alone, up to two workgroups a CU and 16 parts, none
-// under 128 k (14 x 1536 -> 138: 1 / 4 / 8 / 12 parts 22.2 / 10.0 / 8.4 / 7.7 us; 8 x 4096 -> 4096 17.0 with
+// under 128 k (14 x 1536 -> 138: 1 / 4 / 8 / 12 parts 22.2 / 10.0 / 8.4 / 7.7 us; 8 x 4096 -> 4096 16.5 with
 // 4, 15.1 with 8).
 W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   W4Plan p{};
