@@ -1,0 +1,40 @@
+"""linear_w4 on the MI355X at the edges of its tiles: columns past N and values that are not finite."""
+import math
+
+import pytest
+import torch
+
+from lm_reference import w4_case
+from torch_xdna import lm
+
+pytestmark = pytest.mark.gpu
+
+
+def _us(f, before=lambda: None):
+    """The shortest of ten calls of f, each right after `before`."""
+    best = math.inf
+    for _ in range(10):
+        before()
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        f()
+        end.record()
+        torch.cuda.synchronize()
+        best = min(best, start.elapsed_time(end) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_w4_ragged_columns_take_the_same_time_after_any_kernel(gpu, m):
+    """Columns past N have no scales. What a kernel before left in their place in LDS (NaN, from the same kernel with
+    scales of NaN) must not send the last columns through the sums for values that are not finite: those take over 100
+    times as long."""
+    x, q, s, z, _ = w4_case(m, 8200, 1024, 64, True, False, "bf16", seed=1, dev=gpu)
+    full = w4_case(m, 16384, 1024, 64, True, False, "bf16", seed=2, dev=gpu)
+    bad = torch.full_like(full[2], math.nan)
+    want = lm.linear_w4(x, q, s, z)
+    clean = _us(lambda: lm.linear_w4(x, q, s, z), lambda: lm.linear_w4(*full))
+    dirty = _us(lambda: lm.linear_w4(x, q, s, z), lambda: lm.linear_w4(full[0], full[1], bad, full[3]))
+    print(f"after finite scales {clean:.1f} us, after scales of NaN {dirty:.1f} us")
+    assert torch.equal(lm.linear_w4(x, q, s, z), want)
+    assert dirty < 3 * clean

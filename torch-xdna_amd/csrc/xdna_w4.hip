@@ -369,7 +369,7 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
   const int K = a.K, G = a.G, groups = K / G;
   const int64_t w0 = (int64_t)blockIdx.x * COLS, n0 = w0 + wave * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
   const int cols = (int)max<int64_t>(0, min<int64_t>(16, N - n0)), rows = (int)min<int64_t>(16 * MT, a.M - m0);
-  const int wcols = (int)min<int64_t>(COLS, N - w0);
+  const int wcols = (int)min<int64_t>(COLS, N - w0), scol = min(wave * 16 + col, wcols - 1);     // past N: the last one's scales
   // tiles tbeg .. tend - 1 are there, tbeg .. tnom - 1 are gone through
   const int part = blockIdx.z * a.per, last = min((K + KT - 1) / KT, part + a.per), share = (a.per + KG - 1) / KG;
   const int tbeg = part + GI * share, tend = min(last, tbeg + share), tnom = KG == 1 ? tend : tbeg + share;
@@ -468,7 +468,7 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int f = 0; f < GC; ++f) {
-          const int i = (group_of(tile * KT + u * 128 + f * FL * 32) - g0) * COLS + wave * 16 + col;
+          const int i = (group_of(tile * KT + u * 128 + f * FL * 32) - g0) * COLS + scol;
           const float s = sl[i], z = (float)zl[i];
           f32x4 part[MT], sum[MT];
 #pragma unroll
@@ -521,7 +521,7 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) odd |= !(fabsf(acc[t][r]) < INFINITY);
+    for (int r = 0; r < 4; ++r) odd |= col < cols && 16 * t + 4 * quarter + r < rows && !(fabsf(acc[t][r]) < INFINITY);
   if (DT == XDNA_BF16 && __builtin_amdgcn_ballot_w64(odd)) {     // x (or a scale) that is not finite: again, one by one
 #pragma unroll 1
     for (int e = 0; e < MT * 4; ++e) {
