@@ -38,3 +38,18 @@ def test_w4_ragged_columns_take_the_same_time_after_any_kernel(gpu, m):
     print(f"after finite scales {clean:.1f} us, after scales of NaN {dirty:.1f} us")
     assert torch.equal(lm.linear_w4(x, q, s, z), want)
     assert dirty < 3 * clean
+
+
+def test_w4_rows_that_are_not_finite_cost_their_own_sums_only(gpu):
+    """One row of 64 with a NaN: its sums are formed again, value by value, and not those of the other rows (a wave would
+    do 16 rows' worth for one, in turn)."""
+    x, q, s, z, _ = w4_case(64, 4096, 4096, 64, True, False, "bf16", seed=3, dev=gpu)
+    one, every = x.clone(), x.clone()
+    one[37, 100], every[:, 100] = math.nan, math.nan
+    want = lm.linear_w4(x, q, s, z)
+    y = lm.linear_w4(one, q, s, z)
+    keep = torch.arange(64, device=gpu) != 37
+    assert torch.equal(y[keep], want[keep]) and bool(y[37].isnan().all())
+    t1, t64 = _us(lambda: lm.linear_w4(one, q, s, z)), _us(lambda: lm.linear_w4(every, q, s, z))
+    print(f"one row {t1:.1f} us, every row {t64:.1f} us")
+    assert t1 < t64 / 4

@@ -526,7 +526,12 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
 #pragma unroll 1
     for (int e = 0; e < MT * 4; ++e) {
       const int row = 16 * (e >> 2) + 4 * quarter + (e & 3);
-      if (row >= rows || col >= cols) continue;
+      bool again = false;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) again |= t == (e >> 2) && r == (e & 3) && !(fabsf(acc[t][r]) < INFINITY);
+      if (!again || row >= rows || col >= cols) continue;
       float v = 0.0f;
       for (int k = tbeg * KT; k < min(K, tend * KT); ++k) {
         const int64_t sg = (n0 + col) * groups + k / G;
@@ -538,7 +543,7 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (t == (e >> 2) && r == (e & 3) && !(fabsf(acc[t][r]) < INFINITY)) acc[t][r] = v;
+          if (t == (e >> 2) && r == (e & 3)) acc[t][r] = v;
     }
   }
 }
