@@ -53,3 +53,31 @@ def test_w4_rows_that_are_not_finite_cost_their_own_sums_only(gpu):
     t1, t64 = _us(lambda: lm.linear_w4(one, q, s, z)), _us(lambda: lm.linear_w4(every, q, s, z))
     print(f"one row {t1:.1f} us, every row {t64:.1f} us")
     assert t1 < t64 / 4
+
+
+@pytest.mark.parametrize("m,n,k,scales", [(1, 50, 4096, "same"), (1, 9000, 512, "same"), (3, 40, 1024, "same"), (2, 30, 8320, "bf16"),
+                                          (8, 100, 2176, "same"), (40, 64, 4096, "f16")])
+def test_w4_float32_near_the_largest(gpu, m, n, k, scales):
+    """float32 x near the type's largest: the product with q - z passes it, the result does not. Its own row is as the
+    formula has it, the others are as they were; infinities and NaN too."""
+    x, q, s, z, _ = w4_case(m, n, k, 128, True, False, "f32", seed=5, dev=gpu, scales=scales)
+    want = lm.linear_w4(x, q, s, z)
+    r, at = m - 1, k - 28                                     # in the last group
+    d = (q[:, at // 2] & 15).float() - z[:, -1].float()
+    w = d.double() * s[:, -1].double()
+    for value in (2.0 ** 126, -1.5 * 2.0 ** 127):
+        x2 = x.clone()
+        x2[r, at] = value
+        y = lm.linear_w4(x2, q, s, z)
+        assert torch.equal(y[:r], want[:r])
+        # the rest of the row is far below half a step of this product; q - z, the scale and the product round once each
+        expect = w * value
+        assert float(expect.abs().max()) < torch.finfo(torch.float32).max and bool((d.abs() >= 8).any())
+        assert bool(((y[r].double() - expect).abs()[d != 0] <= expect.abs()[d != 0] * 2.0 ** -22).all())
+    for value in (math.inf, math.nan):
+        x2 = x.clone()
+        x2[r, at] = value
+        y = lm.linear_w4(x2, q, s, z)
+        assert torch.equal(y[:r], want[:r])
+        expect = torch.where(d == 0, math.nan, d.sign() * value)
+        torch.testing.assert_close(y[r], expect, rtol=0, atol=0, equal_nan=True)

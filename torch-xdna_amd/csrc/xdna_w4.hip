@@ -14,7 +14,8 @@
 // are then up to 30 times the result's own size, 2^-19 in the float32 sums against the output's 2^-9. Where x is not
 // finite that difference is not what the formula says (inf - inf), so such sums are formed again, value by value.
 // float32 x meets weights converted one by one, q - z; for the matrix units it is cut into three bfloat16 numbers
-// that add up to it exactly.
+// that add up to it exactly; its sums before the scale, up to 255 times |x|, may pass float32 where the result does not,
+// and those that do are formed again too, the scale first.
 //
 // One row (a decode step), and up to four where the weights are few, are dot products on the vector units:
 // w4_row_kernel. More go to the matrix units, x through LDS: w4_tile_kernel.
@@ -315,6 +316,29 @@ __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
     if (b < pend) block(b, ring[0]);
     if (b + per < pend) block(b + per, ring[1]);
   }
+  if constexpr (DT == XDNA_F32) {
+    // x or a scale is not finite, or a sum before its scale passes float32: the lane's values again, the scale first
+    bool odd = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) odd |= cl < cols && !(fabsf(acc[r]) < INFINITY);
+    if (__builtin_amdgcn_ballot_w64(odd)) {
+      const int64_t n = wg0 + min(set * CL + cl, wcols - 1);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (cl >= cols || fabsf(acc[r]) < INFINITY) continue;
+        float v = 0.0f;
+        for (int p0 = 0; p0 < blocks; p0 += piece)
+          for (int b = p0 + ki; b < min(p0 + piece, blocks); b += per)
+            for (int k = (b * KL + kl) * 32; k < min(K, (b * KL + kl) * 32 + 32); ++k) {
+              const int64_t at = n * groups + k / G;
+              const uint8_t w = a.qw[n * (K / 2) + (k >> 1)];
+              const float q = (float)((k & 1) ? w >> 4 : w & 15) - (a.zeros ? (float)a.zeros[at] : 8.0f);
+              v = __builtin_fmaf(q * load_any(a.scales, at, a.sdt), load_as_f32<DT>(a.x, min(r, rows - 1) * a.ldx + k), v);
+            }
+        acc[r] = v;
+      }
+    }
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float v = acc[r];
@@ -522,7 +546,8 @@ __device__ __forceinline__ void w4_tiles(const W4Args& a, f32x4 (&acc)[MT]) {
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) odd |= col < cols && 16 * t + 4 * quarter + r < rows && !(fabsf(acc[t][r]) < INFINITY);
-  if (DT == XDNA_BF16 && __builtin_amdgcn_ballot_w64(odd)) {     // x (or a scale) that is not finite: again, one by one
+  // x or a scale is not finite, or a sum before its scale passes float32: again, one by one, the scale first
+  if (DT != XDNA_F16 && __builtin_amdgcn_ballot_w64(odd)) {
 #pragma unroll 1
     for (int e = 0; e < MT * 4; ++e) {
       const int row = 16 * (e >> 2) + 4 * quarter + (e & 3);
