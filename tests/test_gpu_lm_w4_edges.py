@@ -81,3 +81,15 @@ def test_w4_float32_near_the_largest(gpu, m, n, k, scales):
         assert torch.equal(y[:r], want[:r])
         expect = torch.where(d == 0, math.nan, d.sign() * value)
         torch.testing.assert_close(y[r], expect, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_w4_rows_far_apart(gpu, dtype):
+    """The last token of every prompt, a view whose rows lie further apart than the kernels' offsets reach."""
+    x, q, s, z, b = w4_case(3, 40, 4096, 64, True, True, dtype, seed=6, dev=gpu)
+    want = lm.linear_w4(x, q, s, z, b)
+    states = torch.zeros(3, 1025, 4096, dtype=x.dtype, device=gpu)
+    states[:, -1] = x
+    assert states[:, -1].stride(0) > 1 << 22
+    assert torch.equal(lm.linear_w4(states[:, -1], q, s, z, b), want)
+    assert torch.equal(torch.ops.xdna.linear_w4(states[:, -1:], q, s, z, b), want[:, None])

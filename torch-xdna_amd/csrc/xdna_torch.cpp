@@ -114,7 +114,8 @@ Tensor linear_w4(const Tensor& x, const Tensor& qweight, const Tensor& scales, c
     return t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 &&
            (m == 1 || t.stride(0) * t.element_size() % 16 == 0);
   };
-  if (!fits(x2) || (m > 1 && x2.stride(0) < k)) x2 = x2.clone(at::MemoryFormat::Contiguous);
+  // rows that overlap, or lie further apart than the kernels' offsets reach, are read from a copy
+  if (!fits(x2) || (m > 1 && (x2.stride(0) < k || x2.stride(0) > (1 << 22)))) x2 = x2.clone(at::MemoryFormat::Contiguous);
   const int xc = code(x.scalar_type());
   const Tensor b = bias ? bias->contiguous() : Tensor();
   const int64_t need = xdna_linear_w4_ws_bytes(xc, m, n, k);
