@@ -380,8 +380,8 @@ int xdna_linear_w4_ws(const void* x, int x_dtype, int64_t ldx, const void* qweig
  * head h = softmax over the tokens start(t) .. t of (q . k * scale), times v, of kv head h / (nh / nkv). starts [nseq + 1]:
  * the first token of each sequence, ascending, and T; start(t) is the largest of them that is not above t (0 if
  * none is), so that no value of them reads out of range. d a multiple of 8, at most 128. strides (elements, multiples of
- * 8, below 2^24): {q token, q head, k token, k head, v token, v head}. Pointers 16-byte aligned. Rows whose scores are all
- * -inf are zero. No counterpart in the reference. */
+ * 8; of k and v from token to token d .. 2^24 - 1): {q token, q head, k token, k head, v token, v head}. Pointers
+ * 16-byte aligned. Rows whose scores are all -inf are zero. No counterpart in the reference. */
 int xdna_attention_causal(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
                           const int32_t* starts, int64_t nseq, int64_t T, int nh, int nkv, int d, float scale, void* out,
                           void* stream);
@@ -389,7 +389,7 @@ int xdna_attention_causal(const void* q, const void* k, const void* v, int dtype
 /* One decode step's attention of B sequences that share a prefix: out [B, nh, d], sequence b's row over the P keys of kp /
  * vp and the first lens[b] (clamped to 0 .. S) of the S of kc / vc [b]. Types, d, scale, alignment and empty rows as in
  * xdna_attention_causal; strides: {q sequence, q head, kp token, kp head, vp token, vp head, kc sequence, kc token,
- * kc head, vc sequence, vc token, vc head}, those of sequences of any size. ws: xdna_attention_prefix_ws_bytes(..) bytes
+ * kc head, vc sequence, vc token, vc head}. ws: xdna_attention_prefix_ws_bytes(..) bytes
  * (0: none needed) that the call may overwrite, 16-byte aligned. No counterpart in the reference. */
 int64_t xdna_attention_prefix_ws_bytes(int64_t P, int64_t S, int64_t B, int nh, int nkv, int d);
 int xdna_attention_prefix(const void* q, const void* kp, const void* vp, const void* kc, const void* vc, int dtype,

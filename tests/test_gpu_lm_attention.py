@@ -262,3 +262,26 @@ def test_prefix_offsets_past_32_bits(gpu):
     c = causal_case([p - 200, 200], 4, kv, d, "bf16", seed=17, dev=gpu)
     kf.copy_(c[1])
     assert torch.equal(lm.attention_causal(c[0], kf, c[2], c[3]), lm.attention_causal(*c))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_long_caches_of_one_head_after_another(gpu, dtype):
+    """Keys and values laid out [heads, tokens, dims]: heads 2^24 elements apart and more are read where they lie, without a
+    copy of the cache."""
+    b, p, h, kv, d = 2, 131200, 4, 2, 128
+    q, kp, vp, kc, vc, lens = prefix_case(b, 300, 8, h, kv, d, dtype, seed=12, dev=gpu)
+    want = lm.attention_prefix(q, kp, vp, kc, vc, lens)
+    cache = torch.zeros(2, kv, p, d, dtype=q.dtype, device=gpu)
+    cache[0, :, -300:], cache[1, :, -300:] = kp.transpose(0, 1), vp.transpose(0, 1)
+    k, v = (t[:, -300:].transpose(0, 1) for t in cache)
+    assert k.stride(1) > 1 << 24
+    assert torch.equal(lm.attention_prefix(q, k, v, kc, vc, lens), want)
+    causal = lm.attention_causal(kp.repeat_interleave(2, 1), kp, vp, torch.tensor([0, 300], dtype=torch.int32, device=gpu))
+    assert torch.equal(lm.attention_causal(kp.repeat_interleave(2, 1), k, v, torch.tensor([0, 300], dtype=torch.int32, device=gpu)), causal)
+    k, v = (t.transpose(0, 1) for t in cache)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = lm.attention_prefix(q, k, v, kc, vc, lens)
+    assert torch.cuda.max_memory_allocated() - before < cache.nbytes // 4
+    assert torch.equal(out, lm.attention_prefix(q, k.contiguous(), v.contiguous(), kc, vc, lens))

@@ -897,8 +897,9 @@ int prefix_go(const PrefixArgs& a, hipStream_t st) {
 // above 0, so that an unseen key's -inf stays one: scale 0 weighs all keys alike with it
 float scale_c(float scale) { return std::max(fabsf(scale) * 1.44269504088896340736f, 1.17549435e-38f); }
 
-// a stride in elements that keeps 16-byte alignment and whose offsets within a tile of 64 keys fit 31 bits
-bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (1ll << 24); }
+// A stride in elements that keeps 16-byte alignment; one from token to token: whose offsets within a tile of 64 keys fit
+// 31 bits besides. All others are multiplied in 64 bits.
+bool stride_ok(int64_t s, bool token) { return s >= 0 && s % 8 == 0 && (!token || s < (1ll << 24)); }
 
 }  // namespace
 }  // namespace xdna
@@ -916,7 +917,8 @@ int xdna_attention_causal(const void* q, const void* k, const void* v, int dtype
   if (T == 0) return XDNA_OK;
   XDNA_REQUIRE(q && k && v && strides && starts && out, "null pointer");
   XDNA_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16), "operands must be 16-byte aligned");
-  for (int i = 0; i < 6; ++i) XDNA_REQUIRE(stride_ok(strides[i]), "strides must be multiples of 8 below 2^24");
+  for (int i = 0; i < 6; ++i)
+    XDNA_REQUIRE(stride_ok(strides[i], i == 2 || i == 4), "strides must be multiples of 8, from key to key below 2^24");
   XDNA_REQUIRE(strides[2] >= d && strides[4] >= d, "a token's keys and values must not overlap the next one's");
   // 31-bit row numbers, and the launch's threads
   XDNA_REQUIRE(T * (nh / nkv) < (1ll << 31) - 128 && cdiv(T * (nh / nkv), 128) * nkv <= MAX_LAUNCH_THREADS / 256, "too many tokens");
@@ -951,8 +953,7 @@ int xdna_attention_prefix(const void* q, const void* kp, const void* vp, const v
   XDNA_REQUIRE(aligned(q, 16) && aligned(kp, 16) && aligned(vp, 16) && aligned(kc, 16) && aligned(vc, 16) && aligned(out, 16),
                "operands must be 16-byte aligned");
   for (int i = 0; i < 12; ++i)
-    XDNA_REQUIRE(i == 0 || i == 6 || i == 9 ? strides[i] >= 0 && strides[i] % 8 == 0 : stride_ok(strides[i]),
-                 "strides must be multiples of 8, those of tokens and heads below 2^24");
+    XDNA_REQUIRE(stride_ok(strides[i], i == 2 || i == 4 || i == 7 || i == 10), "strides must be multiples of 8, from key to key below 2^24");
   XDNA_REQUIRE(strides[2] >= d && strides[4] >= d && strides[7] >= d && strides[10] >= d,
                "a token's keys and values must not overlap the next one's");
   PrefixArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kp), static_cast<const uint16_t*>(vp),

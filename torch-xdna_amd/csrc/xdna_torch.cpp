@@ -144,8 +144,8 @@ double attention_args(const char* name, const Tensor& q, std::initializer_list<c
 }
 
 // t [.., heads, d] as the library reads it, and its strides but the last's (of dims of one, any will do): itself
-// where the last dim is dense, it starts on 16 bytes, no token's values overlap the next one's and the strides are
-// multiples of 8 that fit the kernels' offsets; else a copy.
+// where the last dim is dense, it starts on 16 bytes, no token's values overlap the next one's, the strides are
+// multiples of 8 and that of tokens fits the kernels' offsets; else a copy.
 Tensor heads(Tensor t, int64_t* st) {
   const int64_t n = t.dim() - 1, d = t.size(n);
   for (int pass = 0; pass < 2; ++pass) {
@@ -154,7 +154,7 @@ Tensor heads(Tensor t, int64_t* st) {
       st[i] = t.size(i) == 1 ? d : t.stride(i);
       ok = ok && st[i] % 8 == 0;
     }
-    if (ok && st[n - 2] >= d && st[n - 2] < (1 << 24) && st[n - 1] < (1 << 24)) break;
+    if (ok && st[n - 2] >= d && st[n - 2] < (1 << 24)) break;
     t = t.clone(at::MemoryFormat::Contiguous);
   }
   return t;
