@@ -117,3 +117,23 @@ def test_without_the_library(gpu, monkeypatch):
     monkeypatch.setattr(kernels, "TORCH_LIB_PATH", "/nowhere/libxdna_torch.so")
     with pytest.raises(RuntimeError, match="not built"):
         lm.linear_w4(*_cases(gpu)["linear_w4"])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode(gpu, name):
+    """There is no forward-mode derivative: a tangent raises, on the GPU and on the host, and is not dropped."""
+    for dev in (gpu, "cpu"):
+        args = _cases(dev)[name]
+        f = getattr(ops, name)
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(args[0], torch.ones_like(args[0]))
+            with pytest.raises(NotImplementedError):
+                f(dual, *args[1:])
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                f(dual, *args[1:])
+            assert f(*args).shape == f(args[0], *args[1:]).shape
+        first = args[0].clone().requires_grad_()
+        with pytest.raises(RuntimeError):
+            f(first, *args[1:]).float().sum().backward()
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(lambda t: f(t, *args[1:]), (args[0],), (torch.ones_like(args[0]),))

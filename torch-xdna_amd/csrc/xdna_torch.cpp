@@ -2,8 +2,8 @@
 // trip through Python: the checks, the output, the workspace, the stream. A small call is all host time: one row
 // through 1024 x 4096 4-bit weights takes 4.5 us on the GPU, and took 15 to issue from Python.
 //
-// Registered for CUDA (the work) and AutogradCUDA (nothing but the dispatch below it; outputs of inputs that need a
-// gradient get a node that raises when it is asked for). Python's registrations of the ops give them their schemas,
+// Registered for CUDA (the work), AutogradCUDA and AutogradCPU (nothing but the dispatch below them; outputs of inputs
+// that need a gradient get a node that raises when it is asked for, and a tangent raises at once). Python's registrations of the ops give them their schemas,
 // their host kernels and their shapes under fake tensors.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -277,6 +277,10 @@ Tensor logits_adjust(const Tensor& logits, const OptTensor& tokens, const OptTen
 }
 
 // ------------------------------------------------------------------------------ autograd
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <class T>
+bool has_tangent(const T&) { return false; }
 bool needs_grad(const Tensor& t) { return t.requires_grad(); }
 bool needs_grad(const OptTensor& t) { return t && t->requires_grad(); }
 template <class T>
@@ -300,6 +304,7 @@ template <class... A>
 template <int OP>
 Tensor Below<Tensor(A...)>::call(c10::DispatchKeySet ks, A... a) {
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAMES[OP], "").typed<Tensor(A...)>();
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(a) || ...), NAMES[OP], " has no forward-mode derivative");
   Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -324,12 +329,15 @@ TORCH_LIBRARY_IMPL(xdna, CUDA, m) {
   m.impl("logits_adjust", logits_adjust);
 }
 
-TORCH_LIBRARY_IMPL(xdna, AutogradCUDA, m) {
+void autograd(torch::Library& m) {
   m.impl("linear_w4", TORCH_FN((&Below<decltype(linear_w4)>::call<0>)));
   m.impl("attention_causal", TORCH_FN((&Below<decltype(attention_causal)>::call<1>)));
   m.impl("attention_prefix", TORCH_FN((&Below<decltype(attention_prefix)>::call<2>)));
   m.impl("logits_adjust", TORCH_FN((&Below<decltype(logits_adjust)>::call<3>)));
 }
+
+TORCH_LIBRARY_IMPL(xdna, AutogradCUDA, m) { autograd(m); }
+TORCH_LIBRARY_IMPL(xdna, AutogradCPU, m) { autograd(m); }     // Python's own way past autograd drops tangents there too
 
 extern "C" {
 

@@ -8,10 +8,12 @@
 
 Each is also the op torch.ops.xdna.<name>, opaque to torch.compile. Tensors on a GPU go to the HIP
 kernels (csrc/xdna_torch.cpp checks the arguments there as the functions here do), on torch's current stream, without
-synchronizing; a GPU tensor with the library missing raises. Host tensors are computed here with plain torch in float32. There is no backward pass: a call that needs a
-gradient raises where the gradient is asked for. Wrong arguments raise ValueError or TypeError before anything is
-launched; what lies in GPU memory (lengths, starts, token ids) is not read on the host, and the kernels
-clamp it, so that no value of it reads or writes out of range.
+synchronizing; a GPU tensor with the library missing raises. Host tensors are computed here with plain torch in
+float32. The ops have no derivatives, on the GPU and on the host: a gradient raises where it is asked for, a
+forward-mode tangent at the call. (Called here with host tensors the functions are plain torch, derivatives
+included.) Wrong arguments raise ValueError or TypeError before anything is launched; what lies in GPU memory (lengths,
+starts, token ids) is not read on the host, and the kernels clamp it, so that no value of it reads or writes out of
+range.
 """
 
 import math
