@@ -40,3 +40,39 @@ def test_continuations_host():
 def test_continuations(gpu):
     _check(gpu)
     _check(gpu, vocab=1001, width=256, layers=3, heads=6, kv=1, dim=64, inner=512, dtype=torch.float16)
+
+
+def _small(**sizes):
+    return C.Decoder(**{**dict(vocab=300, width=128, layers=1, heads=4, kv=2, dim=32, inner=64), **sizes})
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_fewer_tokens_allowed_than_continuations(device):
+    """Every token is one that may be chosen, also where fewer may than there are continuations (or tokens at all): the
+    others begin with the likeliest."""
+    torch.manual_seed(0)
+    model = _small().to(device)
+    prompt = torch.randint(0, 300, (11,)).to(torch.int32).to(device)
+    for tokens in ([5], [299], [5, 64, 200]):
+        allowed = torch.zeros(10, dtype=torch.int64)
+        for t in tokens:
+            allowed[t // 32] |= 1 << t % 32
+        allowed = allowed.to(torch.int32).to(device)
+        out = C.continuations(model, prompt, 5, 4, allowed=allowed)
+        assert set(out.flatten().tolist()) <= set(tokens)
+        first = out[:, 0].tolist()
+        assert set(first) == set(tokens) and first[len(tokens):] == first[:1] * (5 - len(tokens))
+    out = C.continuations(_small(vocab=3).to(device), prompt % 3, 5, 2)
+    assert set(out[:, 0].tolist()) == {0, 1, 2} and bool((out < 3).all())
+
+
+def test_no_token_allowed():
+    model, prompt = _small(), torch.arange(7, dtype=torch.int32)
+    none = torch.zeros(10, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        C.continuations(model, prompt, 2, 3, allowed=none)
+    none[9] = -1 << 12                                  # tokens 300 .. 319, which there are not
+    with pytest.raises(ValueError):
+        C.continuations(model, prompt, 2, 3, allowed=none)
+    none[9] = 1 << 11
+    assert bool((C.continuations(model, prompt, 2, 3, allowed=none) == 299).all())

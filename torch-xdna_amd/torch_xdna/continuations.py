@@ -101,11 +101,23 @@ class Decoder(torch.nn.Module):
         return self.head(norm(x))
 
 
+def likeliest(scores, n):
+    """The n likeliest tokens of the scores [V]; past those that there are, and that may be chosen, the first of them again."""
+    top = scores.topk(min(n, scores.shape[0]))
+    tokens = torch.where(top.values == -torch.inf, top.indices[:1], top.indices)
+    return torch.cat([tokens, tokens[:1].expand(n - tokens.shape[0])])
+
+
 @torch.no_grad()
 def continuations(model, prompt, batch, steps, repetition=1.1, presence=0.1, frequency=0.1, allowed=None):
-    """`batch` continuations [batch, steps] (int32) of the tokens `prompt` [P]: the first tokens are the `batch` likeliest, each
-    later one the likeliest after its own. allowed: a mask [ceil(V / 32)] of the tokens that may be chosen, or None."""
+    """`batch` continuations [batch, steps] (int32) of the tokens `prompt` [P]: the first tokens are the `batch` likeliest (where
+    there are fewer, the likeliest again), each later one the likeliest after its own. allowed: a mask [ceil(V / 32)] of the
+    tokens that may be chosen, at least one (read on the host, once), or None."""
     dev, p = prompt.device, prompt.shape[0]
+    if allowed is not None:
+        bits = allowed.unsqueeze(-1) >> torch.arange(32, dtype=torch.int32, device=dev) & 1
+        if not bool(bits.flatten()[:model.vocab].any()):
+            raise ValueError("the mask allows no token")
     logits, prefix = model.prefill(prompt)
     own = [tuple(torch.zeros(batch, steps, *t.shape[1:], dtype=t.dtype, device=dev) for t in kv) for kv in prefix]
     said = torch.zeros(batch, p + steps, dtype=torch.int32, device=dev)
@@ -116,7 +128,7 @@ def continuations(model, prompt, batch, steps, repetition=1.1, presence=0.1, fre
     logits = logits[-1:].expand(batch, -1)
     for i in range(steps):
         scores = lm.logits_adjust(logits, said, lens + p, *settings, None, mask)
-        tokens = scores[0].topk(batch).indices if i == 0 else scores.argmax(-1)
+        tokens = likeliest(scores[0], batch) if i == 0 else scores.argmax(-1)
         said[:, p + i] = tokens.to(torch.int32)
         if i + 1 < steps:
             logits = model.step(tokens, prefix, own, lens)
