@@ -363,7 +363,9 @@ int xdna_add_rmsnorm_bf16(float* x, const float* a, int64_t rows, int64_t d, con
  * (q[n][k] - zeros[n][g]) * x[m][k], plus bias[n], float32 sums, in x_dtype (F32 / BF16 / F16), y contiguous.
  * qweight [n][k / 2]: two weights a byte, the even k in the low nibble; group a multiple of 32 that divides k; scales
  * [n][k / group] of s_dtype, zeros [n][k / group] uint8 or NULL (8), bias NULL or of bias_dtype. x rows (stride ldx)
- * and qweight 16-byte aligned. No counterpart in the reference. */
+ * and qweight 16-byte aligned; k and ldx at most 2^22, n 2^26. Sums that are not finite before their scale (x not finite, or
+ * next to the type's largest) are formed again from (q - zero) * scale: slow, but as the formula has it. No counterpart in
+ * the reference. */
 int xdna_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* qweight, const void* scales, int s_dtype,
                    const void* zeros, const void* bias, int bias_dtype, void* y, int64_t m, int64_t n, int64_t k,
                    int64_t group, void* stream);

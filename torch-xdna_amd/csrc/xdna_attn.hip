@@ -7,8 +7,10 @@
 //   out = sum over seen keys j of p_j v_j / sum of p_j,   p_j = 2^(c (s_j - m)),  s_j = q . k_j,  c = scale log2 e
 //
 // with m the running maximum of s (one pass over the keys; sums and outputs rescaled when it grows), float32
-// throughout except for p, which is rounded to the inputs' type for its product with V on the matrix units. A row that
-// sees nothing, or only scores of -inf, is zero.
+// throughout except for p, which is rounded to the inputs' type for its product with V: the matrix units take it no
+// wider, and two such halves of it would be twice the products. The sum of p is that of the rounded ones. Against 64 bits the
+// outputs' error grows from 0.0015 - 0.0017 of their norm with p in float32 to 0.0018 - 0.0022 in bfloat16, from 0.0002 to
+// 0.00024 - 0.00028 in float16. A row that sees nothing, or only scores of -inf, is zero.
 //
 // A wave has 32 rows: rows of a kv head are the pairs (token, q head of its group), so the heads that share K and V
 // share their loads. MFMA 32x32x16 (srcA = X, srcB = Y) gives lane l row l % 32 of Y and, in element 4 g + r, row
@@ -167,7 +169,7 @@ __device__ __forceinline__ void add_not_finite(f32x16a (&o)[D / 32], const float
 
 // Attention of 32 rows by KW waves: wave w has the tiles w, w + KW, ... of 32 keys, in LDS of its own (kl_, vl_: KW
 // tiles of K, and of V, each an array, so that the compiler knows which loads a read has to wait for), and the waves
-// meet in LDS at the end (meet: KW x 32 x D float32, which may lie over the tiles; ml: 2 KW x 64). No barriers before
+// meet there at the end (O over the tiles; ml: 2 KW x 64 maxima and sums). No barriers before
 // that: K of a wave's next tile loads once its scores are done, V after its products. store(chunk, o, m, l) receives
 // dims 8 (chunk % 4) + 32 (chunk / 4) + 4 (lane / 32) .. + 3 of the lane's row: the sum of p v, the maximum and the
 // sum of p.
@@ -323,7 +325,9 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
 //
 // What bounds it: a tile is 32 MFMAs (1024 cycles; heads of 64: 512) and about 130 vector instructions, 32 exps among
 // them, for a wave. Heads of 128: the card's power (1 x 16384, 16 / 8 heads: 1020 us, 1080 TFLOP/s, MFMA busy 57% at
-// 1.76 GHz); heads of 64 the vector units (8192, 16 / 8 heads: 199 us, 690 TFLOP/s). The maximum follows once a tile;
+// 1.76 GHz); heads of 64 no one unit (4096 / 1500 / 700, 12 heads: 57.5 us, 523 TFLOP/s; vector units active 52% of the CUs'
+// busy time, MFMA 28%, waves waiting 29% of theirs, 1.7 of them a SIMD; 8192, 16 / 8 heads: 199 us, 690 TFLOP/s). The maximum
+// follows once a tile;
 // l sums the p that are rounded, two at a time by a dot product with ones. With the masked tiles in the same loop the
 // compiler kept two sets of O (64 moves a tile: 1160 us).
 //
@@ -727,8 +731,9 @@ struct PrefixArgs {
 // time, or 128 (WIDE); the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a
 // workgroup takes all the keys of its (sequence, kv head) and writes the output itself. KW: waves that share out
 // keys. Measured, with the join: 48 rows of 2 / 1 heads of 128 on 8 kv heads over 4096 shared keys and up to 700 own
-// ones 25.6 us (86 MB, 3.4 TB/s); 24 rows of 8 / 1 heads of 64 on 4 over 100000 43 us (107 MB, 2.5 TB/s), bound by
-// the softmax's vector instructions and by six waves on four SIMDs.
+// ones 26 to 28 us (86 MB, 3.2 TB/s), waves waiting 41% of their time; 24 rows of 8 / 1 heads of 64 on 4 over 100000 44 to 47 us
+// (107 MB, 2.4 TB/s), vector units active 49% of the CUs' busy time, MFMA 25%, waves waiting 39% of theirs, and six waves of
+// rows in blocks of four.
 template <int DT, int D, bool WIDE, int KW>
 __global__ __launch_bounds__(KW * 64, 2) void prefix_kernel(PrefixArgs a) {
   static_assert(!WIDE || KW == 4, "four waves in the wide form");

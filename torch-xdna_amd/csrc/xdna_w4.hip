@@ -148,7 +148,7 @@ constexpr int W4_ROW_GROUPS = 4096;   // scales and zero points of a workgroup
 // shuffles, waves in LDS, both in a fixed order.
 // What a CU's address unit can take bounds such a kernel as much as the memory: a load costs it 16 cycles at least,
 // however little it fetches. So x, the scales and the zero points come into LDS once per workgroup, line by line, by
-// pieces of PB blocks (with a lane's own loads of them 1 x 4096 -> 14336 takes 24 us, so 15).
+// pieces of PB blocks (with a lane's own loads of them 1 x 4096 -> 14336 took 24 us, so 12.5).
 template <int DT, bool S4, int KL, int R>
 __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
   constexpr int W = 8, CL = 64 / KL;                    // waves, columns of a load
@@ -367,7 +367,9 @@ __global__ __launch_bounds__(512) void w4_row_kernel(W4Args a) {
 // step's four quarters are 32 consecutive k. Two tiles' x (DMA into LDS) and weights are on their way while a third is
 // used. Scales and zero points come into LDS for WIN k at a time. FL: steps (32 k each) of a group's sum
 // before its scale: 4 where G % 128 == 0, 2 where G % 64 == 0, else 1. Measured with the join: 40 x 14336 -> 4096 in
-// float16 23 us (33.6 MB), 8 x 4096 -> 14336 in bfloat16 13.0 us (33 MB): latency, eight waves a CU.
+// float16 23 us (33.6 MB), 8 x 4096 -> 14336 in bfloat16 13.8 us (33 MB). Counted: 40 rows about 190 vector instructions a
+// wave and 128 k against 12 MFMAs, 1 x 4096 -> 14336 about 200 a wave and 256 k against 16; vector units active 48% and 52%
+// of the CUs' busy time, MFMA 11% and 15%, and waves wait 43% of theirs in both: two waves a SIMD hide neither in the other.
 // KG groups of four waves share out a part's tiles (group GI the GI-th run of them), each with LDS of its own, and meet in
 // LDS at the end: as good as more parts, without their join. All groups pass the same barriers, whatever tiles there are.
 template <int DT, bool S4, int MT, int FL, int KG, int GI>
@@ -633,20 +635,20 @@ struct W4Plan {
   int mt, kg, parts;    // w4_tile_kernel's row blocks of 16, groups of waves and split of K
 };
 
-// One row: the row kernel, but for 16-bit rows and 32 columns a CU (8192) or more (1 x 4096 -> 14336, bfloat16: row
-// 15.2, tiles 14.0 us; 1 x 512 -> 14336 6.8 / 5.9; 1 x 14336 -> 4096 11.8 / 16.5; 1 x 4096 -> 14336 in float32 12.9 /
-// 36). Two to four rows: where the weights are few (3 x 1504 -> 1001 in float32 9.3 / 14.9 us, 4 x 8192 -> 512 7.4 /
-// 10.1, 4 x 4096 -> 4096 12.4 / 10.0). Its lanes along K: 64, so that long K makes waves enough, or 16 where the
-// columns do (4096 -> 14336 in bfloat16: 15.2 with 16, 19.0 with 64; 14336 -> 4096: 25 / 11.8), and more waves along
-// K below four a CU (14336 -> 64: one wave 9.2 us, four 5.8).
+// One row: the row kernel, but for 16-bit rows and 32 columns a CU (8192) or more (bfloat16, row / tiles: 1 x 4096 -> 14336
+// 12.5 / 12.6 us; 1 x 512 -> 14336 5.4 / 5.7; 1 x 14336 -> 4096 12.4 / 14.1; float32 1 x 4096 -> 14336 13.3 / 38.6). Two to four
+// rows: where the weights are few (3 x 1504 -> 1001 in float32 8.7 / 9.2 us, 4 x 8192 -> 512 in bfloat16 9.4 / 8.2,
+// 4 x 4096 -> 4096 12.4 / 9.3). Its lanes along K: 64, so that long K makes waves enough, or 16 where the columns do (4096 ->
+// 14336 in bfloat16: 12.5 with 16, 15.9 with 64; 14336 -> 4096: 19.9 / 12.4), and more waves along K below four a CU (14336 ->
+// 64: one wave 8.3 us, four 5.5).
 //
 // Tiles of 16-bit rows: two groups of waves share out K from 512 k on, unless there are two workgroups a CU without
-// (1 x 4096 -> 14336: one group 16.0 us, two 12.6, four 12.6; 64 x 4096 -> 14336 32.4 / 25.7), and K goes in parts on
+// (1 x 4096 -> 14336: one group 15.6 us, two 12.6, four no better; 64 x 4096 -> 14336 31.6 / 26.4), and K goes in parts on
 // top until there is a workgroup a CU, none under 512 k, 16 at most (40 x 14336 -> 4096 with two groups: 3 / 4 / 8 parts
-// 29.2 / 23.2 / 26.4 us, of which 3.5 the joining; 2 x 14336 -> 1000: 8 / 16 parts 10.6 / 9.4; 5 x 992 -> 2000: 7.3
+// 29.1 / 23.3 / 26.7 us, of which 4.0 the joining; 2 x 14336 -> 1000: 8 / 16 parts 11.0 / 9.6; 5 x 992 -> 2000: 7.5
 // with one). float32, whose tiles take three times the work: parts alone, up to two workgroups a CU and 16 parts, none
-// under 128 k (14 x 1536 -> 138: 1 / 4 / 8 / 12 parts 22.2 / 10.0 / 8.4 / 7.7 us; 8 x 4096 -> 4096 16.5 with
-// 4, 15.1 with 8).
+// under 128 k (14 x 1536 -> 138: 1 / 4 / 8 / 12 parts 22.3 / 10.3 / 8.7 / 8.0 us; 8 x 4096 -> 4096 16.7 with
+// 4, 15.5 with 8).
 W4Plan w4_plan(int64_t M, int64_t N, int64_t K, bool f32) {
   W4Plan p{};
   const int64_t cus = device_cus();

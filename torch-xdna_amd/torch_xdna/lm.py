@@ -77,7 +77,10 @@ def quantize_w4(weight, group=128, symmetric=False):
 def linear_w4(x, qweight, scales, zeros=None, bias=None):
     """y [..., N] = x [..., K] times the transpose of (q - zero) * scale, plus bias [N], summed in float32 and rounded
     once to x's dtype. qweight uint8 [N, K / 2] (the even k of a byte in its low nibble), scales [N, K / G] with G a
-    multiple of 32, zeros uint8 [N, K / G] or None for 8; qweight, scales and zeros contiguous."""
+    multiple of 32, zeros uint8 [N, K / G] or None for 8; qweight, scales and zeros contiguous.
+    On the GPU x is read where it lies if its rows are dense, start on 16 bytes, do not overlap and are at most 2^22
+    elements apart, else copied first. Rows whose x is not finite, or next to its type's largest, take long: their sums
+    are formed a second time, value by value."""
     if x.is_cuda:
         return _on_gpu("linear_w4", x, qweight, scales, zeros, bias)
     _floats("x", x)
@@ -149,10 +152,13 @@ def _softmax_v(scores, seen, v):
 
 
 def attention_causal(q, k, v, starts, scale=None):
-    """Causal attention of packed prompts: out [T, H, D] of q [T, H, D] and k, v [T, KV, D] (bfloat16 or float16, any
-    strides; H a multiple of KV, q head h with kv head h / (H / KV); D a multiple of 8, at most 128). starts int32 [S + 1]: the first
+    """Causal attention of packed prompts: out [T, H, D] of q [T, H, D] and k, v [T, KV, D] (bfloat16 or float16; H a
+    multiple of KV, q head h with kv head h / (H / KV); D a multiple of 8, at most 128). starts int32 [S + 1]: the first
     token of each sequence, ascending, and T. A token sees its own sequence's tokens up to itself. scale: 1 / sqrt(D) if
-    None. Float32 sums; the softmax's weights are rounded to q's dtype for their product with v, and the result once."""
+    None. Float32 sums, and the result rounded once; on the GPU the softmax's weights are rounded to q's dtype for their
+    product with v, on the host they are not.
+    Any strides; but on the GPU a tensor is copied at every call, a whole cache too, unless its last dim is dense, it starts
+    on 16 bytes, its other strides are multiples of 8, and its tokens lie D to 2^24 - 1 elements apart."""
     if q.is_cuda:
         return _on_gpu("attention_causal", q, k, v, starts, scale)
     if q.dim() != 3 or k.dim() != 3 or tuple(v.shape) != tuple(k.shape):
@@ -181,7 +187,8 @@ def attention_causal(q, k, v, starts, scale=None):
 def attention_prefix(q, kp, vp, kc, vc, lens, scale=None):
     """One decode step's attention of B sequences that share a prefix: out [B, H, D] of q [B, H, D] (the new tokens'), kp, vp
     [P, KV, D] (the prefix's, held once) and kc, vc [B, S, KV, D], of which sequence b sees the first lens[b] (int32 [B]; clamped to
-    0 .. S; the new token's own among them). P and S may be 0. Types, scale and rounding as in attention_causal."""
+    0 .. S; the new token's own among them). P and S may be 0. Types, scale, rounding and strides (those of sequences: any
+    multiple of 8) as in attention_causal."""
     if q.is_cuda:
         return _on_gpu("attention_prefix", q, kp, vp, kc, vc, lens, scale)
     if q.dim() != 3 or kp.dim() != 3 or kc.dim() != 4 or tuple(vp.shape) != tuple(kp.shape) or tuple(vc.shape) != tuple(kc.shape):
@@ -214,7 +221,7 @@ def logits_adjust(logits, tokens=None, lens=None, repetition=None, presence=None
     the grammar's bit is 0. In float32, rounded once to logits' dtype (float32, bfloat16 or float16).
     tokens int32 or int64 [B, L] with lens int32 [B] (clamped to 0 .. L; ids outside 0 .. V - 1 count nowhere); repetition,
     presence, frequency float32 [B]; bias float32 [V] or [B, V]; allowed int32 [B, ceil(V / 32)], token v at bit v % 32 of
-    word v / 32. Each may be None."""
+    word v / 32. Each may be None. All three penalties count the same history."""
     if logits.is_cuda:
         return _on_gpu("logits_adjust", logits, tokens, lens, repetition, presence, frequency, bias, allowed)
     _floats("logits", logits)
