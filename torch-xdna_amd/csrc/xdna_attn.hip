@@ -731,7 +731,7 @@ struct PrefixArgs {
 // time, or 128 (WIDE); the others a part of a sequence's own keys for the q heads of a kv head. np == no == 0: a
 // workgroup takes all the keys of its (sequence, kv head) and writes the output itself. KW: waves that share out
 // keys. Measured, with the join: 48 rows of 2 / 1 heads of 128 on 8 kv heads over 4096 shared keys and up to 700 own
-// ones 26 to 28 us (86 MB, 3.2 TB/s), waves waiting 41% of their time; 24 rows of 8 / 1 heads of 64 on 4 over 100000 44 to 47 us
+// ones 26 to 28 us (86 MB, 3.2 TB/s), waves waiting 41% of their time; 24 rows of 8 / 1 heads of 64 on 4 over 100000 43 to 47 us
 // (107 MB, 2.4 TB/s), vector units active 49% of the CUs' busy time, MFMA 25%, waves waiting 39% of theirs, and six waves of
 // rows in blocks of four.
 template <int DT, int D, bool WIDE, int KW>
