@@ -410,6 +410,54 @@ int xdna_logits_adjust(const void* logits, int dtype, int64_t ld, const void* to
                        const float* bias, int64_t ldb, const int32_t* allowed, int64_t lda, void* y, int64_t B, int64_t V,
                        void* stream);
 
+/* Heads turned to their positions, y [T, heads, d] (contiguous) of x [T, heads, d] (strides in elements, the last dim dense; dtype
+ * F32 / BF16 / F16): pair j < half, theta = positions[t] * freqs[j] (formed in float64, good while it is below 2^50),
+ *   (a, b) -> magnitude * (a cos theta - b sin theta, b cos theta + a sin theta) of dims j, half + j (interleaved: 2 j, 2 j + 1),
+ * in float32, rounded once; dims from 2 half on are copied. positions int32 or int64 (wide = 1); freqs float64 [half], radians a
+ * position; half at most 1024. No counterpart in the reference. */
+int xdna_rotary(const void* x, int dtype, int64_t x_token, int64_t x_head, const void* positions, int wide, const double* freqs,
+                int64_t half, float magnitude, int interleaved, void* y, int64_t T, int64_t heads, int64_t d, void* stream);
+
+/* A block's output o added to the residual stream x, and the norm that the next block reads, float32 inside:
+ *   n = post ? post * o / sqrt(mean(o^2) + eps) : o;   sum = x + scale * gate * n;   y = weight * sum / sqrt(mean(sum^2) + eps)
+ * of the sum before it is rounded. x and sum are of x_dtype, o, gate and y of dtype (x_dtype the same, or F32), post and
+ * weight [width] of post_dtype and weight_dtype. Row r starts at (r / inner) * outer stride + (r % inner) * inner stride; strides
+ * (elements): {x outer, x inner, o outer, o inner, gate outer, gate inner} (0, 0: one for all rows); sum and y are
+ * contiguous. o NULL: sum = x, and nothing is written to it (NULL); gate, post and weight NULL: 1, no norm, 1. width at most
+ * 32768. No counterpart in the reference. */
+int xdna_residual_norm(const void* x, int x_dtype, const void* o, int dtype, const void* gate, const int64_t* strides, int64_t inner,
+                       const void* post, int post_dtype, const void* weight, int weight_dtype, float scale, float eps, void* sum,
+                       void* y, int64_t rows, int64_t width, void* stream);
+
+/* New tokens go into a paged cache of keys and values in 8 bits. The cache (page: its tokens G, 16 / 32 / 64 / 128):
+ *   kpages int8 [pages, nkv, G, d], vpages int8 [pages, nkv, d, G], kscales, vscales float32 [pages, nkv]: x ~= q * scale, with
+ *     scale = max|x| / 127 over a page of a head (0: all zero; NaN: a value was not finite), q = round_half_even(x / scale);
+ *   ktail [B, nkv, R, d], vtail [B, nkv, d, R] of dtype (BF16 / F16), R a multiple of G: position p of text b at place p % R, the
+ *     last R tokens of every text; an open page's tokens are read from here until its last one comes;
+ *   table int32 [B, P] (ldt from row to row): the page of positions G j .. G j + G - 1 of text b. A page that new tokens complete
+ *     must be in one text only. One outside 0 .. pages - 1 is not written, tokens past P G are dropped.
+ * k, v [T, nkv, d] (strides: {k token, k head, v token, v head, q token, q head}, elements, the last dim dense) are the tokens
+ * starts[b] .. starts[b + 1] - 1 of text b (starts [B + 1] int32, ascending; NULL: T / B each), at positions lens[b] (clamped to 0 ..
+ * P G) and on. Keys turn to them as by xdna_rotary (freqs [half]; half 0: as they are) and are rounded to dtype. q [T, nh, d] or
+ * NULL: turned the same way into q_out (contiguous); rows of no text are zero. d a multiple of 16, at most 128. lens stays as it
+ * is: the caller adds. No counterpart in the reference. */
+int xdna_cache_append(const void* k, const void* v, int dtype, const int64_t* strides, void* kpages, void* vpages, float* kscales,
+                      float* vscales, void* ktail, void* vtail, const int32_t* table, int64_t ldt, const int32_t* lens,
+                      const int32_t* starts, const void* q, const double* freqs, int64_t half, float magnitude, int interleaved,
+                      void* q_out, int64_t T, int64_t B, int64_t P, int64_t pages, int64_t page, int64_t R, int nh, int nkv, int d,
+                      void* stream);
+
+/* Attention of the newest N tokens of each of B texts over such a cache, which holds them already: out [B, N, nh, d] (contiguous)
+ * of q [B, N, nh, d] (strides {text, token, head}, multiples of 8; 16-byte aligned). Token n of text b sees positions 0 ..
+ * lens[b] - N + n (lens clamped to 0 .. P G); a page outside 0 .. pages - 1 is seen by no one. Float32 sums; p rounds to dtype
+ * for its product with v. Rows that see nothing, or only scores of -inf, are zero. ws: xdna_attention_cache_ws_bytes(..) bytes (0:
+ * none needed) that the call may overwrite, 16-byte aligned. No counterpart in the reference. */
+int64_t xdna_attention_cache_ws_bytes(int64_t B, int64_t N, int nh, int nkv, int d, int64_t P, int64_t page);
+int xdna_attention_cache(const void* q, int dtype, const int64_t* strides, const void* kpages, const void* vpages, const float* kscales,
+                         const float* vscales, const void* ktail, const void* vtail, const int32_t* table, int64_t ldt,
+                         const int32_t* lens, int64_t B, int64_t N, int64_t P, int64_t pages, int64_t page, int64_t R, int nh, int nkv,
+                         int d, float scale, void* out, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -276,6 +276,203 @@ Tensor logits_adjust(const Tensor& logits, const OptTensor& tokens, const OptTen
   return y;
 }
 
+// ------------------------------------------------------------------------------ rotary
+void check_freqs(const Tensor& freqs, int64_t d) {
+  TORCH_CHECK_TYPE(freqs.scalar_type() == at::kDouble, "freqs must be float64, got ", freqs.scalar_type());
+  TORCH_CHECK_VALUE(freqs.dim() == 1 && 2 * freqs.size(0) <= d, "freqs must be [R / 2] with R at most the heads' ", d, " dims, got ",
+                    freqs.sizes());
+}
+
+// t whose last dim is dense and whose strides are not negative: itself, or a copy
+Tensor dense(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+Tensor rotary(const Tensor& x, const Tensor& positions, const Tensor& freqs, double magnitude, bool interleaved) {
+  Record rec;
+  check_float("x", x);
+  TORCH_CHECK_TYPE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "positions must be int32 or int64, got ",
+                   positions.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 3, "rotary takes x [.., H, D], got ", x.sizes());
+  const int64_t d = x.size(-1), h = x.size(-2);
+  check_freqs(freqs, d);
+  TORCH_CHECK_VALUE(freqs.size(0) <= 1024, "rotary turns at most 1024 pairs, got ", freqs.size(0));
+  check_shape("positions", positions, x.sizes().slice(0, x.dim() - 2));
+  check_device(x, positions), check_device(x, freqs);
+  const Launch go(x);
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return y;
+  const int64_t t = x.numel() / (h * d);
+  rec.macs = 2 * t * h * freqs.size(0);
+  const Tensor xs = dense(x.dim() == 3 ? x : x.reshape({t, h, d})), ps = positions.contiguous(), fs = freqs.contiguous();
+  done(xdna_rotary(xs.const_data_ptr(), code(x.scalar_type()), xs.stride(0), xs.stride(1), ps.const_data_ptr(),
+                   ps.scalar_type() == at::kLong, fs.const_data_ptr<double>(), fs.size(0), (float)magnitude, interleaved,
+                   y.mutable_data_ptr(), t, h, d, go.stream),
+       "rotary");
+  rec.launched = true;
+  return y;
+}
+
+// ------------------------------------------------------------------------------ residual_norm
+std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& o, const OptTensor& weight, const OptTensor& post,
+                                         const OptTensor& gate, double scale, double eps) {
+  Record rec;
+  check_float("x", x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) <= 32768, "residual_norm takes x [.., W] with W at most 32768, got ", x.sizes());
+  TORCH_CHECK_VALUE(o || (!post && !gate), "residual_norm: post and gate need o");
+  const int64_t w = x.size(-1);
+  if (o) {
+    check_float("o", *o);
+    TORCH_CHECK_TYPE(x.scalar_type() == o->scalar_type() || x.scalar_type() == at::kFloat, "x must be of o's type or float32, got ",
+                     x.scalar_type(), " and ", o->scalar_type());
+    check_shape("o", *o, x.sizes());
+  }
+  for (const auto& [name, t] : {std::pair<const char*, const OptTensor*>{"weight", &weight}, {"post", &post}})
+    if (*t) {
+      check_float(name, **t);
+      check_shape(name, **t, {w});
+    }
+  if (gate) {
+    TORCH_CHECK_TYPE(gate->scalar_type() == o->scalar_type(), "gate must be of o's type, got ", gate->scalar_type());
+    TORCH_CHECK_VALUE(gate->sizes() == x.sizes() || (gate->dim() == 1 && gate->size(0) == w), "gate must have shape ", x.sizes(), " or [",
+                      w, "], got ", gate->sizes());
+  }
+  for (const OptTensor* t : {&o, &weight, &post, &gate}) check_device(x, *t);
+  const Launch go(x);
+  const auto ot = o ? o->options() : x.options();
+  Tensor sum = o ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options()), y = at::empty(x.sizes(), ot);
+  if (x.numel() == 0) return {sum, y};
+  const int64_t rows = x.numel() / w, inner = x.dim() >= 2 ? x.size(-2) : 1;
+  // as [outer, inner, W]: where that is no view of it, or the last dim is not dense, a copy
+  int64_t st[6] = {0, 0, 0, 0, 0, 0};
+  const auto shaped = [&](const Tensor& t, int64_t* s) {
+    const Tensor v = dense(t.dim() == 3 ? t : t.reshape({rows / inner, inner, w}));
+    s[0] = v.stride(0), s[1] = v.stride(1);
+    return v;
+  };
+  const Tensor xs = shaped(x, st), os = o ? shaped(*o, st + 2) : Tensor();
+  Tensor gs;
+  if (gate && gate->dim() == 1 && x.dim() != 1) gs = gate->contiguous();
+  else if (gate) gs = shaped(*gate, st + 4);
+  const Tensor ws = weight ? weight->contiguous() : Tensor(), ps = post ? post->contiguous() : Tensor();
+  const auto at = [](const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; };
+  const auto type = [](const Tensor& t) { return t.defined() ? code(t.scalar_type()) : XDNA_F32; };
+  done(xdna_residual_norm(at(xs), type(xs), at(os), code(y.scalar_type()), at(gs), st, inner, at(ps), type(ps), at(ws), type(ws),
+                          (float)scale, (float)eps, o ? sum.mutable_data_ptr() : nullptr, y.mutable_data_ptr(), rows, w, go.stream),
+       "residual_norm");
+  rec.launched = true;
+  return {sum, y};
+}
+
+// ------------------------------------------------------------------------------ the 8-bit cache
+struct CacheSizes {
+  int64_t b, p, pages, kv, g, d, r;
+};
+
+CacheSizes check_cache(const char* name, const Tensor& x, const Tensor& kpages, const Tensor& vpages, const Tensor& kscales,
+                       const Tensor& vscales, const Tensor& ktail, const Tensor& vtail, const Tensor& table, const Tensor& lens) {
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, name, " takes bfloat16 or float16, got ",
+                   x.scalar_type());
+  TORCH_CHECK_TYPE(kpages.scalar_type() == at::kChar && vpages.scalar_type() == at::kChar, "kpages and vpages must be int8");
+  TORCH_CHECK_TYPE(kscales.scalar_type() == at::kFloat && vscales.scalar_type() == at::kFloat, "kscales and vscales must be float32");
+  TORCH_CHECK_TYPE(ktail.scalar_type() == x.scalar_type() && vtail.scalar_type() == x.scalar_type(), "ktail and vtail must be ",
+                   x.scalar_type(), ", got ", ktail.scalar_type(), " and ", vtail.scalar_type());
+  TORCH_CHECK_VALUE(kpages.dim() == 4 && ktail.dim() == 4, "kpages must be [pages, KV, G, D] and ktail [B, KV, R, D], got ", kpages.sizes(),
+                    " and ", ktail.sizes());
+  check_whole("table", table, 2, "[B, P]");
+  const CacheSizes s{ktail.size(0), table.size(1), kpages.size(0), kpages.size(1), kpages.size(2), kpages.size(3), ktail.size(2)};
+  TORCH_CHECK_VALUE(s.g == 16 || s.g == 32 || s.g == 64 || s.g == 128, name, ": pages hold 16, 32, 64 or 128 tokens, got ", s.g);
+  TORCH_CHECK_VALUE(s.d >= 16 && s.d <= 128 && s.d % 16 == 0, name, ": head dims must be a multiple of 16, at most 128, got ", s.d);
+  TORCH_CHECK_VALUE(s.r >= s.g && s.r % s.g == 0 && s.r < 65536, name, ": R must be a multiple of ", s.g, " below 65536, got ", s.r);
+  TORCH_CHECK_VALUE(s.kv >= 1, name, ": no key heads");
+  TORCH_CHECK_VALUE(s.pages >= 1 || s.p == 0, name, ": a table of no pages");
+  check_shape("vpages", vpages, {s.pages, s.kv, s.d, s.g});
+  check_shape("kscales", kscales, {s.pages, s.kv});
+  check_shape("vscales", vscales, {s.pages, s.kv});
+  check_shape("ktail", ktail, {s.b, s.kv, s.r, s.d});
+  check_shape("vtail", vtail, {s.b, s.kv, s.d, s.r});
+  check_shape("table", table, {s.b, s.p});
+  check_whole("lens", lens, 1, "[B]");
+  check_shape("lens", lens, {s.b});
+  for (const Tensor* t : {&kpages, &vpages, &kscales, &vscales, &ktail, &vtail}) {
+    TORCH_CHECK_VALUE(t->is_contiguous() && reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0, name,
+                      ": the cache must be contiguous and 16-byte aligned");
+    check_device(x, *t);
+  }
+  check_device(x, table), check_device(x, lens);
+  return s;
+}
+
+Tensor cache_append(const Tensor& k, const Tensor& v, const Tensor& kpages, const Tensor& vpages, const Tensor& kscales,
+                    const Tensor& vscales, const Tensor& ktail, const Tensor& vtail, const Tensor& table, const Tensor& lens,
+                    const OptTensor& starts, const OptTensor& q, const OptTensor& freqs, double magnitude, bool interleaved) {
+  Record rec;
+  const CacheSizes s = check_cache("cache_append", k, kpages, vpages, kscales, vscales, ktail, vtail, table, lens);
+  TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type() && (!q || q->scalar_type() == k.scalar_type()),
+                   "cache_append: q, k and v must be of one dtype");
+  TORCH_CHECK_VALUE(k.dim() == 3 && k.sizes() == v.sizes(), "cache_append takes k, v [T, KV, D], got ", k.sizes(), " and ", v.sizes());
+  const int64_t t = k.size(0);
+  check_shape("k", k, {t, s.kv, s.d});
+  if (starts) {
+    check_whole("starts", *starts, 1, "[B + 1]");
+    check_shape("starts", *starts, {s.b + 1});
+  } else {
+    TORCH_CHECK_VALUE(s.b ? t % s.b == 0 : t == 0, "cache_append: ", t, " tokens are not the same number for each of ", s.b,
+                      " texts; starts must say which are whose");
+  }
+  if (freqs) check_freqs(*freqs, s.d);
+  if (q) {
+    TORCH_CHECK_VALUE(freqs, "cache_append: q turns with freqs, and there are none");
+    TORCH_CHECK_VALUE(q->dim() == 3 && q->size(1) >= 1, "q must be [T, H, D], got ", q->sizes());
+    check_shape("q", *q, {t, q->size(1), s.d});
+  }
+  check_device(k, v), check_device(k, starts), check_device(k, q), check_device(k, freqs);
+  const Launch go(k);
+  Tensor out = q ? at::empty(q->sizes(), k.options()) : at::empty({0}, k.options());
+  if (t == 0) return out;
+  if (s.b == 0) return out.zero_();
+  rec.macs = 2 * t * s.kv * s.d;
+  const Tensor ks = dense(k), vs = dense(v), qs = q ? dense(*q) : Tensor(), ls = lens.contiguous(), fs = freqs ? freqs->contiguous() : Tensor(),
+               ss = starts ? starts->contiguous() : Tensor(), ts = dense(table);
+  const int64_t st[6] = {ks.stride(0), ks.stride(1), vs.stride(0), vs.stride(1), q ? qs.stride(0) : 0, q ? qs.stride(1) : 0};
+  done(xdna_cache_append(ks.const_data_ptr(), vs.const_data_ptr(), code(k.scalar_type()), st, kpages.mutable_data_ptr(),
+                         vpages.mutable_data_ptr(), (float*)kscales.mutable_data_ptr(), (float*)vscales.mutable_data_ptr(),
+                         ktail.mutable_data_ptr(), vtail.mutable_data_ptr(), ts.const_data_ptr<int32_t>(), ts.stride(0),
+                         ls.const_data_ptr<int32_t>(), starts ? ss.const_data_ptr<int32_t>() : nullptr,
+                         q ? qs.const_data_ptr() : nullptr, freqs ? fs.const_data_ptr<double>() : nullptr, freqs ? fs.size(0) : 0,
+                         (float)magnitude, interleaved, q ? out.mutable_data_ptr() : nullptr, t, s.b, s.p, s.pages, s.g, s.r,
+                         q ? (int)q->size(1) : 0, (int)s.kv, (int)s.d, go.stream),
+       "cache_append");
+  rec.launched = true;
+  return out;
+}
+
+Tensor attention_cache(const Tensor& q, const Tensor& kpages, const Tensor& vpages, const Tensor& kscales, const Tensor& vscales,
+                       const Tensor& ktail, const Tensor& vtail, const Tensor& table, const Tensor& lens, std::optional<double> scale_) {
+  Record rec;
+  const CacheSizes s = check_cache("attention_cache", q, kpages, vpages, kscales, vscales, ktail, vtail, table, lens);
+  TORCH_CHECK_VALUE(q.dim() == 4, "attention_cache takes q [B, N, H, D], got ", q.sizes());
+  const int64_t n = q.size(1), h = q.size(2);
+  check_shape("q", q, {s.b, n, h, s.d});
+  TORCH_CHECK_VALUE(h && h % s.kv == 0, "attention_cache: ", h, " q heads do not share ", s.kv, " key heads evenly");
+  const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)s.d);
+  const Launch go(q);
+  Tensor out = at::empty(q.sizes(), q.options());
+  if (s.b == 0 || n == 0) return out;
+  rec.macs = 2 * s.b * n * h * s.d * s.p * s.g;        // at most: the lengths are not read
+  int64_t st[3];
+  const Tensor qs = heads(q, st), ls = lens.contiguous(), ts = dense(table);
+  const int64_t need = xdna_attention_cache_ws_bytes(s.b, n, (int)h, (int)s.kv, (int)s.d, s.p, s.g);
+  const Tensor ws = need > 0 ? bytes(q, need) : Tensor();
+  done(need < 0 ? (int)need
+                : xdna_attention_cache(qs.const_data_ptr(), code(q.scalar_type()), st, kpages.const_data_ptr(), vpages.const_data_ptr(),
+                                       kscales.const_data_ptr<float>(), vscales.const_data_ptr<float>(), ktail.const_data_ptr(),
+                                       vtail.const_data_ptr(), ts.const_data_ptr<int32_t>(), ts.stride(0), ls.const_data_ptr<int32_t>(),
+                                       s.b, n, s.p, s.pages, s.g, s.r, (int)h, (int)s.kv, (int)s.d, (float)scale, out.mutable_data_ptr(),
+                                       need > 0 ? ws.mutable_data_ptr() : nullptr, need, go.stream),
+       "attention_cache");
+  rec.launched = true;
+  return out;
+}
+
 // ------------------------------------------------------------------------------ autograd
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
@@ -290,32 +487,50 @@ void take(std::vector<Tensor>& v, const OptTensor& t) { if (t) v.push_back(*t); 
 template <class T>
 void take(std::vector<Tensor>&, const T&) {}
 
+void each(const Tensor& t, const std::shared_ptr<torch::autograd::Node>& node) { torch::autograd::set_history(t, node); }
+void each(const std::tuple<Tensor, Tensor>& t, const std::shared_ptr<torch::autograd::Node>& node) {
+  for (const Tensor& x : {std::get<0>(t), std::get<1>(t)}) torch::autograd::set_history(x, node);
+}
+
 template <class F>
 struct Below;
-template <class... A>
-struct Below<Tensor(A...)> {
+template <class R, class... A>
+struct Below<R(A...)> {
   template <int OP>
-  static Tensor call(c10::DispatchKeySet ks, A... a);
+  static R call(c10::DispatchKeySet ks, A... a);
 };
 
-constexpr const char* NAMES[] = {"xdna::linear_w4", "xdna::attention_causal", "xdna::attention_prefix", "xdna::logits_adjust"};
+constexpr const char* NAMES[] = {"xdna::linear_w4", "xdna::attention_causal", "xdna::attention_prefix", "xdna::logits_adjust",
+                                 "xdna::rotary", "xdna::residual_norm", "xdna::attention_cache", "xdna::cache_append"};
+constexpr int APPEND = 7;      // writes to its arguments 2 .. 7
 
 template <class... A>
+void written(const A&... a) {
+  const std::tuple<const A&...> t(a...);
+  for (const Tensor* x : {&std::get<2>(t), &std::get<3>(t), &std::get<4>(t), &std::get<5>(t), &std::get<6>(t), &std::get<7>(t)})
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+}
+
+template <class R, class... A>
 template <int OP>
-Tensor Below<Tensor(A...)>::call(c10::DispatchKeySet ks, A... a) {
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAMES[OP], "").typed<Tensor(A...)>();
+R Below<R(A...)>::call(c10::DispatchKeySet ks, A... a) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAMES[OP], "").typed<R(A...)>();
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(a) || ...), NAMES[OP], " has no forward-mode derivative");
-  Tensor out;
+  const bool grad = at::GradMode::is_enabled() && (needs_grad(a) || ...);
+  // what it writes would hold values of such inputs, with no way back to them
+  if (OP == APPEND) TORCH_CHECK_NOT_IMPLEMENTED(!grad, NAMES[OP], " has no derivative, and an input needs a gradient: call it under torch.no_grad()");
+  R out;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     out = op.redispatch(ks & c10::after_autograd_keyset, a...);
   }
-  if (at::GradMode::is_enabled() && (needs_grad(a) || ...)) {
+  if constexpr (OP == APPEND) written(a...);
+  if (grad) {
     std::vector<Tensor> in;
     (take(in, a), ...);
     auto node = std::shared_ptr<torch::autograd::NotImplemented>(new torch::autograd::NotImplemented(NAMES[OP]), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(in));
-    torch::autograd::set_history(out, node);
+    each(out, node);
   }
   return out;
 }
@@ -327,6 +542,10 @@ TORCH_LIBRARY_IMPL(xdna, CUDA, m) {
   m.impl("attention_causal", attention_causal);
   m.impl("attention_prefix", attention_prefix);
   m.impl("logits_adjust", logits_adjust);
+  m.impl("rotary", rotary);
+  m.impl("residual_norm", residual_norm);
+  m.impl("attention_cache", attention_cache);
+  m.impl("cache_append", cache_append);
 }
 
 void autograd(torch::Library& m) {
@@ -334,6 +553,10 @@ void autograd(torch::Library& m) {
   m.impl("attention_causal", TORCH_FN((&Below<decltype(attention_causal)>::call<1>)));
   m.impl("attention_prefix", TORCH_FN((&Below<decltype(attention_prefix)>::call<2>)));
   m.impl("logits_adjust", TORCH_FN((&Below<decltype(logits_adjust)>::call<3>)));
+  m.impl("rotary", TORCH_FN((&Below<decltype(rotary)>::call<4>)));
+  m.impl("residual_norm", TORCH_FN((&Below<decltype(residual_norm)>::call<5>)));
+  m.impl("attention_cache", TORCH_FN((&Below<decltype(attention_cache)>::call<6>)));
+  m.impl("cache_append", TORCH_FN((&Below<decltype(cache_append)>::call<APPEND>)));
 }
 
 TORCH_LIBRARY_IMPL(xdna, AutogradCUDA, m) { autograd(m); }

@@ -140,6 +140,13 @@ def _declare(L):
         "xdna_attention_prefix_ws_bytes": ([i64, i64, i64, i, i, i], i64),
         "xdna_attention_prefix": ([p, p, p, p, p, i, p, p, i64, i64, i64, i, i, i, ctypes.c_float, p, p, i64, p], i),
         "xdna_logits_adjust": ([p, i, i64, p, i, i64, i64, p, p, p, p, p, i64, p, i64, p, i64, i64, p], i),
+        "xdna_rotary": ([p, i, i64, i64, p, i, p, i64, ctypes.c_float, i, p, i64, i64, i64, p], i),
+        "xdna_residual_norm": ([p, i, p, i, p, p, i64, p, i, p, i, ctypes.c_float, ctypes.c_float, p, p, i64, i64, p], i),
+        "xdna_cache_append": ([p, p, i, p, p, p, p, p, p, p, p, i64, p, p, p, p, i64, ctypes.c_float, i, p, i64, i64, i64, i64, i64,
+                               i64, i, i, i, p], i),
+        "xdna_attention_cache_ws_bytes": ([i64, i64, i, i, i, i64, i64], i64),
+        "xdna_attention_cache": ([p, i, p, p, p, p, p, p, p, p, i64, p, i64, i64, i64, i64, i64, i64, i, i, i, ctypes.c_float, p, p,
+                                  i64, p], i),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -158,7 +165,8 @@ EXPORTS = ("xdna_abi_version", "xdna_last_error", "xdna_device_info", "xdna_quan
            "xdna_tile_set", "xdna_tile_get", "xdna_tile_plan", "xdna_tile_clear", "xdna_rmsnorm_bf16",
            "xdna_add_rmsnorm_bf16", "xdna_qk_norm_rope",
            "xdna_attention_bf16", "xdna_silu_mul_bf16", "xdna_add_f32", "xdna_linear_w4", "xdna_linear_w4_ws_bytes", "xdna_linear_w4_ws", "xdna_attention_causal",
-           "xdna_attention_prefix_ws_bytes", "xdna_attention_prefix", "xdna_logits_adjust")
+           "xdna_attention_prefix_ws_bytes", "xdna_attention_prefix", "xdna_logits_adjust", "xdna_rotary", "xdna_residual_norm",
+           "xdna_cache_append", "xdna_attention_cache_ws_bytes", "xdna_attention_cache")
 
 
 def _check(status, what):
@@ -804,8 +812,8 @@ def add_(x, y):
 
 
 # ------------------------------------------------------------------------------ language model operators
-# torch.ops.xdna.linear_w4, attention_causal, attention_prefix and logits_adjust reach the library from C++ (csrc/
-# xdna_torch.cpp), registered for GPU tensors when it is loaded.
+# torch.ops.xdna.linear_w4, attention_causal, attention_prefix, logits_adjust, rotary, residual_norm, cache_append and
+# attention_cache reach the library from C++ (csrc/xdna_torch.cpp), registered for GPU tensors when it is loaded.
 TORCH_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libxdna_torch.so")
 _torch_lib = None
 

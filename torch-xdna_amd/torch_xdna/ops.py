@@ -185,6 +185,64 @@ def _(logits, tokens=None, lens=None, repetition=None, presence=None, frequency=
     return logits.new_empty(logits.shape)
 
 
+@torch.library.custom_op("xdna::rotary", mutates_args=())
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, magnitude: float = 1.0,
+           interleaved: bool = False) -> torch.Tensor:
+    """lm.rotary: heads turned to their positions."""
+    return lm.rotary(x, positions, freqs, magnitude, interleaved)
+
+
+@rotary.register_fake
+def _(x, positions, freqs, magnitude=1.0, interleaved=False):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("xdna::residual_norm", mutates_args=())
+def residual_norm(x: torch.Tensor, o: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                  post: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0,
+                  eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """lm.residual_norm: the residual sum and the norms around it. Without o the sum is x, and the first result empty."""
+    s, y = lm.residual_norm(x, o, weight, post, gate, scale, eps)
+    return (x.new_empty(0) if o is None else s), y
+
+
+@residual_norm.register_fake
+def _(x, o=None, weight=None, post=None, gate=None, scale=1.0, eps=1e-6):
+    if o is None:
+        return x.new_empty(0), x.new_empty(x.shape)
+    return x.new_empty(x.shape), o.new_empty(x.shape)
+
+
+@torch.library.custom_op("xdna::cache_append", mutates_args=("kpages", "vpages", "kscales", "vscales", "ktail", "vtail"))
+def cache_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor,
+                 vscales: torch.Tensor, ktail: torch.Tensor, vtail: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                 starts: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
+                 magnitude: float = 1.0, interleaved: bool = False) -> torch.Tensor:
+    """lm.cache_append: new tokens into a paged 8-bit cache; q turned, or empty without."""
+    cache = lm.Cache8(kpages, vpages, kscales, vscales, ktail, vtail, table)
+    out = lm.cache_append(cache, lens, k, v, starts, q, freqs, magnitude, interleaved)
+    return k.new_empty(0) if out is None else out
+
+
+@cache_append.register_fake
+def _(k, v, kpages, vpages, kscales, vscales, ktail, vtail, table, lens, starts=None, q=None, freqs=None, magnitude=1.0,
+      interleaved=False):
+    return k.new_empty(0 if q is None else q.shape)
+
+
+@torch.library.custom_op("xdna::attention_cache", mutates_args=())
+def attention_cache(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
+                    ktail: torch.Tensor, vtail: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """lm.attention_cache: the newest tokens' attention over a paged 8-bit cache."""
+    return lm.attention_cache(q, lm.Cache8(kpages, vpages, kscales, vscales, ktail, vtail, table), lens, scale)
+
+
+@attention_cache.register_fake
+def _(q, kpages, vpages, kscales, vscales, ktail, vtail, table, lens, scale=None):
+    return q.new_empty(q.shape)
+
+
 # ------------------------------------------------------------------------------ GPU calls that need no autograd
 # custom_op's own route from the dispatcher to the function above passes through its autograd and backend wrappers in
 # Python, 9 us a call, as much as a small op's launches. A call whose tensors are ordinary GPU tensors, none of which
