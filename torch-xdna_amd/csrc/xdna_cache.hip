@@ -16,12 +16,15 @@
 //   S = K Q^T over 64 keys, four tiles of 16: row 4 h' + r of tile t is key 16 h' + 4 t + r, so that lane l, h = l / 16, gets the
 //     scores of keys 16 h .. 16 h + 15 for query row l % 16; lane h's 16 bytes of K are dims 16 (h + 4 j) .. + 15, two steps.
 //   O^T = V^T P^T: those 16 scores are lane h's values of two 32-deep steps, and 16 bytes of a row of V are the same keys.
-// int8 is exact in either 16-bit type. K's scale is applied to the float32 scores; V's, as a share of the largest met so far,
-// goes into P before its rounding, and O is held in units of that largest one.
+// The products with pages run in float16, which holds int8 exactly and is the cheaper to widen to: bfloat16 rows of q are brought
+// into its range by a power of two. K's scale goes into the exponent's factor, in float32; V's, as a share of the largest met so
+// far, into P before its rounding to float16, and O is held in units of that largest one. The open page's products run
+// in the tensors' own type.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "xdna_common.h"
 #include "xdna_hip.h"
@@ -31,7 +34,19 @@ namespace xdna {
 namespace {
 
 typedef __bf16 bf16x8c __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x2c __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8c __attribute__((ext_vector_type(8)));
+
+// n / d for 0 <= n < 2^31 by a product: m = 2^32 (2^s - d) / d + 1, s = ceil(log2 d); q = (n + high(n m)) >> s
+struct Divisor {
+  uint32_t m, s, d;
+  Divisor() = default;
+  explicit Divisor(int64_t by) : m(0), s(0), d((uint32_t)by) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((((1ull << s) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)(((uint32_t)n + __umulhi((uint32_t)n, m)) >> s); }
+};
 
 bool sixteen(int dtype) { return dtype == XDNA_BF16 || dtype == XDNA_F16; }
 int log2_page(int64_t g) { return g == 16 ? 4 : g == 32 ? 5 : g == 64 ? 6 : g == 128 ? 7 : -1; }
@@ -383,7 +398,8 @@ struct CacheArgs {
   const int32_t *table, *lens;
   int64_t ldt;
   int B, N, nh, nkv, d, P, pages, logg, R;
-  int parts, rblocks;                   // parts of a text's keys; blocks of rows of a (text, kv head)
+  int parts, rblocks, items;            // parts of a text's keys; blocks of rows of a (text, kv head); parts B nkv
+  Divisor by_rblocks, by_nkv, by_b, by_grp, by_parts;
   float c;                              // scale log2 e
   uint32_t sign;
   float *po, *pml;                      // [parts][B N nh][d] sums, [parts][B N nh][2] maxima and sums of p
@@ -398,27 +414,17 @@ __device__ __forceinline__ f32x4 mfma16(const i32x4& a, const i32x4& b, const f3
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8c, a), __builtin_bit_cast(bf16x8c, b), c, 0, 0, 0);
 }
 
-// Four int8 as two words of 16-bit floats, exactly. float16: q + 128 is the low bits of 1024 + .., and 1152 comes off again.
-template <int DT>
-__device__ __forceinline__ void widen(uint32_t w, int& lo, int& hi) {
-  if constexpr (DT == XDNA_F16) {
-    const uint32_t u = w ^ 0x80808080u;
-    const f16x2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    lo = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
-    hi = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
-  } else {
-    lo = (int)f32x2_to_bf16x2_bits((float)(int8_t)w, (float)(int8_t)(w >> 8));
-    hi = (int)f32x2_to_bf16x2_bits((float)(int8_t)(w >> 16), (float)((int32_t)w >> 24));
-  }
-}
-template <int DT>
+// Eight int8 as float16, exactly: q + 128 is the low bits of 1024 + .., and 1152 comes off again. Five instructions for four of
+// them; to bfloat16 it would be six.
 __device__ __forceinline__ i32x4 widen8(uint32_t a, uint32_t b) {
+  const f16x2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  const uint32_t w[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
   i32x4 r;
-  int x, y;
-  widen<DT>(a, x, y);
-  r[0] = x, r[1] = y;
-  widen<DT>(b, x, y);
-  r[2] = x, r[3] = y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    r[2 * i] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) - off);
+    r[2 * i + 1] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) - off);
+  }
   return r;
 }
 
@@ -436,54 +442,50 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// float16 p are held 2^14 times as large, so that those down to 2^-28 of the largest stay normal numbers
-template <int DT>
-constexpr float SHIFT = DT == XDNA_F16 ? 14.0f : 0.0f;
+// A row's maximum follows the scores once they pass it by more than 2^SLACK: nearly never after a row's first keys, where
+// otherwise some row of sixteen finds a larger one at nearly every step, and all of O is multiplied. p are held 2^SHIFT times
+// as large, so that float16 takes them from 2^-23 of the maximum (normal) to 2^SLACK times it.
+constexpr float SLACK = 6.0f, SHIFT = 9.0f;
 template <int DT>
 constexpr uint32_t ALL_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
 
 // A wave's rows: RB blocks of 16, their maxima, sums and outputs. Rows of a (text, kv head) are the pairs (new token, q head
 // of the group), so that the heads that share K and V share their loads.
-template <int DT, int D, int RB>
+template <int D, int RB>
 struct Rows {
-  static constexpr int S = D / 32, ND = D / 16;
-  i32x4 q[RB][S];
+  static constexpr int ND = D / 16;
   f32x4 o[RB][ND];
-  float m[RB], l[RB];
+  float m[RB], l[RB];       // m in units of the exponent
   int limit[RB];            // keys that the lane's row sees
   float unit;               // O is held in units of it
 
-  // p of the 64 keys whose scores are here, K's scale and masks applied, as the second product's operand
-  __device__ __forceinline__ void weigh(f32x4 (&sc)[4], int rb, float c, float share, bool masked, int first, int lim, i32x4 (&pf)[2]) {
+  // p of T tiles of 16 keys as the second product's operand: 2^(c score - m), c with K's scale
+  template <int DT, int T>
+  __device__ __forceinline__ void weigh(const f32x4* sc, int rb, float c, float share, int* pf) {
     float mx = sc[0][0];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, sc[t][r]);
-    mx = quad_max(mx);
-    const bool grow = mx > m[rb];
+    mx = quad_max(mx * c);
+    const bool grow = mx > m[rb] + SLACK;
     if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float mn = grow ? mx : m[rb];
-      const float alpha = m[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[rb] - mn) * c);
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m[rb] - mx) : 1.0f;      // from -inf: 0
       l[rb] *= alpha;
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[rb][i] *= alpha;
-      m[rb] = mn;
+      m[rb] = grow ? mx : m[rb];
     }
-    const float mc = (m[rb] == -INFINITY ? 0.0f : m[rb] * c) - SHIFT<DT>;
+    const float mc = (m[rb] == -INFINITY ? 0.0f : m[rb]) - SHIFT;      // only -inf scores so far: p = 0
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
         float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -mc)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r + 1], c, -mc));
         l[rb] += p0;
         l[rb] += p1;
         p0 *= share, p1 *= share;
-        if (masked) {                     // a share that is not finite is not the row's unless it sees the key
-          if (first + 4 * t + r >= lim) p0 = 0.0f;
-          if (first + 4 * t + r + 1 >= lim) p1 = 0.0f;
-        }
-        pf[t >> 1][(t & 1) * 2 + r / 2] = (int)pack16<DT>(p0, p1);
+        pf[2 * t + r / 2] = (int)pack16<DT>(p0, p1);
       }
   }
 
@@ -492,8 +494,10 @@ struct Rows {
     float top = vs;
     if (!uniform) {
       // the largest number among the four groups of keys (fmaxf leaves out NaN)
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
     }
     if (__builtin_amdgcn_ballot_w64(top > unit)) {
       const float to = unit / top;
@@ -508,139 +512,237 @@ struct Rows {
 };
 
 // W waves share out the 64-key steps of a part of a text's keys for 16 RB rows and meet in LDS. Registers hold the step in
-// work and nothing else: K of the wave's next step is on its way once its scores are done, V after its products.
-template <int DT, int D, int RB, int W>
-__global__ __launch_bounds__(W * 64, RB == 1 ? 3 : 2) void cache_kernel(CacheArgs a) {
-  constexpr int S = D / 32, ND = D / 16, DC = D / 64;
-  __shared__ __attribute__((aligned(16))) float ol[W][RB * ND][256];
+// work and nothing else: K of the wave's next step is on its way once its scores are done, V after its products. The last
+// step is a copy of the loop's body that loads nothing: past a branch around loads the compiler waits for all of them.
+// Heads are held as D dims, a multiple of 32; dims past a.d (D - 16 then) are copies of others, times zeros of q, and of no output.
+// EXACT: the heads have D dims.
+template <int DT, int D, int RB, int W, bool EXACT>
+__global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
+  // a lane's bytes of K: 16 of each 64 dims, and 8 of the last 32
+  constexpr int S = D / 32, ND = D / 16, DC = D / 64, REST = S - 2 * DC;
+  constexpr bool QLDS = RB > 1;                 // more rows: q in LDS, registers for O
+  __shared__ __attribute__((aligned(16))) float ol[W / 2][RB * ND][256];
   __shared__ float ml[2][W][RB][16];
+  __shared__ i32x4 ql[QLDS ? RB * S : 1][64];
+  __shared__ float qls[QLDS ? RB : 1][16];
   const int lane = threadIdx.x & 63, h = lane >> 4, i16 = lane & 15, hk = i16 >> 2;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp = a.nh / a.nkv, nrows = a.N * grp, g = 1 << a.logg;
-  int rest = blockIdx.x;
-  const int rblock = rest % a.rblocks;
-  rest /= a.rblocks;
-  const int kvh = rest % a.nkv;
-  rest /= a.nkv;
-  const int b = rest % a.B, part = rest / a.B;
+  const int grp = a.by_grp.d, nrows = a.N * grp, g = 1 << a.logg, d = EXACT ? D : a.d;
+  // the blocks of rows of one item (part, text, kv head), which read the same keys, 8 apart: on one XCD
+  const int eight = a.by_rblocks.of(blockIdx.x >> 3), rblock = (blockIdx.x >> 3) - eight * a.rblocks, item = eight * 8 + (blockIdx.x & 7);
+  if (item >= a.items) return;
+  const int pb = a.by_nkv.of(item), kvh = item - pb * a.nkv, part = a.by_b.of(pb), b = pb - part * a.B;
   const int len = min(max(a.lens[b], 0), a.P << a.logg);
   const int npages = len >> a.logg, nfull = npages << a.logg, ntail = len - nfull;
   const int steps = (nfull + 63) >> 6, all = steps + ((ntail + 63) >> 6);
-  const int per = (all + a.parts - 1) / a.parts, from = min(part * per, all), to = min(from + per, all);
-  const int row0 = rblock * 16 * RB, dchunks = a.d >> 4;
+  const int per = a.by_parts.of(all + a.parts - 1), from = min(part * per, all), to = min(from + per, all);
+  const int end = min(to, steps), row0 = rblock * 16 * RB, dchunks = d >> 4;
 
-  Rows<DT, D, RB> w;
+  Rows<D, RB> w;
   w.unit = 0.0f;
-  int64_t orow[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int row = min(row0 + 16 * rb + i16, nrows - 1), n = row / grp, head = kvh * grp + row - n * grp;
-    orow[rb] = ((int64_t)b * a.N + n) * a.nh + head;
-    w.limit[rb] = len - a.N + n + 1;
+    w.limit[rb] = len - a.N + a.by_grp.of(min(row0 + 16 * rb + i16, nrows - 1)) + 1;
     w.m[rb] = -INFINITY;
     w.l[rb] = 0.0f;
-    const uint16_t* const q = a.q + b * a.qb + n * a.qn + head * a.qh;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int at = 16 * (h + 4 * (s >> 1)) + 8 * (s & 1);
-      w.q[rb][s] = i32x4{0, 0, 0, 0};
-      if (at < a.d) w.q[rb][s] = *reinterpret_cast<const i32x4*>(q + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w.q[rb][s][e] ^= (int)a.sign;
-    }
 #pragma unroll
     for (int i = 0; i < ND; ++i) w.o[rb][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  // the first row's tokens are the fewest that a row of this workgroup sees
-  const int sure = min(nfull, __builtin_amdgcn_readfirstlane(w.limit[0]));
+  // the lane's row of a block: its new token and q head. Found again where it is needed: held, it costs the loop registers.
+  const auto row_of = [&](int rb, int& n, int& head) {
+    int at = row0;
+    asm volatile("" : "+s"(at));
+    const int row = min(at + 16 * rb + i16, nrows - 1);
+    n = a.by_grp.of(row), head = kvh * grp + row - n * grp;
+  };
+  const auto load_q = [&](int rb, i32x4 (&x)[S]) {
+    int n, head;
+    row_of(rb, n, head);
+    const uint16_t* const q = a.q + b * a.qb + n * a.qn + head * a.qh;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int dim = s < 2 * DC ? 16 * (h + 4 * (s >> 1)) + 8 * (s & 1) : 64 * DC + 8 * h;
+      x[s] = *reinterpret_cast<const i32x4*>(q + min(dim, d - 8));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[s][e] = dim < d ? x[s][e] ^ (int)a.sign : 0;
+    }
+  };
+  // q for the pages, in float16: bfloat16 rows are scaled by a power of two that brings their largest value to 2^14 .. 2^15;
+  // those down to 2^-32 of it stay exact (beside one that is not finite none matters). The inverse goes to the scores.
+  const auto half_q = [&](i32x4 (&x)[S], float& back) {
+    back = 1.0f;
+    if constexpr (DT == XDNA_BF16) {
+      u16x2c big = {0, 0};
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2c, (uint32_t)x[s][e] & 0x7fff7fffu));
+      uint32_t top = max(big[0], big[1]);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      const uint32_t e8 = max(top >> 7, 15u);
+      const float by = __uint_as_float((268u - e8) << 23);
+      back = __uint_as_float((e8 - 14u) << 23);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[s][e] = (int)f32x2_to_f16x2_bits(bf16_bits_to_f32((uint16_t)x[s][e]) * by, bf16_bits_to_f32((uint16_t)((uint32_t)x[s][e] >> 16)) * by);
+    }
+  };
+  i32x4 qf[S];
+  float back[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    if (!QLDS || wave == rb) load_q(rb, qf);
 
   // A lane's part of a step: the page of the keys that it loads K of (16 hk ..), and of those that it has scores and V of
-  // (16 h ..). Pages past the last one, and what is no page, are read as a page that there is, and masked.
+  // (16 h ..). Pages past the last one, and what is no page, are read as a page that there is, and masked. A step's pages are
+  // asked for before the K of the step before it, so that no later load has to be waited for with them.
   const int32_t* const table = a.table + b * a.ldt;
-  auto page_at = [&](int step, int quarter) {
-    const int at = min((step * 64 + 16 * quarter) >> a.logg, npages - 1);
-    return table[max(at, 0)];
-  };
-  const auto safe = [&](int id) { return id >= 0 && id < a.pages ? id : 0; };
-  int idk = 0, idv = 0;
-  i32x4 k[4 * DC], v[ND];
+  const auto page_at = [&](int at, int quarter) { return table[min((at * 64 + 16 * quarter) >> a.logg, a.P - 1)]; };
+  const auto known = [&](int id) { return id >= 0 && id < a.pages; };
+  int asked_k = 0, asked_v = 0;
+  i32x4 k[4 * DC + 1], v[ND];
+  int2 kr[4];
   float ksc = 0.0f, vsc = 0.0f;
-  auto load_k = [&](int step) {
-    const int in = (step * 64 + 16 * hk) & (g - 1);
-    const int8_t* const base = a.kp + (((int64_t)safe(idk) * a.nkv + kvh) * g + in + (lane & 3)) * a.d;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int j = 0; j < DC; ++j) k[t * DC + j] = *reinterpret_cast<const i32x4*>(base + 4 * t * a.d + 16 * min(h + 4 * j, dchunks - 1));
+  // what differs from lane to lane goes into one offset, the rest is uniform
+  const int klane = (lane & 3) * d + 16 * min(h, dchunks - 1), kmore = 16 * (min(h + 4, dchunks - 1) - min(h, dchunks - 1));
+  const int krest = (lane & 3) * d + 64 * DC + 8 * (64 * DC + 8 * h < d ? h : h & 1);
+  const auto k_base = [&](int at, int id) {
+    return a.kp + ((int64_t)(known(id) ? id : 0) * a.nkv + kvh) * (g * d) + ((at * 64 + 16 * hk) & (g - 1)) * d;
   };
-  auto load_v = [&](int step, int id) {
-    const int in = (step * 64 + 16 * h) & (g - 1);
-    const int8_t* const base = a.vp + ((int64_t)safe(id) * a.nkv + kvh) * a.d * g + in;
-#pragma unroll
-    for (int i = 0; i < ND; ++i) v[i] = *reinterpret_cast<const i32x4*>(base + (int64_t)(16 * min(i, dchunks - 1) + i16) * g);
+  const auto v_base = [&](int at, int id) {
+    return a.vp + ((int64_t)(known(id) ? id : 0) * a.nkv + kvh) * (g * d) + (i16 * g + ((at * 64 + 16 * h) & (g - 1)));
   };
-  auto load_scales = [&](int id) {
-    const int64_t at = (int64_t)safe(id) * a.nkv + kvh;
+  const auto load_k = [&](const int8_t* base) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if constexpr (DC > 0) k[t * DC] = *reinterpret_cast<const i32x4*>(base + (klane + 4 * t * d));
+      if constexpr (DC > 1) k[t * DC + 1] = *reinterpret_cast<const i32x4*>(base + (klane + kmore + 4 * t * d));
+      if constexpr (REST) kr[t] = *reinterpret_cast<const int2*>(base + (krest + 4 * t * d));
+    }
+  };
+  const auto load_v = [&](const int8_t* base) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i) v[i] = *reinterpret_cast<const i32x4*>(base + 16 * min(i, dchunks - 1) * g);
+  };
+  const auto load_scales = [&](int id) {
+    const int64_t at = (int64_t)(known(id) ? id : 0) * a.nkv + kvh;
     ksc = a.ks[at];
     vsc = a.vs[at];
   };
-  int step = from + wave;
-  const int end = min(to, steps);
-  if (step < end) {
-    idk = page_at(step, hk), idv = page_at(step, h);
-    load_k(step);
-    load_v(step, idv);
-    load_scales(idv);
+  int step = (a.parts == 1 ? 0 : from) + wave;       // alone, a wave's first page is known before the length is
+  bool good = false;
+  if (a.P > 0) {
+    const int id_k = page_at(step, hk), id_v = page_at(step, h);
+    asked_k = page_at(step + W, hk), asked_v = page_at(step + W, h);
+    good = known(id_v);
+    if (step < end) {
+      load_k(k_base(step, id_k));
+      load_scales(id_v);
+      load_v(v_base(step, id_v));
+    }
   }
-#pragma unroll 1
-  for (; step < end; step += W) {
+  if constexpr (QLDS) {
+    if (wave < RB) {
+      half_q(qf, back[0]);
+#pragma unroll
+      for (int s = 0; s < S; ++s) ql[wave * S + s][lane] = qf[s];
+      if (h == 0) qls[wave][i16] = back[0];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) back[rb] = qls[rb][i16];
+  } else {
+    half_q(qf, back[0]);
+  }
+  const auto q_frag = [&](int rb, int s) {
+    if constexpr (QLDS) return ql[rb * S + s][lane];
+    else return qf[s];
+  };
+  // the first row's tokens are the fewest that a row of this workgroup sees
+  const int sure = min(nfull, __builtin_amdgcn_readfirstlane(w.limit[0]));
+
+  const auto pages = [&](auto more) {
     const int first = step * 64 + 16 * h, next = step + W;
-    const bool good = idv >= 0 && idv < a.pages;
     const bool masked = step * 64 + 64 > sure || __builtin_amdgcn_ballot_w64(!good) != 0;
-    f32x4 sc[RB][4];
+    const bool mine = good;
+    // T tiles of 16 keys at a time: with more rows fewer scores in registers
+    constexpr int T = RB == 1 ? 4 : 2;
+    float ks = ksc, share = 0.0f;
+    const int8_t* next_v = nullptr;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t0 = 0; t0 < 4; t0 += T) {
+      i32x4 pf[RB][T / 2];
+      f32x4 sc[RB][T];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) sc[rb][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) sc[rb][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const i32x4 x = k[t * DC + (s >> 1)];
-        const i32x4 f = widen8<DT>(x[2 * (s & 1)], x[2 * (s & 1) + 1]);
+        i32x4 q[RB];
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) sc[rb][t] = mfma16<DT>(f, w.q[rb][s], sc[rb][t]);
+        for (int rb = 0; rb < RB; ++rb) q[rb] = q_frag(rb, s);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const int tt = t0 + t;
+          i32x4 f;
+          if (s < 2 * DC) f = widen8(k[tt * DC + (s >> 1)][2 * (s & 1)], k[tt * DC + (s >> 1)][2 * (s & 1) + 1]);
+          else f = widen8(kr[tt].x, kr[tt].y);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) sc[rb][t] = mfma16<XDNA_F16>(f, q[rb], sc[rb][t]);
+        }
       }
-    }
-    const float ks = ksc, vs = good && first < nfull ? vsc : 0.0f;
-    if (next < end) {
-      idk = page_at(next, hk), idv = page_at(next, h);
-      load_k(next);
-      load_scales(idv);
-    }
-    const float share = w.share_of(vs, g >= 64);
-    i32x4 pf[RB][2];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int lim = good ? min(nfull, w.limit[rb]) : 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) sc[rb][t] *= ks;
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (first + 4 * t + r >= lim) sc[rb][t][r] = -INFINITY;
+      if (t0 + T == 4) {
+        const float vs = mine && first < nfull ? vsc : 0.0f;
+        if (T == 4) share = w.share_of(vs, g >= 64);
+        if constexpr (more) {
+          const int8_t* const next_k = k_base(next, asked_k);
+          next_v = v_base(next, asked_v);
+          const int id = asked_v;
+          good = known(id);
+          asked_k = page_at(next + W, hk), asked_v = page_at(next + W, h);
+          load_k(next_k);
+          load_scales(id);
+        }
+      } else {
+        share = w.share_of(mine && first < nfull ? vsc : 0.0f, g >= 64);
       }
-      w.weigh(sc[rb], rb, a.c, share, masked, first, lim, pf[rb]);
-    }
 #pragma unroll
-    for (int i = 0; i < ND; ++i)
+      for (int rb = 0; rb < RB; ++rb) {
+        const int lim = mine ? min(nfull, w.limit[rb]) : 0;
+        if (masked) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const i32x4 f = widen8<DT>(v[i][2 * u], v[i][2 * u + 1]);
+          for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) w.o[rb][i] = mfma16<DT>(f, pf[rb][u], w.o[rb][i]);
+            for (int r = 0; r < 4; ++r)
+              if (first + 4 * (t0 + t) + r >= lim) sc[rb][t][r] = -INFINITY;
+        }
+        // above 0, so that an unseen key's -inf stays one; the scales of a page that the row does not see do not matter
+        float c = __builtin_elementwise_maximum(ks * (back[rb] * a.c), 1.17549435e-38f);
+        const bool unseen = masked && first >= lim;
+        if (unseen) c = 1.0f;
+        w.template weigh<XDNA_F16, T>(sc[rb], rb, c, unseen ? 0.0f : share, reinterpret_cast<int*>(&pf[rb][0]));
       }
-    if (next < end) load_v(next, idv);
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int u = 0; u < T / 2; ++u) {
+          const i32x4 f = widen8(v[i][t0 + 2 * u], v[i][t0 + 2 * u + 1]);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) w.o[rb][i] = mfma16<XDNA_F16>(f, pf[rb][u], w.o[rb][i]);
+        }
+    }
+    if constexpr (more) load_v(next_v);
+  };
+#pragma unroll 1
+  for (; step + W < end; step += W) pages(std::true_type{});
+  if (step < end) {
+    pages(std::false_type{});
+    step += W;
   }
   // the open page, in 16 bits
 #pragma unroll 1
@@ -648,22 +750,42 @@ __global__ __launch_bounds__(W * 64, RB == 1 ? 3 : 2) void cache_kernel(CacheArg
     const int at = (step - steps) * 64, left = ntail - at;          // keys of this step: nfull + at ..
     const int slot = nfull % a.R + at;
     const int64_t head = (int64_t)b * a.nkv + kvh;
-    const uint16_t* const kt = a.ktail + (head * a.R + slot) * a.d;
+    const uint16_t* const kt = a.ktail + (head * a.R + slot) * d;
     // a group of 16 places without keys is read as the first one, and masked
-    const uint16_t* const vt = a.vtail + head * a.d * a.R + slot + (16 * h < left ? 16 * h : 0);
+    const uint16_t* const vt = a.vtail + head * d * a.R + (i16 * a.R + slot + (16 * h < left ? 16 * h : 0));
     f32x4 sc[RB][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint16_t* const row = kt + (int64_t)min(16 * hk + 4 * t + (lane & 3), left - 1) * a.d;
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) sc[rb][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // a block of rows after the other, so that few registers hold q and K
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const i32x4 f = *reinterpret_cast<const i32x4*>(row + 16 * min(h + 4 * (s >> 1), dchunks - 1) + 8 * (s & 1));
+    for (int rb = 0; rb < RB; ++rb) {
+      i32x4 q[S];
+      load_q(rb, q);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) sc[rb][t] = mfma16<DT>(f, w.q[rb][s], sc[rb][t]);
-      }
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const int dim = s < 2 * DC ? 16 * min(h + 4 * (s >> 1), dchunks - 1) + 8 * (s & 1) : 64 * DC + 8 * (64 * DC + 8 * h < d ? h : h & 1);
+          const i32x4 f = *reinterpret_cast<const i32x4*>(kt + (min(16 * hk + 4 * t + (lane & 3), left - 1) * d + dim));
+          sc[rb][t] = mfma16<DT>(f, q[s], sc[rb][t]);
+        }
+      if (RB > 1) asm volatile("" ::: "memory");
     }
+    // V in two halves: its 16-bit fragments of all dims are as many registers again as a step of pages has
+    constexpr int HALF = ND / 2;
+    i32x4 f[HALF][2];
+    const auto load_half = [&](int n) {
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < HALF; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          f[i][u] = *reinterpret_cast<const i32x4*>(vt + 16 * min(n * HALF + i, dchunks - 1) * a.R + 8 * u);
+      asm volatile("" ::: "memory");
+    };
+    load_half(0);
     const int first = nfull + at + 16 * h;
     const float share = w.share_of(1.0f, true);
     i32x4 pf[RB][2];
@@ -675,168 +797,267 @@ __global__ __launch_bounds__(W * 64, RB == 1 ? 3 : 2) void cache_kernel(CacheArg
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (first + 4 * t + r >= lim) sc[rb][t][r] = -INFINITY;
-      w.weigh(sc[rb], rb, a.c, share, true, first, lim, pf[rb]);
+      w.template weigh<DT, 4>(sc[rb], rb, a.c, share, reinterpret_cast<int*>(&pf[rb][0]));
     }
-#pragma unroll 1
-    for (int i = 0; i < ND; ++i) {
-      if (i >= dchunks) break;
-      i32x4 f[2];
-      bool odd = false;
+    // Places without keys are zeros. What is not finite may belong to a key that some rows do not see (of one new token's rows
+    // every row sees every key), and 0 times it would be NaN: taken out, and added below to the rows that see it.
+    uint32_t keep[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f[u] = *reinterpret_cast<const i32x4*>(vt + (int64_t)(16 * i + i16) * a.R + 8 * u);
+    for (int e = 0; e < 8; ++e) keep[e] = (16 * h + 2 * e < left ? 0xffffu : 0u) | (16 * h + 2 * e + 1 < left ? 0xffff0000u : 0u);
+    bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = 16 * h + 8 * u + 2 * e;
-          uint32_t x = (uint32_t)f[u][e];
-          if (key >= left) x = 0;
-          else if (key + 1 >= left) x &= 0xffffu;
-          // what is not finite may belong to a key that some rows do not see, and 0 times it would be NaN: taken out, and
-          // added below to the rows that see it
-          if ((x & ALL_ONES<DT>) == ALL_ONES<DT>) x &= 0xffff0000u, odd = true;
-          if ((x >> 16 & ALL_ONES<DT>) == ALL_ONES<DT>) x &= 0xffffu, odd = true;
-          f[u][e] = (int)x;
-        }
-      }
-      const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+    for (int n = 0; n < 2; ++n) {
+      if (n) load_half(1);
+      u16x2c big = {0, 0};
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        f32x4 o = w.o[rb][0];
+      for (int i = 0; i < HALF; ++i)
 #pragma unroll
-        for (int n = 1; n < ND; ++n)
-          if (n == i) o = w.o[rb][n];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) o = mfma16<DT>(f[u], pf[rb][u], o);
-        if (any) {
-#pragma unroll 1
-          for (int key = 0; key < min(left, 64); ++key) {
-            // lane 16 (key / 16) + i16 holds the row's p of it, in half key % 2 of word (key % 16) / 2
-            uint32_t x = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e == (key & 15) >> 1) x = (uint32_t)pf[rb][e >> 2][e & 3];
-            x = __shfl(x, 16 * (key >> 4) + i16, 64) >> (16 * (key & 1)) & 0xffffu;
-            const float p = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)x) : bf16_bits_to_f32((uint16_t)x);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint16_t y = a.vtail[(head * a.d + 16 * i + 4 * h + r) * a.R + slot + key];
-              if ((y & ALL_ONES<DT>) == ALL_ONES<DT> && nfull + at + key < w.limit[rb])
-                o[r] += p * (DT == XDNA_F16 ? f16_bits_to_f32(y) : bf16_bits_to_f32(y));
-            }
+          for (int e = 0; e < 4; ++e) {
+            f[i][u][e] &= (int)keep[4 * u + e];
           }
+      if (a.N > 1) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2c, (uint32_t)f[i][u][e] & 0x7fff7fffu));
+      }
+      if (a.N > 1 && __builtin_amdgcn_ballot_w64(big[0] >= ALL_ONES<DT> || big[1] >= ALL_ONES<DT>)) {
+        odd = true;
+#pragma unroll
+        for (int i = 0; i < HALF; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t x = (uint32_t)f[i][u][e];
+              if ((x & ALL_ONES<DT>) == ALL_ONES<DT>) x &= 0xffff0000u;
+              if ((x >> 16 & ALL_ONES<DT>) == ALL_ONES<DT>) x &= 0xffffu;
+              f[i][u][e] = (int)x;
+            }
+      }
+#pragma unroll
+      for (int i = 0; i < HALF; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) w.o[rb][n * HALF + i] = mfma16<DT>(f[i][u], pf[rb][u], w.o[rb][n * HALF + i]);
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int x = 0; x < min(left, 64) * dchunks; ++x) {
+        const int i = x % dchunks, key = x / dchunks;
+        f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint16_t z = a.vtail[(head * d + 16 * i + 4 * h + r) * a.R + slot + key];
+          y[r] = (z & ALL_ONES<DT>) != ALL_ONES<DT> ? 0.0f : DT == XDNA_F16 ? f16_bits_to_f32(z) : bf16_bits_to_f32(z);
         }
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-          if (n == i) w.o[rb][n] = o;
+        for (int rb = 0; rb < RB; ++rb) {
+          // lane 16 (key / 16) + i16 holds the row's p of it, in half key % 2 of word (key % 16) / 2
+          uint32_t z = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e == (key & 15) >> 1) z = (uint32_t)pf[rb][e >> 2][e & 3];
+          z = __shfl(z, 16 * (key >> 4) + i16, 64) >> (16 * (key & 1)) & 0xffffu;
+          const float p = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)z) : bf16_bits_to_f32((uint16_t)z);
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n == i && y[r] != 0.0f && nfull + at + key < w.limit[rb]) w.o[rb][n][r] += p * y[r];
+        }
       }
     }
   }
 
-  // the waves' rows joined
+  // The waves' rows joined: the second half's into the first half's, then those by all waves.
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    w.l[rb] = quad_sum(w.l[rb]);
-    if (h == 0) ml[0][wave][rb][i16] = w.m[rb], ml[1][wave][rb][i16] = w.l[rb];
+  for (int rb = 0; rb < RB; ++rb) w.l[rb] = quad_sum(w.l[rb]);
+  const auto leave = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      f32x4 o = w.o[rb][i];
-      o *= w.unit;
-      *reinterpret_cast<f32x4*>(&ol[wave][rb * ND + i][lane * 4]) = o;
+    for (int rb = 0; rb < RB; ++rb) {
+      if (h == 0) ml[0][wave][rb][i16] = w.m[rb], ml[1][wave][rb][i16] = w.l[rb];
+#pragma unroll
+      for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4*>(&ol[at][rb * ND + i][lane * 4]) = w.o[rb][i];
     }
+  };
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int i = 0; i < ND; ++i) w.o[rb][i] *= w.unit;
+  if (wave >= W / 2) leave(wave - W / 2);
+  __syncthreads();
+  if (wave < W / 2) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float m1 = ml[0][wave + W / 2][rb][i16], l1 = ml[1][wave + W / 2][rb][i16], mt = fmaxf(w.m[rb], m1);
+      const float w0 = w.m[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m[rb] - mt);
+      const float w1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - mt);
+      w.l[rb] = (w.m[rb] == -INFINITY ? w.l[rb] : w.l[rb] * w0) + (m1 == -INFINITY ? l1 : l1 * w1);     // 0 or NaN where there is no maximum
+      w.m[rb] = mt;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&ol[wave][rb * ND + i][lane * 4]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w.o[rb][i][r] = w.o[rb][i][r] * w0 + x[r] * w1;
+      }
+    }
+    leave(wave);                     // where its partner's were, which no other wave reads
   }
   __syncthreads();
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    float mt = -INFINITY, lt = 0.0f, weight[W];
+    float mt = -INFINITY, lt = 0.0f, weight[W / 2];
 #pragma unroll
-    for (int x = 0; x < W; ++x) mt = fmaxf(mt, ml[0][x][rb][i16]);
+    for (int x = 0; x < W / 2; ++x) mt = fmaxf(mt, ml[0][x][rb][i16]);
 #pragma unroll
-    for (int x = 0; x < W; ++x) {
+    for (int x = 0; x < W / 2; ++x) {
       const float mg = ml[0][x][rb][i16], lg = ml[1][x][rb][i16];
-      weight[x] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mg - mt) * a.c);
-      lt += mg == -INFINITY ? lg : lg * weight[x];            // lg is 0 then, or NaN
+      weight[x] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mg - mt);
+      lt += mg == -INFINITY ? lg : lg * weight[x];
     }
     const bool mine = row0 + 16 * rb + i16 < nrows;
+    int token, qhead;
+    row_of(rb, token, qhead);
+    const int64_t orow = ((int64_t)b * a.N + token) * a.nh + qhead;
 #pragma unroll
     for (int n = 0; n < (ND + W - 1) / W; ++n) {
       const int i = wave + n * W;
       if (i >= dchunks) break;
       f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int x = 0; x < W; ++x) {
-        const f32x4 part_o = *reinterpret_cast<const f32x4*>(&ol[x][rb * ND + i][lane * 4]);
+      for (int x = 0; x < W / 2; ++x) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(&ol[x][rb * ND + i][lane * 4]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] += part_o[r] * weight[x];
+        for (int r = 0; r < 4; ++r) o[r] += y[r] * weight[x];
       }
       if (!mine) continue;
       const int dim = 16 * i + 4 * h;
       if (a.parts == 1) {
         const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-        *reinterpret_cast<uint2*>(a.out + orow[rb] * a.d + dim) = make_uint2(pack16<DT>(o[0] * inv, o[1] * inv), pack16<DT>(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(a.out + orow * d + dim) = make_uint2(pack16<DT>(o[0] * inv, o[1] * inv), pack16<DT>(o[2] * inv, o[3] * inv));
       } else {
-        const int64_t at = (int64_t)part * a.B * a.N * a.nh + orow[rb];
-        *reinterpret_cast<f32x4*>(a.po + at * a.d + dim) = o;
+        const int64_t at = (int64_t)part * a.B * a.N * a.nh + orow;
+        *reinterpret_cast<f32x4*>(a.po + at * d + dim) = o;
         if (dim == 0) *reinterpret_cast<float2*>(a.pml + at * 2) = make_float2(mt, lt);
       }
     }
   }
 }
 
-// The parts of a row joined: a workgroup per row, wave w the parts w, w + 4, .., then the waves in their order; lane l dims
-// 2 l, 2 l + 1.
-template <int DT>
+// The parts of a row joined: G waves have a row, wave w of them the parts w, w + G, .., U at once, then the waves in their
+// order; lane l dims 2 l, 2 l + 1.
+template <int DT, int G, int U>
 __global__ __launch_bounds__(256) void cache_join_kernel(const float* __restrict__ po, const float* __restrict__ pml, int parts,
-                                                         int64_t rows, int d, float c, uint16_t* __restrict__ out) {
-  __shared__ float2 ov[4][64];
-  __shared__ float lv[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x;
-  float mt = -INFINITY;
-  for (int i = lane; i < parts; i += 64) mt = fmaxf(mt, pml[(i * rows + row) * 2]);
-  mt = wave_max(mt);
-  float l = 0.0f, x = 0.0f, y = 0.0f;
+                                                         int64_t rows, int d, uint16_t* __restrict__ out) {
+  __shared__ float2 ov[4][64], mv[4];
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % G;
+  const int64_t row = (int64_t)blockIdx.x * (4 / G) + all / G;
+  if (G == 1 && row >= rows) return;
+  float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
   const int at = min(2 * lane, d - 2);
-#pragma unroll 8
-  for (int i = wave; i < parts; i += 4) {
-    const float2 p = *reinterpret_cast<const float2*>(pml + (i * rows + row) * 2);
-    const float2 v = *reinterpret_cast<const float2*>(po + (i * rows + row) * d + at);
-    const float w = p.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((p.x - mt) * c);
-    l += p.x == -INFINITY ? p.y : p.y * w;
-    x += v.x * w;
-    y += v.y * w;
-  }
-  ov[wave][lane] = make_float2(x, y);
-  if (lane == 0) lv[wave] = l;
-  __syncthreads();
-  if (wave || 2 * lane >= d) return;
-  l = lv[0];
+  for (int i0 = wave; i0 < parts; i0 += G * U) {
+    float2 p[U], v[U];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    l += lv[w];
-    x += ov[w][lane].x;
-    y += ov[w][lane].y;
+    for (int i = 0; i < U; ++i) {
+      const int64_t from = min(i0 + G * i, parts - 1) * rows + row;
+      p[i] = *reinterpret_cast<const float2*>(pml + from * 2);
+      v[i] = *reinterpret_cast<const float2*>(po + from * d + at);
+    }
+    float mt = m;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mt = fmaxf(mt, p[i].x);
+    const float alpha = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mt);       // without a maximum l is 0 or NaN, x and y are 0
+    l *= alpha, x *= alpha, y *= alpha;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i0 + G * i < parts) {
+        const float w = p[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[i].x - mt);
+        l += p[i].x == -INFINITY ? p[i].y : p[i].y * w;
+        x += v[i].x * w;
+        y += v[i].y * w;
+      }
+    m = mt;
   }
+  if constexpr (G > 1) {
+    ov[wave][lane] = make_float2(x, y);
+    if (lane == 0) mv[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave) return;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < G; ++g) mt = fmaxf(mt, mv[g].x);
+    l = x = y = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float w = mv[g].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv[g].x - mt);
+      l += mv[g].x == -INFINITY ? mv[g].y : mv[g].y * w;
+      x += ov[g][lane].x * w;
+      y += ov[g][lane].y * w;
+    }
+  }
+  if (2 * lane >= d) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack16<DT>(x * inv, y * inv);
 }
 
-// A workgroup has 16 rows, or 32 where there are more. The keys of a text go to as many parts as make two workgroups a CU, none
-// under 256 keys if the texts are as long as the table has room for: a part is its share of the keys that there are.
-void cache_plan(CacheArgs& a) {
-  const int64_t rows = (int64_t)a.N * (a.nh / a.nkv), cus = device_cus();
-  a.rblocks = (int)cdiv(rows, rows <= 16 ? 16 : 32);
-  const int64_t wgs = (int64_t)a.B * a.nkv * a.rblocks, room = (int64_t)a.P << a.logg;
-  a.parts = (int)std::max<int64_t>(1, std::min(2 * cus / wgs, cdiv(room, 256)));
+// How a call is split. A workgroup has up to 48 rows (heads over 96 dims: 32, more do not fit the registers): rows in one
+// workgroup share the widening of K and V. Up to a workgroup a CU, eight waves share out the keys, and a text's keys go to as
+// many parts as fill the CUs, none under 512 keys; with more of them four waves do, two workgroups side by side on a CU, and
+// parts are for balance, none under 2048 keys. A part is its share of the keys that there are; the host knows only how long
+// texts can be. Measured, eight waves / four (texts x longest, 16 / 8 heads of 128): 4 x 330 7.3 / 8.3 us, 20 x 600 9.2 / 9.9, 24 x 2000
+// 19.8 / 20.8, 8 x 32768 80.7 / 82.8, 48 x 1000 23.1 / 19.5, 64 x 600 20.6 / 16.9, 48 x 8192 116.5 / 114.4 (one part 137, two
+// 119, four 115, five 114); 1 x 131000 on 4 kv heads: 64 parts 16.6, 128 19.9.
+struct CachePlan {
+  int blocks, rblocks, parts;
+  bool eight;
+  explicit CachePlan(const CacheArgs& a) {
+    const int64_t rows = (int64_t)a.N * (a.nh / a.nkv), cus = device_cus(), sixteens = cdiv(rows, 16);
+    rblocks = (int)cdiv(sixteens, a.d > 96 ? 2 : 3);
+    blocks = (int)cdiv(sixteens, rblocks);
+    const int64_t wgs = (int64_t)a.B * a.nkv * rblocks, room = (int64_t)a.P << a.logg;
+    eight = wgs <= cus;
+    parts = (int)std::max<int64_t>(1, eight ? std::min(cus / wgs, cdiv(room, 512)) : std::min(8 * cus / wgs, room / 2048));
+  }
+};
+
+template <int DT, int D, int RB, bool EXACT>
+void cache_waves(const CacheArgs& a, bool eight, hipStream_t st) {
+  const unsigned grid = (unsigned)(cdiv(a.items, 8) * 8 * a.rblocks);
+  if (eight) cache_kernel<DT, D, RB, 8, EXACT><<<grid, 512, 0, st>>>(a);
+  else cache_kernel<DT, D, RB, 4, EXACT><<<grid, 256, 0, st>>>(a);
+}
+
+template <int DT, int D, bool EXACT>
+void cache_rows(const CacheArgs& a, const CachePlan& p, hipStream_t st) {
+  if (p.blocks == 1) cache_waves<DT, D, 1, EXACT>(a, p.eight, st);
+  else if (p.blocks == 2) cache_waves<DT, D, 2, EXACT>(a, p.eight, st);
+  else if constexpr (D <= 96) cache_waves<DT, D, 3, EXACT>(a, p.eight, st);
 }
 
 template <int DT, int D>
-int cache_go(const CacheArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.N * (a.nh / a.nkv), grid = (int64_t)a.B * a.nkv * a.rblocks * a.parts;
-  if (rows <= 16) cache_kernel<DT, D, 1, 4><<<(unsigned)grid, 256, 0, st>>>(a);
-  else cache_kernel<DT, D, 2, 4><<<(unsigned)grid, 256, 0, st>>>(a);
+void cache_dims(const CacheArgs& a, const CachePlan& p, hipStream_t st) {
+  if (a.d == D) cache_rows<DT, D, true>(a, p, st);
+  else cache_rows<DT, D, false>(a, p, st);
+}
+
+template <int DT>
+int cache_go(const CacheArgs& a, const CachePlan& p, hipStream_t st) {
+  if (a.d <= 32) cache_dims<DT, 32>(a, p, st);
+  else if (a.d <= 64) cache_dims<DT, 64>(a, p, st);
+  else if (a.d <= 96) cache_dims<DT, 96>(a, p, st);
+  else cache_dims<DT, 128>(a, p, st);
   if (a.parts > 1) {
     const int64_t all = (int64_t)a.B * a.N * a.nh;
-    cache_join_kernel<DT><<<(unsigned)all, 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.c, a.out);
+    // a wave a row for few parts, which many rows have (2240 rows of 4 parts 4.0 us; four waves a row and sixteen loads 8)
+    if (a.parts <= 4) cache_join_kernel<DT, 1, 4><<<(unsigned)cdiv(all, 4), 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
+    else if (a.parts <= 16) cache_join_kernel<DT, 4, 4><<<(unsigned)all, 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
+    else cache_join_kernel<DT, 4, 16><<<(unsigned)all, 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
   }
   return launch_status("attention_cache");
 }
@@ -895,8 +1116,8 @@ int64_t xdna_attention_cache_ws_bytes(int64_t B, int64_t N, int nh, int nkv, int
   if (B == 0 || N == 0) return 0;
   CacheArgs a{};
   a.B = (int)B, a.N = (int)N, a.nh = nh, a.nkv = nkv, a.d = d, a.P = (int)P, a.logg = log2_page(page);
-  cache_plan(a);
-  return a.parts > 1 ? (int64_t)a.parts * B * N * nh * (d + 2) * 4 : 0;
+  const CachePlan p(a);
+  return p.parts > 1 ? (int64_t)p.parts * B * N * nh * (d + 2) * 4 : 0;
 }
 
 int xdna_attention_cache(const void* q, int dtype, const int64_t* strides, const void* kpages, const void* vpages, const float* kscales,
@@ -921,14 +1142,15 @@ int xdna_attention_cache(const void* q, int dtype, const int64_t* strides, const
   a.c = std::max(fabsf(scale) * 1.44269504088896340736f, 1.17549435e-38f);    // above 0: an unseen key's -inf stays one
   a.sign = scale < 0.0f ? 0x80008000u : 0u;
   a.out = static_cast<uint16_t*>(out);
-  cache_plan(a);
+  const CachePlan p(a);
+  a.parts = p.parts, a.rblocks = p.rblocks, a.items = (int)(p.parts * B * nkv);
+  a.by_rblocks = Divisor(a.rblocks), a.by_nkv = Divisor(nkv), a.by_b = Divisor(B), a.by_grp = Divisor(nh / nkv), a.by_parts = Divisor(a.parts);
   const int64_t rows = B * N * nh, need = a.parts > 1 ? a.parts * rows * (d + 2) * 4 : 0;
   XDNA_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need), "workspace too small or misaligned");
   a.po = static_cast<float*>(ws);
   a.pml = a.po + (int64_t)a.parts * rows * d;
   hipStream_t st = as_stream(stream);
-  if (dtype == XDNA_BF16) return d > 64 ? cache_go<XDNA_BF16, 128>(a, st) : cache_go<XDNA_BF16, 64>(a, st);
-  return d > 64 ? cache_go<XDNA_F16, 128>(a, st) : cache_go<XDNA_F16, 64>(a, st);
+  return dtype == XDNA_BF16 ? cache_go<XDNA_BF16>(a, p, st) : cache_go<XDNA_F16>(a, p, st);
 }
 
 }  // extern "C"
