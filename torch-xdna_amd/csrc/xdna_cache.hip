@@ -67,6 +67,7 @@ struct AppendArgs {
   float magnitude;
   uint16_t* qout;
   int items, qtokens;                   // pages that the new tokens can fall into, of all texts; tokens of a workgroup of q
+  int both;                             // the smaller of the numbers of heads' pages and of workgroups of q
 };
 
 // A text's part of the call: its tokens [s0, s1) go to the places len ..
@@ -125,11 +126,20 @@ __device__ __forceinline__ float group_amax(float v, float* part) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(part[0], part[1]), __builtin_elementwise_maximum(part[2], part[3]));
 }
 
-// round_half_even(x / s) as a byte; a block of zeros (s == 0) is zeros; a value that is not a number, or of a block that
-// holds one or an infinity, is 0 (its scale is not finite, so the whole block reads as NaN).
-__device__ __forceinline__ int quant_byte(float x, float s) {
-  const float t = s > 0.0f ? rintf(x / s) : 0.0f;
-  return t == t ? (int)fminf(fmaxf(t, -127.0f), 127.0f) : 0;
+// Eight values as bytes, round_half_even(x / s), two words. By a product with the reciprocal and a division where that is near a
+// half (quant_pack, the same integers) as long as the reciprocal is a normal number. Blocks of zeros (s == 0), and those
+// that hold a value that is not finite (s NaN: all of it reads as NaN), are zeros.
+__device__ __forceinline__ void quant8(const float (&x)[8], float s, float r, uint32_t (&w)[2]) {
+  if (s >= 0x1p-100f) return quant_pack<8>(x, s, r, w);          // s is the workgroup's
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    w[g] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float t = s > 0.0f ? rintf(x[4 * g + e] / s) : 0.0f;
+      w[g] |= (uint32_t)((int)fminf(fmaxf(t, -127.0f), 127.0f) & 255) << (8 * e);
+    }
+  }
 }
 
 // A unit of a key: from the call (turned), or from the open page.
@@ -169,35 +179,36 @@ __device__ __forceinline__ void key_to_tail(const AppendArgs& a, int b, int kvh,
   store_upto8<DT>(a.ktail, at + u.b, u.nb, q);
 }
 
-__device__ __forceinline__ void store_bytes(int8_t* to, int n, const float (&x)[8], float s) {
-  int w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = quant_byte(x[e], s);
+__device__ __forceinline__ void store_bytes(int8_t* to, int n, const float (&x)[8], float s, float r) {
+  uint32_t w[2];
+  quant8(x, s, r, w);
   if (n == 8) {
     typedef uint32_t u32x2_1 __attribute__((ext_vector_type(2), aligned(1)));
-    u32x2_1 v;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      v[h] = (w[4 * h] & 255) | (w[4 * h + 1] & 255) << 8 | (w[4 * h + 2] & 255) << 16 | (uint32_t)w[4 * h + 3] << 24;
-    *reinterpret_cast<u32x2_1*>(to) = v;
+    *reinterpret_cast<u32x2_1*>(to) = u32x2_1{w[0], w[1]};
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) to[e] = (int8_t)w[e];
+      if (e < n) to[e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
   }
 }
 
-// A workgroup has a page of one head's keys (blockIdx.y 0) or values (1), or some tokens of all heads' queries (2, the first
-// qblocks). Texts whose open page holds old tokens: only their first page's workgroup reads the ring, and writes what would
+// A workgroup has a page of one head's keys (kind 0) or values (1), or some tokens of all heads' queries (2); kinds in turn, so that
+// those that compute more and those that read more share a CU. Texts whose open page holds old tokens: only their first page's workgroup reads the ring, and writes what would
 // fall on the old tokens' places after that. U: units of keys a thread has.
-template <int DT, bool INTER, int U>
+template <int DT, bool INTER, int U, int KINDS>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float part[4];
   const int g = 1 << a.logg;
-  if (blockIdx.y == 2) {
+  int index = blockIdx.x / KINDS, kind = blockIdx.x - index * KINDS;
+  if (KINDS == 3 && index >= a.both) {          // of one sort there are no more
+    const int rest = blockIdx.x - 3 * a.both;
+    if (a.items * a.nkv > a.both) index = a.both + (rest >> 1), kind = rest & 1;
+    else index = a.both + rest, kind = 2;
+  }
+  if (KINDS == 3 && kind == 2) {
     __shared__ float cs[256], sn[256];
     __shared__ int known[16];
-    const int64_t t0 = (int64_t)blockIdx.x * a.qtokens;
+    const int64_t t0 = (int64_t)index * a.qtokens;
     if (t0 >= a.T) return;
     const int n = (int)min<int64_t>(a.qtokens, a.T - t0);
     for (int i = threadIdx.x; i < n * max(1, a.half); i += 256) {
@@ -255,7 +266,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
     return;
   }
-  const int item = blockIdx.x / a.nkv, kvh = blockIdx.x - item * a.nkv;
+  const int item = index / a.nkv, kvh = index - item * a.nkv;
   if (item >= a.items) return;
   int b, nth;
   if (a.starts) {
@@ -277,7 +288,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   // places of the ring that old tokens hold while the first page's workgroup reads them: written by it, afterwards
   const int later = (x.len & (g - 1)) ? (page0 << a.logg) + a.R : 0x7fffffff, oldest = x.end - a.R;
   const int64_t head = (int64_t)b * a.nkv + kvh, block = (int64_t)id * a.nkv + kvh;
-  if (blockIdx.y == 0) {
+  if (kind == 0) {
     const int per_token = units_of(a.d, a.half), units = g * per_token;
     float p[U][8], q[U][8], top = 0.0f;
 #pragma unroll
@@ -294,7 +305,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       }
     }
     if (whole) {
-      const float amax = group_amax(top, part), s = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf("");
+      const float amax = group_amax(top, part), s = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf(""), r = 1.0f / s;
       if (good) {
         if (threadIdx.x == 0) a.ks[block] = s;
 #pragma unroll
@@ -303,8 +314,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
           if (at >= units) continue;
           const Unit u = unit_of<INTER>(at - tok * per_token, a.d, a.half);
           int8_t* const to = a.kp + (block * g + tok) * a.d;
-          store_bytes(to + u.a, u.na, p[i], s);
-          store_bytes(to + u.b, u.nb, q[i], s);
+          store_bytes(to + u.a, u.na, p[i], s, r);
+          store_bytes(to + u.b, u.nb, q[i], s, r);
         }
       }
     }
@@ -348,17 +359,26 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
   }
   if (whole) {
-    const float amax = group_amax(top, part), s = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf("");
+    const float amax = group_amax(top, part), s = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf(""), r = 1.0f / s;
     if (good) {
       if (threadIdx.x == 0) a.vs[block] = s;
-      const int chunks = g >> 4, tasks = a.d * chunks;
+      // two dims of 8 tokens: a word of LDS a token, 8 bytes of either dim's row of the page
+      const int logc = a.logg - 3, tasks = (a.d >> 1) << logc;
       for (int i = threadIdx.x; i < tasks; i += 256) {
-        const int dim = i / chunks, c = i - dim * chunks;
-        u32x4 w = {0, 0, 0, 0};
+        const int pair = i >> logc, c = i & ((1 << logc) - 1);
+        float lo[8], hi[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          w[e >> 2] |= (uint32_t)(quant_byte(load_as_f32<DT>(vl, (16 * c + e) * ld + dim), s) & 255) << (8 * (e & 3));
-        *reinterpret_cast<u32x4*>(a.vp + (block * a.d + dim) * g + 16 * c) = w;
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t y = *reinterpret_cast<const uint32_t*>(vl + (8 * c + e) * ld + 2 * pair);
+          lo[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)y) : bf16_bits_to_f32((uint16_t)y);
+          hi[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)(y >> 16)) : bf16_bits_to_f32((uint16_t)(y >> 16));
+        }
+        uint32_t w[2];
+        int8_t* const to = a.vp + (block * a.d + 2 * pair) * g + 8 * c;
+        quant8(lo, s, r, w);
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        quant8(hi, s, r, w);
+        *reinterpret_cast<uint2*>(to + g) = make_uint2(w[0], w[1]);
       }
     }
   }
@@ -374,18 +394,24 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
 }
 
-template <int DT, bool INTER>
-int append_go(const AppendArgs& a, hipStream_t st) {
+template <int DT, bool INTER, int KINDS>
+int append_go(AppendArgs a, hipStream_t st) {
   const int g = 1 << a.logg;
-  const int64_t blocks = (int64_t)a.items * a.nkv, qblocks = a.q ? cdiv(a.T, a.qtokens) : 0;
-  const dim3 grid((unsigned)std::max(blocks, qblocks), a.q ? 3 : 2);
+  const int64_t blocks = (int64_t)a.items * a.nkv, qblocks = KINDS == 3 ? cdiv(a.T, a.qtokens) : 0;
+  a.both = (int)std::min(blocks, qblocks);
+  const unsigned grid = (unsigned)(2 * blocks + qblocks);
   const int per = (int)cdiv((int64_t)g * units_of(a.d, a.half), 256);
   const unsigned lds = (unsigned)(g * (a.d + 2) * 2);
-  if (per <= 1) append_kernel<DT, INTER, 1><<<grid, 256, lds, st>>>(a);
-  else if (per <= 2) append_kernel<DT, INTER, 2><<<grid, 256, lds, st>>>(a);
-  else if (per <= 3) append_kernel<DT, INTER, 3><<<grid, 256, lds, st>>>(a);
-  else append_kernel<DT, INTER, 5><<<grid, 256, lds, st>>>(a);
+  if (per <= 1) append_kernel<DT, INTER, 1, KINDS><<<grid, 256, lds, st>>>(a);
+  else if (per <= 2) append_kernel<DT, INTER, 2, KINDS><<<grid, 256, lds, st>>>(a);
+  else append_kernel<DT, INTER, 5, KINDS><<<grid, 256, lds, st>>>(a);
   return launch_status("cache_append");
+}
+
+template <int DT>
+int append_kinds(const AppendArgs& a, bool interleaved, hipStream_t st) {
+  if (a.q) return interleaved ? append_go<DT, true, 3>(a, st) : append_go<DT, false, 3>(a, st);
+  return interleaved ? append_go<DT, true, 2>(a, st) : append_go<DT, false, 2>(a, st);
 }
 
 // ------------------------------------------------------------------------------ attention_cache
@@ -1104,11 +1130,10 @@ int xdna_cache_append(const void* k, const void* v, int dtype, const int64_t* st
   a.each = starts ? 0 : (int)(T / B);
   const int64_t items = starts ? T / page + 2 * B : B * ((a.each + page - 2) / page + 1);
   a.qtokens = (int)std::min<int64_t>(half ? std::min<int64_t>(16, std::max<int64_t>(1, 256 / half)) : 16, std::max<int64_t>(1, T / (2 * device_cus())));
-  XDNA_REQUIRE(items * nkv <= MAX_LAUNCH_THREADS / 256 && T <= MAX_LAUNCH_THREADS / 256, "too many tokens");
+  XDNA_REQUIRE(items * nkv <= MAX_LAUNCH_THREADS / 768 && T <= MAX_LAUNCH_THREADS / 768, "too many tokens");
   a.items = (int)items;
   hipStream_t st = as_stream(stream);
-  if (dtype == XDNA_BF16) return interleaved ? append_go<XDNA_BF16, true>(a, st) : append_go<XDNA_BF16, false>(a, st);
-  return interleaved ? append_go<XDNA_F16, true>(a, st) : append_go<XDNA_F16, false>(a, st);
+  return dtype == XDNA_BF16 ? append_kinds<XDNA_BF16>(a, interleaved, st) : append_kinds<XDNA_F16>(a, interleaved, st);
 }
 
 int64_t xdna_attention_cache_ws_bytes(int64_t B, int64_t N, int nh, int nkv, int d, int64_t P, int64_t page) {

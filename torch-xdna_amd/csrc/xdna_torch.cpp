@@ -522,7 +522,8 @@ R Below<R(A...)>::call(c10::DispatchKeySet ks, A... a) {
   R out;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
-    out = op.redispatch(ks & c10::after_autograd_keyset, a...);
+    // past ADInplaceOrView too, which for an op that writes is a kernel in Python: what it would count, written() counts
+    out = op.redispatch(ks & c10::after_ADInplaceOrView_keyset, a...);
   }
   if constexpr (OP == APPEND) written(a...);
   if (grad) {
