@@ -254,14 +254,16 @@ def test_attention_long(gpu, dtype):
 def test_attention_scales(gpu, dtype):
     """Values' scales that grow and fall by powers of ten from page to page, scales of zero, and the softmax's scale: none, zero,
     negative."""
-    cache = random_cache(2, 2, 32, 400, 16, dtype, dev=gpu)
-    cache.vscales.copy_(10.0 ** torch.randint(-6, 3, cache.vscales.shape))
-    cache.vscales[::5] = 0
-    cache.kscales[::7] = 0
-    q = _query(2, 2, 4, 32, dtype, gpu)
-    lens = [390, 401]
-    for scale in (None, 0.0, -0.2, 1e-3, 1.5):
-        _within(lm.attention_cache(q, cache, _lens(lens, gpu), scale), *cache_reference(q, cache, lens, scale))
+    for seed in range(8):
+        page, g = (16, 32, 64, 128)[seed % 4], torch.Generator().manual_seed(seed)
+        cache = random_cache(2, 2, 32, 400, page, dtype, seed=seed, dev=gpu)
+        cache.vscales.copy_(10.0 ** torch.randint(-6, 3, cache.vscales.shape, generator=g))
+        cache.vscales[::5] = 0
+        cache.kscales[::7] = 0
+        q = _query(2, 2, 4, 32, dtype, gpu, seed=seed)
+        lens = [390, 401]
+        for scale in (None, 0.0, -0.2, 1e-3, 1.5):
+            _within(lm.attention_cache(q, cache, _lens(lens, gpu), scale), *cache_reference(q, cache, lens, scale))
     tiny = cache._replace(vscales=torch.full_like(cache.vscales, 1e-30))
     # under the open page's values such a page is next to nothing; without it, it is all there is
     for n in ([384, 400], [390, 395]):

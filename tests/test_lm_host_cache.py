@@ -135,6 +135,9 @@ def test_append_host(page, turned, interleaved, dtype):
     other = clone(start)
     ops.cache_append(k, v, *other, lens, starts, q, freqs, 1.0, interleaved)
     assert all(torch.equal(a, b) for a, b in zip(other, cache))
+    for args in ((None, None, None), (starts, q, freqs)):
+        torch.library.opcheck(ops.cache_append.default, (k[:84] if args[0] is None else k, v[:84] if args[0] is None else v, *clone(start), lens, *args),
+                              test_utils=("test_schema", "test_faketensor"))
     small = random_cache(1, kv, dim, 4 * page, page, dtype, places=page)
     want, got = clone(small), clone(small)
     lm.cache_append(want, _i32(0), k[:3 * page], v[:3 * page], None, None, freqs)
@@ -320,7 +323,7 @@ def test_entry_point_checks():
     assert norm(rows=0) == 0 and norm(width=0) == 0
     neg = (ctypes.c_int64 * 6)(64, 64, 64, -64, 64, 64)
     for bad in (dict(xd=2), dict(dt=3), dict(pd=3), dict(wd=7), dict(x=None), dict(y=None), dict(total=None), dict(s=None), dict(s=neg), dict(inner=0),
-                dict(o=None, gate=p), dict(o=None, post=p), dict(width=32769), dict(rows=-1), dict(rows=1 << 23)):
+                dict(o=None, gate=p), dict(o=None, post=p), dict(width=32769), dict(rows=-1), dict(rows=1 << 40)):
         assert norm(**bad) == -1, bad
 
     def append(k=p, v=p, dt=1, s=st, kp=p, vt=p, table=p, lens=p, starts=p, q=None, f=p, half=8, out=p, t=4, b=2, P=4, pages=8, g=16, r=32, nh=4,
@@ -337,7 +340,7 @@ def test_entry_point_checks():
     ws_bytes = L.xdna_attention_cache_ws_bytes
     assert ws_bytes(0, 1, 4, 2, 16, 4, 16) == 0
     for bad in ((1, 1, 3, 2, 16, 4, 16), (1, 1, 4, 2, 20, 4, 16), (1, 1, 4, 2, 16, 4, 48), (-1, 1, 4, 2, 16, 4, 16), (1, -1, 4, 2, 16, 4, 16),
-                (1 << 22, 1, 4, 2, 16, 4, 16)):
+                (1 << 21, 1, 4, 2, 16, 4, 16)):
         assert ws_bytes(*bad) == -1, bad
 
     def attend(q=p, dt=1, s=st, kp=p, kt=p, table=p, lens=p, b=2, n=1, P=4, pages=8, g=16, r=32, nh=4, kv=2, d=16, out=p):

@@ -17,9 +17,8 @@
 //     scores of keys 16 h .. 16 h + 15 for query row l % 16; lane h's 16 bytes of K are dims 16 (h + 4 j) .. + 15, two steps.
 //   O^T = V^T P^T: those 16 scores are lane h's values of two 32-deep steps, and 16 bytes of a row of V are the same keys.
 // The products with pages run in float16, which holds int8 exactly and is the cheaper to widen to: bfloat16 rows of q are brought
-// into its range by a power of two. K's scale goes into the exponent's factor, in float32; V's, as a share of the largest met so
-// far, into P before its rounding to float16, and O is held in units of that largest one. The open page's products run
-// in the tensors' own type.
+// into its range by a power of two. K's scale goes into the exponent's factor, in float32; V's into the weights that P holds,
+// before their rounding to float16. The open page's products run in the tensors' own type.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,17 +35,6 @@ namespace {
 typedef __bf16 bf16x8c __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x2c __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8c __attribute__((ext_vector_type(8)));
-
-// n / d for 0 <= n < 2^31 by a product: m = 2^32 (2^s - d) / d + 1, s = ceil(log2 d); q = (n + high(n m)) >> s
-struct Divisor {
-  uint32_t m, s, d;
-  Divisor() = default;
-  explicit Divisor(int64_t by) : m(0), s(0), d((uint32_t)by) {
-    while ((1ull << s) < d) ++s;
-    m = (uint32_t)((((1ull << s) - d) << 32) / d + 1);
-  }
-  __device__ __forceinline__ int of(int n) const { return (int)(((uint32_t)n + __umulhi((uint32_t)n, m)) >> s); }
-};
 
 bool sixteen(int dtype) { return dtype == XDNA_BF16 || dtype == XDNA_F16; }
 int log2_page(int64_t g) { return g == 16 ? 4 : g == 32 ? 5 : g == 64 ? 6 : g == 128 ? 7 : -1; }
@@ -67,6 +55,8 @@ struct AppendArgs {
   float magnitude;
   uint16_t* qout;
   int items, qtokens;                   // pages that the new tokens can fall into, of all texts; tokens of a workgroup of q
+  Divisor by_nkv, by_each;              // heads; pages of a text, without starts
+  Divisor by_token, by_value, by_qtoken, by_head;   // units of a token of keys, of values, of all q heads, of a head
   int both;                             // the smaller of the numbers of heads' pages and of workgroups of q
 };
 
@@ -239,9 +229,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       }
     }
     __syncthreads();
-    const int per_head = units_of(a.d, a.half), per_token = per_head * a.nh;
+    const int per_head = a.by_head.d, per_token = a.by_qtoken.d;
     for (int i = threadIdx.x; i < n * per_token; i += 256) {
-      const int tok = i / per_token, at = i - tok * per_token, head = at / per_head;
+      const int tok = a.by_qtoken.of(i), at = i - tok * per_token, head = a.by_head.of(at);
       const Unit u = unit_of<INTER>(at - head * per_head, a.d, a.half);
       const int64_t from = (t0 + tok) * a.qt + head * a.qh, to = ((t0 + tok) * a.nh + head) * a.d;
       float p[8], q[8];
@@ -266,7 +256,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
     return;
   }
-  const int item = index / a.nkv, kvh = index - item * a.nkv;
+  const int item = a.by_nkv.of(index), kvh = index - item * a.nkv;
   if (item >= a.items) return;
   int b, nth;
   if (a.starts) {
@@ -275,7 +265,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     nth = item - __builtin_amdgcn_readfirstlane(first);
   } else {
     const int each = ((a.each + g - 2) >> a.logg) + 1;
-    b = item / each;
+    b = a.by_each.of(item);
     nth = item - b * each;
   }
   const Text x = text_of(a, b);
@@ -287,17 +277,20 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const bool good = id >= 0 && id < a.pages;      // no page for it: its tokens pass through the ring only
   // places of the ring that old tokens hold while the first page's workgroup reads them: written by it, afterwards
   const int later = (x.len & (g - 1)) ? (page0 << a.logg) + a.R : 0x7fffffff, oldest = x.end - a.R;
-  const int64_t head = (int64_t)b * a.nkv + kvh, block = (int64_t)id * a.nkv + kvh;
+  const bool writes_later = nth == 0 && later < x.end;
   if (kind == 0) {
-    const int per_token = units_of(a.d, a.half), units = g * per_token;
+    const int per_token = a.by_token.d, units = g * per_token;
     float p[U][8], q[U][8], top = 0.0f;
+    Unit u[U];
+    int pos[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int at = i * 256 + threadIdx.x, tok = at / per_token, pos = begin + tok;
-      if (at >= units || pos >= hi || (pos < lo && !whole)) continue;
-      const Unit u = unit_of<INTER>(at - tok * per_token, a.d, a.half);
-      key_unit<DT, INTER>(a, x, b, kvh, u, pos, p[i], q[i]);
-      if (pos >= lo && pos >= oldest && pos < later) key_to_tail<DT>(a, b, kvh, u, pos, p[i], q[i]);
+      const int at = i * 256 + threadIdx.x, tok = a.by_token.of(at);
+      pos[i] = at < units ? begin + tok : 0x7fffffff;
+      u[i] = unit_of<INTER>(at - tok * per_token, a.d, a.half);
+      if (pos[i] >= hi || (pos[i] < lo && !whole)) continue;
+      key_unit<DT, INTER>(a, x, b, kvh, u[i], pos[i], p[i], q[i]);
+      if (pos[i] >= lo && pos[i] >= oldest && pos[i] < later) key_to_tail<DT>(a, b, kvh, u[i], pos[i], p[i], q[i]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = __builtin_elementwise_maximum(top, fabsf(p[i][e]));
@@ -305,48 +298,49 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       }
     }
     if (whole) {
-      const float amax = group_amax(top, part), s = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf(""), r = 1.0f / s;
+      const int64_t block = (int64_t)id * a.nkv + kvh;
+      const float amax = group_amax(top, part), scale = __builtin_isfinite(amax) ? amax / 127.0f : __builtin_nanf(""), r = 1.0f / scale;
       if (good) {
-        if (threadIdx.x == 0) a.ks[block] = s;
+        if (threadIdx.x == 0) a.ks[block] = scale;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const int at = i * 256 + threadIdx.x, tok = at / per_token;
-          if (at >= units) continue;
-          const Unit u = unit_of<INTER>(at - tok * per_token, a.d, a.half);
-          int8_t* const to = a.kp + (block * g + tok) * a.d;
-          store_bytes(to + u.a, u.na, p[i], s, r);
-          store_bytes(to + u.b, u.nb, q[i], s, r);
+          if (pos[i] >= hi) continue;
+          int8_t* const to = a.kp + (block * g + pos[i] - begin) * a.d;
+          store_bytes(to + u[i].a, u[i].na, p[i], scale, r);
+          store_bytes(to + u[i].b, u[i].nb, q[i], scale, r);
         }
       }
     }
-    if (nth == 0 && later < x.end) {
+    if (writes_later) {
       __syncthreads();
       const int from = max(later, oldest), n = (x.end - from) * per_token;
       for (int at = threadIdx.x; at < n; at += 256) {
-        const int tok = at / per_token;
-        const Unit u = unit_of<INTER>(at - tok * per_token, a.d, a.half);
+        const int tok = a.by_token.of(at);
+        const Unit v = unit_of<INTER>(at - tok * per_token, a.d, a.half);
         float pp[8], qq[8];
-        key_unit<DT, INTER>(a, x, b, kvh, u, from + tok, pp, qq);
-        key_to_tail<DT>(a, b, kvh, u, from + tok, pp, qq);
+        key_unit<DT, INTER>(a, x, b, kvh, v, from + tok, pp, qq);
+        key_to_tail<DT>(a, b, kvh, v, from + tok, pp, qq);
       }
     }
     return;
   }
   // values: through LDS, [token][d + 2] so that a walk along the tokens of 16 dims meets every bank
   extern __shared__ uint16_t vl[];
-  const int per_token = a.d / 8, units = g * per_token, ld = a.d + 2;
-  auto value = [&](int pos, int u, float (&p)[8]) {
+  const int per_token = a.by_value.d, units = g * per_token, ld = a.d + 2;
+  const int64_t head = (int64_t)b * a.nkv + kvh, block = (int64_t)id * a.nkv + kvh;
+  const auto value = [&](int pos, int u, float (&p)[8]) {
     if (pos >= x.len) return load8<DT>(a.v, (x.s0 + pos - x.len) * a.vt + kvh * a.vh + 8 * u, p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = load_as_f32<DT>(a.vtail, (head * a.d + 8 * u + e) * a.R + pos % a.R);
   };
-  auto to_tail = [&](int pos, int u, const float (&p)[8]) {
+  const auto to_tail = [&](int pos, int u, const float (&p)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) store_from_f32<DT>(a.vtail, (head * a.d + 8 * u + e) * a.R + pos % a.R, p[e]);
   };
   float top = 0.0f;
+#pragma unroll 4
   for (int at = threadIdx.x; at < units; at += 256) {
-    const int tok = at / per_token, u = at - tok * per_token, pos = begin + tok;
+    const int tok = a.by_value.of(at), u = at - tok * per_token, pos = begin + tok;
     if (pos >= hi || (pos < lo && !whole)) continue;
     float p[8];
     value(pos, u, p);
@@ -366,27 +360,27 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const int logc = a.logg - 3, tasks = (a.d >> 1) << logc;
       for (int i = threadIdx.x; i < tasks; i += 256) {
         const int pair = i >> logc, c = i & ((1 << logc) - 1);
-        float lo[8], hi[8];
+        float lo8[8], hi8[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t y = *reinterpret_cast<const uint32_t*>(vl + (8 * c + e) * ld + 2 * pair);
-          lo[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)y) : bf16_bits_to_f32((uint16_t)y);
-          hi[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)(y >> 16)) : bf16_bits_to_f32((uint16_t)(y >> 16));
+          lo8[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)y) : bf16_bits_to_f32((uint16_t)y);
+          hi8[e] = DT == XDNA_F16 ? f16_bits_to_f32((uint16_t)(y >> 16)) : bf16_bits_to_f32((uint16_t)(y >> 16));
         }
         uint32_t w[2];
         int8_t* const to = a.vp + (block * a.d + 2 * pair) * g + 8 * c;
-        quant8(lo, s, r, w);
+        quant8(lo8, s, r, w);
         *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        quant8(hi, s, r, w);
+        quant8(hi8, s, r, w);
         *reinterpret_cast<uint2*>(to + g) = make_uint2(w[0], w[1]);
       }
     }
   }
-  if (nth == 0 && later < x.end) {
+  if (writes_later) {
     __syncthreads();
     const int from = max(later, oldest), n = (x.end - from) * per_token;
     for (int at = threadIdx.x; at < n; at += 256) {
-      const int tok = at / per_token, u = at - tok * per_token;
+      const int tok = a.by_value.of(at), u = at - tok * per_token;
       float p[8];
       value(from + tok, u, p);
       to_tail(from + tok, u, p);
@@ -396,12 +390,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 template <int DT, bool INTER, int KINDS>
 int append_go(AppendArgs a, hipStream_t st) {
-  const int g = 1 << a.logg;
+  const int units = units_of(a.d, a.half), per = (int)cdiv((int64_t)units << a.logg, 256), g = 1 << a.logg;
   const int64_t blocks = (int64_t)a.items * a.nkv, qblocks = KINDS == 3 ? cdiv(a.T, a.qtokens) : 0;
   a.both = (int)std::min(blocks, qblocks);
-  const unsigned grid = (unsigned)(2 * blocks + qblocks);
-  const int per = (int)cdiv((int64_t)g * units_of(a.d, a.half), 256);
-  const unsigned lds = (unsigned)(g * (a.d + 2) * 2);
+  a.by_nkv = Divisor(a.nkv), a.by_each = Divisor(((a.each + g - 2) >> a.logg) + 1);
+  a.by_head = a.by_token = Divisor(units), a.by_value = Divisor(a.d / 8);
+  if (KINDS == 3) a.by_qtoken = Divisor((int64_t)units * a.nh);
+  const unsigned grid = (unsigned)(2 * blocks + qblocks), lds = (unsigned)((a.d + 2) * 2 << a.logg);
   if (per <= 1) append_kernel<DT, INTER, 1, KINDS><<<grid, 256, lds, st>>>(a);
   else if (per <= 2) append_kernel<DT, INTER, 2, KINDS><<<grid, 256, lds, st>>>(a);
   else append_kernel<DT, INTER, 5, KINDS><<<grid, 256, lds, st>>>(a);
@@ -468,72 +463,65 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A row's maximum follows the scores once they pass it by more than 2^SLACK: nearly never after a row's first keys, where
-// otherwise some row of sixteen finds a larger one at nearly every step, and all of O is multiplied. p are held 2^SHIFT times
-// as large, so that float16 takes them from 2^-23 of the maximum (normal) to 2^SLACK times it.
-constexpr float SLACK = 6.0f, SHIFT = 9.0f;
+// A row's maxima follow once they are passed by more than 2^SLACK: nearly never after a row's first keys, where otherwise some
+// row of sixteen finds a larger one at nearly every step, and all of O is multiplied. O's weights are held 2^SHIFT times as large,
+// so that float16 takes them from 2^-22 of the maximum (normal) to 2^(SLACK + 1) times it.
+constexpr float SLACK = 6.0f, SHIFT = 8.0f;
 template <int DT>
 constexpr uint32_t ALL_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
 
 // A wave's rows: RB blocks of 16, their maxima, sums and outputs. Rows of a (text, kv head) are the pairs (new token, q head
 // of the group), so that the heads that share K and V share their loads.
+// A key's weight in O is p times its values' scale, f 2^k with f in 1 .. 2: those weights have a maximum of their own, so that
+// pages whose scales lie far apart all reach float16 as near to a row's largest weight as they count.
 template <int D, int RB>
 struct Rows {
   static constexpr int ND = D / 16;
   f32x4 o[RB][ND];
-  float m[RB], l[RB];       // m in units of the exponent
-  int limit[RB];            // keys that the lane's row sees
-  float unit;               // O is held in units of it
+  float l[RB], m[RB];       // sum of p, 2^m its unit
+  float mo[RB];             // 2^(mo - SHIFT) is O's
 
-  // p of T tiles of 16 keys as the second product's operand: 2^(c score - m), c with K's scale
+  // The weights of T tiles of 16 keys as the second product's operand, 2^(c score) f 2^k in O's unit; c with K's scale, k and f
+  // the lane's. same: k is that of all 64 keys.
   template <int DT, int T>
-  __device__ __forceinline__ void weigh(const f32x4* sc, int rb, float c, float share, int* pf) {
-    float mx = sc[0][0];
+  __device__ __forceinline__ void weigh(const f32x4* sc, int rb, float c, float k, float f, bool same, int* pf) {
+    float top = sc[0][0];
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, sc[t][r]);
-    mx = quad_max(mx * c);
-    const bool grow = mx > m[rb] + SLACK;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m[rb] - mx) : 1.0f;      // from -inf: 0
-      l[rb] *= alpha;
+      for (int r = 0; r < 4; ++r) top = __builtin_elementwise_maximum(top, sc[t][r]);
+    top *= c;
+    const float mx = quad_max(top), mxo = same ? mx + k : quad_max(top + k);
+    const bool grow = mx > m[rb] + SLACK, growo = mxo > mo[rb] + SLACK;
+    if (__builtin_amdgcn_ballot_w64(grow || growo)) {
+      if (grow) {
+        l[rb] *= __builtin_amdgcn_exp2f(m[rb] - mx);                             // from -inf: 0
+        m[rb] = mx;
+      }
+      const float alpha = growo ? __builtin_amdgcn_exp2f(mo[rb] - mxo) : 1.0f;
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[rb][i] *= alpha;
-      m[rb] = grow ? mx : m[rb];
+      mo[rb] = growo ? mxo : mo[rb];
     }
-    const float mc = (m[rb] == -INFINITY ? 0.0f : m[rb]) - SHIFT;      // only -inf scores so far: p = 0
+    const float m0 = m[rb] == -INFINITY ? 0.0f : m[rb], mo0 = mo[rb] == -INFINITY ? 0.0f : mo[rb];       // only -inf scores so far: p = 0
+    const float shift = k + SHIFT - mo0, back = -(shift + m0);                   // of the weights, and from there to p
+    const bool far = __builtin_amdgcn_ballot_w64(back > 64.0f) != 0;             // too far for the weights to tell p
+    if (far) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) l[rb] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -m0));
+    }
+    const float scale = far ? 0.0f : __builtin_amdgcn_exp2f(back);
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -mc)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r + 1], c, -mc));
-        l[rb] += p0;
-        l[rb] += p1;
-        p0 *= share, p1 *= share;
-        pf[2 * t + r / 2] = (int)pack16<DT>(p0, p1);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, shift)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r + 1], c, shift));
+        l[rb] = __builtin_fmaf(p0, scale, l[rb]);
+        l[rb] = __builtin_fmaf(p1, scale, l[rb]);
+        pf[2 * t + r / 2] = (int)pack16<DT>(p0 * f, p1 * f);
       }
-  }
-
-  // units for a block of keys whose values have this scale; its share of the unit
-  __device__ __forceinline__ float share_of(float vs, bool uniform) {
-    float top = vs;
-    if (!uniform) {
-      // the largest number among the four groups of keys (fmaxf leaves out NaN)
-      auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    }
-    if (__builtin_amdgcn_ballot_w64(top > unit)) {
-      const float to = unit / top;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[rb][i] *= to;
-      unit = top;
-    }
-    return unit > 0.0f ? vs / unit : vs * 0.0f;
   }
 };
 
@@ -551,6 +539,7 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   __shared__ float ml[2][W][RB][16];
   __shared__ i32x4 ql[QLDS ? RB * S : 1][64];
   __shared__ float qls[QLDS ? RB : 1][16];
+  __shared__ int qlim[QLDS ? RB : 1][16];
   const int lane = threadIdx.x & 63, h = lane >> 4, i16 = lane & 15, hk = i16 >> 2;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = a.by_grp.d, nrows = a.N * grp, g = 1 << a.logg, d = EXACT ? D : a.d;
@@ -565,15 +554,16 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   const int end = min(to, steps), row0 = rblock * 16 * RB, dchunks = d >> 4;
 
   Rows<D, RB> w;
-  w.unit = 0.0f;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    w.limit[rb] = len - a.N + a.by_grp.of(min(row0 + 16 * rb + i16, nrows - 1)) + 1;
-    w.m[rb] = -INFINITY;
+    w.m[rb] = w.mo[rb] = -INFINITY;
     w.l[rb] = 0.0f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) w.o[rb][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
+  // keys that the lane's row of a block sees
+  const auto limit_of = [&](int rb) { return len - a.N + a.by_grp.of(min(row0 + 16 * rb + i16, nrows - 1)) + 1; };
+  const int limit0 = limit_of(0);
   // the lane's row of a block: its new token and q head. Found again where it is needed: held, it costs the loop registers.
   const auto row_of = [&](int rb, int& n, int& head) {
     int at = row0;
@@ -618,7 +608,7 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
     }
   };
   i32x4 qf[S];
-  float back[RB];
+  float back = 1.0f;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
     if (!QLDS || wave == rb) load_q(rb, qf);
@@ -673,23 +663,24 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   }
   if constexpr (QLDS) {
     if (wave < RB) {
-      half_q(qf, back[0]);
+      half_q(qf, back);
 #pragma unroll
       for (int s = 0; s < S; ++s) ql[wave * S + s][lane] = qf[s];
-      if (h == 0) qls[wave][i16] = back[0];
+      if (h == 0) qls[wave][i16] = back * a.c, qlim[wave][i16] = limit_of(wave);
     }
     __syncthreads();
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) back[rb] = qls[rb][i16];
   } else {
-    half_q(qf, back[0]);
+    half_q(qf, back);
+    back *= a.c;
   }
+  const auto factor = [&](int rb) { return QLDS ? qls[rb][i16] : back; };
+  const auto limit = [&](int rb) { return QLDS ? qlim[rb][i16] : limit0; };
   const auto q_frag = [&](int rb, int s) {
     if constexpr (QLDS) return ql[rb * S + s][lane];
     else return qf[s];
   };
   // the first row's tokens are the fewest that a row of this workgroup sees
-  const int sure = min(nfull, __builtin_amdgcn_readfirstlane(w.limit[0]));
+  const int sure = min(nfull, __builtin_amdgcn_readfirstlane(limit0));
 
   const auto pages = [&](auto more) {
     const int first = step * 64 + 16 * h, next = step + W;
@@ -697,7 +688,9 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
     const bool mine = good;
     // T tiles of 16 keys at a time: with more rows fewer scores in registers
     constexpr int T = RB == 1 ? 4 : 2;
-    float ks = ksc, share = 0.0f;
+    const float ks = ksc, vs = vsc;
+    const int e8 = (int)(__float_as_uint(vs) >> 23 & 255u) - 127;
+    const float vk = (float)e8, vf = __builtin_amdgcn_ldexpf(vs, -e8);          // f of a scale that is not finite is not
     const int8_t* next_v = nullptr;
 #pragma unroll
     for (int t0 = 0; t0 < 4; t0 += T) {
@@ -723,8 +716,6 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
         }
       }
       if (t0 + T == 4) {
-        const float vs = mine && first < nfull ? vsc : 0.0f;
-        if (T == 4) share = w.share_of(vs, g >= 64);
         if constexpr (more) {
           const int8_t* const next_k = k_base(next, asked_k);
           next_v = v_base(next, asked_v);
@@ -734,12 +725,10 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
           load_k(next_k);
           load_scales(id);
         }
-      } else {
-        share = w.share_of(mine && first < nfull ? vsc : 0.0f, g >= 64);
       }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const int lim = mine ? min(nfull, w.limit[rb]) : 0;
+        const int lim = mine ? min(nfull, limit(rb)) : 0;
         if (masked) {
 #pragma unroll
           for (int t = 0; t < T; ++t)
@@ -748,10 +737,10 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
               if (first + 4 * (t0 + t) + r >= lim) sc[rb][t][r] = -INFINITY;
         }
         // above 0, so that an unseen key's -inf stays one; the scales of a page that the row does not see do not matter
-        float c = __builtin_elementwise_maximum(ks * (back[rb] * a.c), 1.17549435e-38f);
+        float c = __builtin_elementwise_maximum(ks * factor(rb), 1.17549435e-38f);
         const bool unseen = masked && first >= lim;
         if (unseen) c = 1.0f;
-        w.template weigh<XDNA_F16, T>(sc[rb], rb, c, unseen ? 0.0f : share, reinterpret_cast<int*>(&pf[rb][0]));
+        w.template weigh<XDNA_F16, T>(sc[rb], rb, c, vk, unseen ? 0.0f : vf, g >= 64, reinterpret_cast<int*>(&pf[rb][0]));
       }
 #pragma unroll
       for (int i = 0; i < ND; ++i)
@@ -813,17 +802,16 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
     };
     load_half(0);
     const int first = nfull + at + 16 * h;
-    const float share = w.share_of(1.0f, true);
     i32x4 pf[RB][2];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int lim = w.limit[rb];
+      const int lim = limit(rb);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (first + 4 * t + r >= lim) sc[rb][t][r] = -INFINITY;
-      w.template weigh<DT, 4>(sc[rb], rb, a.c, share, reinterpret_cast<int*>(&pf[rb][0]));
+      w.template weigh<DT, 4>(sc[rb], rb, a.c, 0.0f, 1.0f, true, reinterpret_cast<int*>(&pf[rb][0]));
     }
     // Places without keys are zeros. What is not finite may belong to a key that some rows do not see (of one new token's rows
     // every row sees every key), and 0 times it would be NaN: taken out, and added below to the rows that see it.
@@ -895,7 +883,7 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
           for (int n = 0; n < ND; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (n == i && y[r] != 0.0f && nfull + at + key < w.limit[rb]) w.o[rb][n][r] += p * y[r];
+              if (n == i && y[r] != 0.0f && nfull + at + key < limit(rb)) w.o[rb][n][r] += p * y[r];
         }
       }
     }
@@ -913,9 +901,11 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
     }
   };
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
+  for (int rb = 0; rb < RB; ++rb) {
+    const float unit = w.mo[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.mo[rb] - SHIFT - w.m[rb]);       // O in p's
 #pragma unroll
-    for (int i = 0; i < ND; ++i) w.o[rb][i] *= w.unit;
+    for (int i = 0; i < ND; ++i) w.o[rb][i] *= unit;
+  }
   if (wave >= W / 2) leave(wave - W / 2);
   __syncthreads();
   if (wave < W / 2) {
@@ -1090,7 +1080,7 @@ int cache_go(const CacheArgs& a, const CachePlan& p, hipStream_t st) {
 
 bool cache_sizes_ok(int64_t B, int64_t N, int64_t nh, int64_t nkv, int64_t d, int64_t P, int64_t pages, int64_t g, int64_t R) {
   return B >= 0 && N >= 0 && nh >= 1 && nkv >= 1 && nh % nkv == 0 && nh < (1 << 16) && B < (1 << 22) && N < (1 << 22) &&
-         B * N * nh < (1ll << 22) && d >= 16 && d <= 128 && d % 16 == 0 && log2_page(g) >= 0 && P >= 0 && P * g < (1ll << 30) &&
+         B * N * nh < (1ll << 23) && d >= 16 && d <= 128 && d % 16 == 0 && log2_page(g) >= 0 && P >= 0 && P * g < (1ll << 30) &&
          pages >= 0 && pages < (1ll << 31) && R >= g && R % g == 0 && R < (1 << 16);
 }
 
@@ -1130,7 +1120,7 @@ int xdna_cache_append(const void* k, const void* v, int dtype, const int64_t* st
   a.each = starts ? 0 : (int)(T / B);
   const int64_t items = starts ? T / page + 2 * B : B * ((a.each + page - 2) / page + 1);
   a.qtokens = (int)std::min<int64_t>(half ? std::min<int64_t>(16, std::max<int64_t>(1, 256 / half)) : 16, std::max<int64_t>(1, T / (2 * device_cus())));
-  XDNA_REQUIRE(items * nkv <= MAX_LAUNCH_THREADS / 768 && T <= MAX_LAUNCH_THREADS / 768, "too many tokens");
+  XDNA_REQUIRE(2 * items * nkv + T <= MAX_LAUNCH_THREADS / 256, "too many tokens");
   a.items = (int)items;
   hipStream_t st = as_stream(stream);
   return dtype == XDNA_BF16 ? append_kinds<XDNA_BF16>(a, interleaved, st) : append_kinds<XDNA_F16>(a, interleaved, st);

@@ -11,6 +11,17 @@
 
 namespace xdna {
 
+// n / d for 0 <= n < 2^31 by a product: m = 2^32 (2^s - d) / d + 1, s = ceil(log2 d); q = (n + high(n m)) >> s
+struct Divisor {
+  uint32_t m, s, d;
+  Divisor() = default;
+  explicit Divisor(int64_t by) : m(0), s(0), d((uint32_t)by) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((((1ull << s) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)(((uint32_t)n + __umulhi((uint32_t)n, m)) >> s); }
+};
+
 constexpr double QUARTERS = 0.636619772367581343;      // 2 / pi
 
 struct Turn {

@@ -23,6 +23,7 @@ struct RotaryArgs {
   int wide;
   const double* freqs;
   int half, d, heads, tokens; // tokens of a workgroup
+  Divisor by_head, by_token, by_half;           // units of a head, of a token; pairs
   int64_t T;
   float magnitude;
   void* y;
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n = (int)min<int64_t>(a.tokens, a.T - t0);
   for (int i = threadIdx.x; i < n * a.half; i += 256) {
-    const int tok = i / a.half, j = i - tok * a.half;
+    const int tok = a.by_half.of(i), j = i - tok * a.half;
     const double pos = a.wide ? (double)static_cast<const int64_t*>(a.positions)[t0 + tok]
                               : (double)static_cast<const int32_t*>(a.positions)[t0 + tok];
     const Turn t = turn_of(pos, a.freqs[j] * QUARTERS);
@@ -46,9 +47,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     sn[i] = t.sin * a.magnitude;
   }
   __syncthreads();
-  const int per_head = units_of(a.d, a.half), per_token = per_head * a.heads;
+  const int per_head = a.by_head.d, per_token = a.by_token.d;
   for (int i = threadIdx.x; i < n * per_token; i += 256) {
-    const int tok = i / per_token, at = i - tok * per_token, head = at / per_head;
+    const int tok = a.by_token.of(i), at = i - tok * per_token, head = a.by_head.of(at);
     const Unit u = unit_of<INTER>(at - head * per_head, a.d, a.half);
     const int64_t from = (t0 + tok) * a.xt + head * a.xh, to = ((t0 + tok) * a.heads + head) * a.d;
     float p[8], q[8];
@@ -73,6 +74,7 @@ template <int DT>
 int rotary_go(RotaryArgs a, bool interleaved, hipStream_t st) {
   const int most = a.half ? std::max(1, 256 / a.half) : 16;
   a.tokens = (int)std::min<int64_t>(most, std::max<int64_t>(1, a.T / (4 * device_cus())));
+  a.by_head = Divisor(units_of(a.d, a.half)), a.by_token = Divisor((int64_t)units_of(a.d, a.half) * a.heads), a.by_half = Divisor(std::max(1, a.half));
   const int64_t grid = cdiv(a.T, a.tokens), step = MAX_LAUNCH_THREADS / 256;
   const int64_t esz = DT == XDNA_F32 ? 4 : 2;
   for (int64_t b = 0; b < grid; b += step) {
@@ -95,7 +97,7 @@ struct NormArgs {
   const void *o, *gate, *post, *weight;
   int64_t x0, x1, o0, o1, g0, g1, inner;      // where row r starts: r / inner and r % inner times these
   int wdt, pdt;               // types of weight and post
-  int64_t rows;
+  int64_t row0, rows;         // rows of this launch: row0 .., up to the last
   int width;
   float scale, eps;
   void *sum, *y;
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void norm_kernel(NormArgs a) {
   constexpr int THREADS = L > 256 ? L : 256, ROWS = THREADS / L;
   __shared__ float part[THREADS / 64];
   const int lane = threadIdx.x % L;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / L, r = min(row, a.rows - 1);
+  const int64_t row = a.row0 + (int64_t)blockIdx.x * ROWS + threadIdx.x / L, r = min(row, a.rows - 1);
   const int64_t ro = r / a.inner, ri = r - ro * a.inner, xr = ro * a.x0 + ri * a.x1, orow = ro * a.o0 + ri * a.o1, gr = ro * a.g0 + ri * a.g1;
   float x[C][8];
   int n[C];
@@ -195,9 +197,11 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void norm_kernel(NormArgs a) {
 constexpr int64_t MAX_WIDTH = 1024 * 8 * 4;
 
 template <int DTX, int DTO, int L, int C>
-void norm_launch(const NormArgs& a, hipStream_t st) {
-  constexpr int THREADS = L > 256 ? L : 256;
-  norm_kernel<DTX, DTO, L, C><<<(unsigned)cdiv(a.rows, THREADS / L), THREADS, 0, st>>>(a);
+void norm_launch(NormArgs a, hipStream_t st) {
+  constexpr int THREADS = L > 256 ? L : 256, ROWS = THREADS / L;
+  constexpr int64_t STEP = MAX_LAUNCH_THREADS / THREADS * ROWS;
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += STEP)
+    norm_kernel<DTX, DTO, L, C><<<(unsigned)cdiv(std::min(STEP, a.rows - a.row0), ROWS), THREADS, 0, st>>>(a);
 }
 
 template <int DTX, int DTO>
@@ -229,7 +233,7 @@ int xdna_rotary(const void* x, int dtype, int64_t x_token, int64_t x_head, const
   if (T == 0 || heads == 0 || d == 0) return XDNA_OK;
   XDNA_REQUIRE(x && positions && y && (freqs || half == 0), "null pointer");
   XDNA_REQUIRE(x_token >= 0 && x_head >= 0, "strides must not be negative");
-  RotaryArgs a{x, x_token, x_head, positions, wide, freqs, (int)half, (int)d, (int)heads, 0, T, magnitude, y};
+  RotaryArgs a{x, x_token, x_head, positions, wide, freqs, (int)half, (int)d, (int)heads, 0, {}, {}, {}, T, magnitude, y};
   if (dtype == XDNA_F32) return rotary_go<XDNA_F32>(a, interleaved, as_stream(stream));
   if (dtype == XDNA_BF16) return rotary_go<XDNA_BF16>(a, interleaved, as_stream(stream));
   return rotary_go<XDNA_F16>(a, interleaved, as_stream(stream));
@@ -241,13 +245,13 @@ int xdna_residual_norm(const void* x, int x_dtype, const void* o, int dtype, con
   XDNA_REQUIRE(is_float(x_dtype) && (x_dtype == dtype || x_dtype == XDNA_F32) && is_float(dtype),
                "dtype must be F32/BF16/F16, and x's the same or F32");
   XDNA_REQUIRE(is_float(post_dtype) && is_float(weight_dtype), "weights must be F32/BF16/F16");
-  XDNA_REQUIRE(rows >= 0 && width >= 0 && width <= MAX_WIDTH && rows <= MAX_LAUNCH_THREADS / 1024, "bad sizes (width: at most 32768)");
+  XDNA_REQUIRE(rows >= 0 && width >= 0 && width <= MAX_WIDTH && rows < (1ll << 40), "bad sizes (width: at most 32768)");
   if (rows == 0 || width == 0) return XDNA_OK;
   XDNA_REQUIRE(x && y && strides && (!o || sum) && (o || (!gate && !post)), "null pointer, or a gate or norm of nothing");
   XDNA_REQUIRE(inner >= 1, "inner must be at least 1");
   for (int i = 0; i < 6; ++i) XDNA_REQUIRE(strides[i] >= 0, "strides must not be negative");
   NormArgs a{x, o, gate, post, weight, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], inner, weight_dtype,
-             post_dtype, rows, (int)width, scale, eps, sum, y};
+             post_dtype, 0, rows, (int)width, scale, eps, sum, y};
   hipStream_t st = as_stream(stream);
   if (x_dtype == XDNA_F32) {
     if (dtype == XDNA_F32) return norm_go<XDNA_F32, XDNA_F32>(a, st);
