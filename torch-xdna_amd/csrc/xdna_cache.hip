@@ -182,9 +182,14 @@ __device__ __forceinline__ void store_bytes(int8_t* to, int n, const float (&x)[
   }
 }
 
-// A workgroup has a page of one head's keys (kind 0) or values (1), or some tokens of all heads' queries (2); kinds in turn, so that
-// those that compute more and those that read more share a CU. Texts whose open page holds old tokens: only their first page's workgroup reads the ring, and writes what would
-// fall on the old tokens' places after that. U: units of keys a thread has.
+// A workgroup has a page of one head's keys (kind 0) or values (1), or some tokens of all heads' queries (2); kinds in turn, so
+// that those that compute more and those that read more share a CU. Texts whose open page holds old tokens: only their first
+// page's workgroup reads the ring, and writes what would fall on the old tokens' places after that. U: units of keys a thread
+// has. One pass over the tokens: a page's values stay in registers (keys) or LDS (values, which turn there) until their maximum
+// is known. 16384 tokens, 16 / 8 heads of 128, with q: 235 MB, 44 us (5.3 TB/s; a large copy 4.8), vector units as busy as memory
+// (turns, roundings, bytes; with a division for each byte 55 us; four heads a workgroup, the angles theirs in common, 53:
+// fewer workgroups side by side). 48 new tokens 5.4 us: the launch and three round trips (lengths, tokens and frequencies,
+// stores).
 template <int DT, bool INTER, int U, int KINDS>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ float part[4];
@@ -464,8 +469,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 
 // A row's maxima follow once they are passed by more than 2^SLACK: nearly never after a row's first keys, where otherwise some
-// row of sixteen finds a larger one at nearly every step, and all of O is multiplied. O's weights are held 2^SHIFT times as large,
-// so that float16 takes them from 2^-22 of the maximum (normal) to 2^(SLACK + 1) times it.
+// row of sixteen finds a larger one at nearly every step, and all of O is multiplied. O's weights are held 2^SHIFT times as
+// large, so that float16 takes them from 2^-22 of the maximum (normal) to 2^(SLACK + 1) times it.
 constexpr float SLACK = 6.0f, SHIFT = 8.0f;
 template <int DT>
 constexpr uint32_t ALL_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
@@ -530,6 +535,12 @@ struct Rows {
 // step is a copy of the loop's body that loads nothing: past a branch around loads the compiler waits for all of them.
 // Heads are held as D dims, a multiple of 32; dims past a.d (D - 16 then) are copies of others, times zeros of q, and of no output.
 // EXACT: the heads have D dims.
+//
+// What bounds it: one new token a text, the stream of K and V (48 texts of 4096 .. 8192, 604 MB: 115 us, 5.2 TB/s; texts of one
+// length 5.9; a kernel that only reads reaches 6.3), the rest the unequal lengths. More rows, the vector units: a step of 48
+// rows and heads of 96 is about 1000 vector instructions, 240 of them the widening, and 72 MFMAs; 16 texts x 5 tokens x 7 heads
+// a kv head over 2500 .. 5000 keys 18 to 21 us, vector units 50%, waits 44% of the waves' time. Short texts, the chain of lengths,
+// pages, keys, and about 2000 instructions of one wave (4 x 330: 7.2 us).
 template <int DT, int D, int RB, int W, bool EXACT>
 __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   // a lane's bytes of K: 16 of each 64 dims, and 8 of the last 32
@@ -1070,7 +1081,7 @@ int cache_go(const CacheArgs& a, const CachePlan& p, hipStream_t st) {
   else cache_dims<DT, 128>(a, p, st);
   if (a.parts > 1) {
     const int64_t all = (int64_t)a.B * a.N * a.nh;
-    // a wave a row for few parts, which many rows have (2240 rows of 4 parts 4.0 us; four waves a row and sixteen loads 8)
+    // a wave a row for few parts, which many rows have (2240 rows of 4 parts 4.0 us, about 2 less than with sixteen loads a wave)
     if (a.parts <= 4) cache_join_kernel<DT, 1, 4><<<(unsigned)cdiv(all, 4), 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
     else if (a.parts <= 16) cache_join_kernel<DT, 4, 4><<<(unsigned)all, 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
     else cache_join_kernel<DT, 4, 16><<<(unsigned)all, 256, 0, st>>>(a.po, a.pml, a.parts, all, a.d, a.out);
