@@ -364,6 +364,49 @@ def test_attention_strides_streams_and_graphs(gpu):
         n += 1
 
 
+@pytest.mark.parametrize("b,n,group,kv,dim,page,longest", [(1, 30, 4, 2, 64, 64, 3000), (1, 150, 3, 1, 128, 32, 700), (2, 40, 1, 3, 96, 16, 5000),
+                                                           (3000, 1, 2, 1, 32, 16, 40), (300, 2, 3, 4, 128, 64, 300), (40, 1, 4, 8, 128, 64, 5000)])
+def test_attention_blocks_and_parts(gpu, b, n, group, kv, dim, page, longest):
+    """Several blocks of rows, parts of keys, both, and as many texts as make four waves a workgroup: some rows of each."""
+    g = torch.Generator().manual_seed(b + n)
+    lens = torch.randint(0, longest + 1, (b,), generator=g).tolist()
+    cache = random_cache(b, kv, dim, longest, page, "bf16", seed=n, dev=gpu)
+    q = _query(b, n, kv * group, dim, "bf16", gpu)
+    o = lm.attention_cache(q, cache, _lens(lens, gpu))
+    some = list(range(b))[::max(1, b // 7)]
+    part = cache._replace(ktail=cache.ktail[some], vtail=cache.vtail[some], table=cache.table[some])
+    _within(o[some], *cache_reference(q[some], part, [lens[i] for i in some]))
+    # every text alone, split another way: the same up to the order of sums
+    if b <= 300:
+        for i in some:
+            one = cache._replace(ktail=cache.ktail[i:i + 1], vtail=cache.vtail[i:i + 1], table=cache.table[i:i + 1])
+            torch.testing.assert_close(lm.attention_cache(q[i:i + 1], one, _lens(lens[i:i + 1], gpu)), o[i:i + 1], rtol=2 ** -6, atol=2 ** -6)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_steps(gpu, seed):
+    """Texts of any lengths get a few tokens each, then all of them attend: the cache's own contents in float64 beside it."""
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda *v: v[int(torch.randint(0, len(v), (1,), generator=g))]  # noqa: E731
+    page, kv, dim, group, dtype = pick(16, 32, 64, 128), pick(1, 2, 3, 8), pick(16, 32, 48, 64, 80, 96, 112, 128), pick(1, 2, 5, 8, 16, 17), pick("bf16", "f16")
+    b, n = pick(1, 2, 5, 9), pick(1, 1, 2, 3, 7)
+    old = [int(v) for v in torch.randint(0, pick(3 * page, 900, 2500), (b,), generator=g)]
+    cache = random_cache(b, kv, dim, max(old) + n, page, dtype, places=page * pick(1, 2, 3), seed=seed, dev=gpu)
+    q, k, v = tokens(b * n, kv * group, kv, dim, dtype, seed=seed, dev=gpu)
+    freqs, magnitude = lm.rotary_freqs(dim // 2 // 2 * 2, factor=pick(1.0, 4.0), original=2048, device=gpu)
+    inter = pick(False, True)
+    turned = lm.cache_append(cache, _lens(old, gpu), k, v, None, q, freqs, magnitude, inter)
+    pos = torch.cat([torch.arange(o, o + n) for o in old])
+    _within(turned, *rotary_reference(q, pos, freqs, magnitude, inter))
+    want = rotary_reference(k, pos, freqs, magnitude, inter)
+    ring = torch.cat([cache.ktail[i][:, torch.arange(o, o + n) % cache.ktail.shape[2]].transpose(0, 1) for i, o in enumerate(old)])
+    if n <= cache.ktail.shape[2]:
+        _within(ring, *want)
+    lens = [o + n for o in old]
+    o = lm.attention_cache(turned.view(b, n, kv * group, dim), cache, _lens(lens, gpu))
+    _within(o, *cache_reference(turned.view(b, n, kv * group, dim), cache, lens))
+
+
 def test_far_pages(gpu):
     """Pages past 2^32 bytes of the pool are written and read where they lie."""
     page, kv, dim = 64, 8, 128

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     return;
   }
   // values: through LDS, [token][d + 2] so that a walk along the tokens of 16 dims meets every bank
-  extern __shared__ uint16_t vl[];
+  extern __shared__ __attribute__((aligned(16))) uint16_t vl[];
   const int per_token = a.by_value.d, units = g * per_token, ld = a.d + 2;
   const int64_t head = (int64_t)b * a.nkv + kvh, block = (int64_t)id * a.nkv + kvh;
   const auto value = [&](int pos, int u, float (&p)[8]) {
