@@ -540,13 +540,15 @@ struct Rows {
 // length 5.9; a kernel that only reads reaches 6.3), the rest the unequal lengths. More rows, the vector units: a step of 48
 // rows and heads of 96 is about 1000 vector instructions, 240 of them the widening, and 72 MFMAs; 16 texts x 5 tokens x 7 heads
 // a kv head over 2500 .. 5000 keys 18 to 21 us, vector units 50%, waits 44% of the waves' time. Short texts, the chain of lengths,
-// pages, keys, and about 2000 instructions of one wave (4 x 330: 7.2 us).
+// pages, keys, and about 2000 instructions of one wave (4 x 330: 6.8 us).
 template <int DT, int D, int RB, int W, bool EXACT>
 __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   // a lane's bytes of K: 16 of each 64 dims, and 8 of the last 32
   constexpr int S = D / 32, ND = D / 16, DC = D / 64, REST = S - 2 * DC;
+  // blocks of rows that the waves join at once: all, where two workgroups' LDS has room for them
+  constexpr int JB = RB * ND <= 16 ? RB : 1;
   constexpr bool QLDS = RB > 1;                 // more rows: q in LDS, registers for O
-  __shared__ __attribute__((aligned(16))) float ol[W / 2][RB * ND][256];
+  __shared__ __attribute__((aligned(16))) float ol[W][JB * ND][256];
   __shared__ float ml[2][W][RB][16];
   __shared__ i32x4 ql[QLDS ? RB * S : 1][64];
   __shared__ float qls[QLDS ? RB : 1][16];
@@ -900,53 +902,36 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
     }
   }
 
-  // The waves' rows joined: the second half's into the first half's, then those by all waves.
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) w.l[rb] = quad_sum(w.l[rb]);
-  const auto leave = [&](int at) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      if (h == 0) ml[0][wave][rb][i16] = w.m[rb], ml[1][wave][rb][i16] = w.l[rb];
-#pragma unroll
-      for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4*>(&ol[at][rb * ND + i][lane * 4]) = w.o[rb][i];
-    }
-  };
+  // The waves' rows joined, JB blocks of them at a time: all waves' at once; halves in turn took 0.4 us
+  // more (4 x 330).
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const float unit = w.mo[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.mo[rb] - SHIFT - w.m[rb]);       // O in p's
-#pragma unroll
-    for (int i = 0; i < ND; ++i) w.o[rb][i] *= unit;
+    const float l = quad_sum(w.l[rb]);
+    if (h == 0) ml[0][wave][rb][i16] = w.m[rb], ml[1][wave][rb][i16] = l;
   }
-  if (wave >= W / 2) leave(wave - W / 2);
-  __syncthreads();
-  if (wave < W / 2) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float m1 = ml[0][wave + W / 2][rb][i16], l1 = ml[1][wave + W / 2][rb][i16], mt = fmaxf(w.m[rb], m1);
-      const float w0 = w.m[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m[rb] - mt);
-      const float w1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - mt);
-      w.l[rb] = (w.m[rb] == -INFINITY ? w.l[rb] : w.l[rb] * w0) + (m1 == -INFINITY ? l1 : l1 * w1);     // 0 or NaN where there is no maximum
-      w.m[rb] = mt;
+  for (int rb = 0; rb < RB; ++rb) {
+    if (rb % JB == 0) {
+      if (rb > 0) __syncthreads();                   // those before are read
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(&ol[wave][rb * ND + i][lane * 4]);
+      for (int j = 0; j < JB; ++j) {
+        const float unit = w.mo[rb + j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.mo[rb + j] - SHIFT - w.m[rb + j]);     // O in p's
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w.o[rb][i][r] = w.o[rb][i][r] * w0 + x[r] * w1;
+        for (int i = 0; i < ND; ++i) {
+          const f32x4 o = w.o[rb + j][i] * unit;
+          *reinterpret_cast<f32x4*>(&ol[wave][j * ND + i][lane * 4]) = o;
+        }
       }
+      __syncthreads();
     }
-    leave(wave);                     // where its partner's were, which no other wave reads
-  }
-  __syncthreads();
+    float mt = -INFINITY, lt = 0.0f, weight[W];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    float mt = -INFINITY, lt = 0.0f, weight[W / 2];
+    for (int x = 0; x < W; ++x) mt = fmaxf(mt, ml[0][x][rb][i16]);
 #pragma unroll
-    for (int x = 0; x < W / 2; ++x) mt = fmaxf(mt, ml[0][x][rb][i16]);
-#pragma unroll
-    for (int x = 0; x < W / 2; ++x) {
+    for (int x = 0; x < W; ++x) {
       const float mg = ml[0][x][rb][i16], lg = ml[1][x][rb][i16];
-      weight[x] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mg - mt);
-      lt += mg == -INFINITY ? lg : lg * weight[x];
+      weight[x] = mg == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mg - mt);     // a wave without keys: nothing
+      lt += mg == -INFINITY ? lg : lg * weight[x];           // lg is 0 then, or NaN
     }
     const bool mine = row0 + 16 * rb + i16 < nrows;
     int token, qhead;
@@ -958,8 +943,8 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
       if (i >= dchunks) break;
       f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int x = 0; x < W / 2; ++x) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(&ol[x][rb * ND + i][lane * 4]);
+      for (int x = 0; x < W; ++x) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(&ol[x][(rb % JB) * ND + i][lane * 4]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] += y[r] * weight[x];
       }
@@ -1037,9 +1022,10 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const float* __restrict
 // workgroup share the widening of K and V. Up to a workgroup a CU, eight waves share out the keys, and a text's keys go to as
 // many parts as fill the CUs, none under 512 keys; with more of them four waves do, two workgroups side by side on a CU, and
 // parts are for balance, none under 2048 keys. A part is its share of the keys that there are; the host knows only how long
-// texts can be. Measured, eight waves / four (texts x longest, 16 / 8 heads of 128): 4 x 330 7.3 / 8.3 us, 20 x 600 9.2 / 9.9, 24 x 2000
-// 19.8 / 20.8, 8 x 32768 80.7 / 82.8, 48 x 1000 23.1 / 19.5, 64 x 600 20.6 / 16.9, 48 x 8192 116.5 / 114.4 (one part 137, two
-// 119, four 115, five 114); 1 x 131000 on 4 kv heads: 64 parts 16.6, 128 19.9.
+// texts can be. Measured, eight waves / four (texts x longest, 16 / 8 heads of 128): 4 x 330 6.8 / 8.2 us, 20 x 600 9.0 / 9.7, 24 x 2000
+// 19.5 / 19.7, 8 x 32768 80.7 / 83.2, 48 x 1000 22.2 / 19.3, 64 x 600 19.8 / 16.5, 48 x 8192 125 / 116 (one part 133, two
+// 118, four 115.5, five 114); 1 x 131000 on 4 kv heads: 64 parts 16.7, 128 19.5. Keys of a part side by side and not spread over
+// the text: 8 x 32768 80.7 against 84.
 struct CachePlan {
   int blocks, rblocks, parts;
   bool eight;
