@@ -539,7 +539,7 @@ struct Rows {
 // What bounds it: one new token a text, the stream of K and V (48 texts of 4096 .. 8192, 604 MB: 115 us, 5.2 TB/s; texts of one
 // length 5.9; a kernel that only reads reaches 6.3), the rest the unequal lengths. More rows, the vector units: a step of 48
 // rows and heads of 96 is about 1000 vector instructions, 240 of them the widening, and 72 MFMAs; 16 texts x 5 tokens x 7 heads
-// a kv head over 2500 .. 5000 keys 18 to 21 us, vector units 50%, waits 44% of the waves' time. Short texts, the chain of lengths,
+// a kv head over 2500 .. 5000 keys 18 to 21 us, vector units 48%, waits 45% of the waves' time. Short texts, the chain of lengths,
 // pages, keys, and about 2000 instructions of one wave (4 x 330: 6.8 us).
 template <int DT, int D, int RB, int W, bool EXACT>
 __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
