@@ -533,7 +533,8 @@ struct Rows {
 // W waves share out the 64-key steps of a part of a text's keys for 16 RB rows and meet in LDS. Registers hold the step in
 // work and nothing else: K of the wave's next step is on its way once its scores are done, V after its products. The last
 // step is a copy of the loop's body that loads nothing: past a branch around loads the compiler waits for all of them.
-// Heads are held as D dims, a multiple of 32; dims past a.d (D - 16 then) are copies of others, times zeros of q, and of no output.
+// Heads are held as D dims, a multiple of 32; dims past a.d (D - 16 then) are copies of others (int8, finite; in the open page, where
+// keys may not be, zeros), times zeros of q, and of no output.
 // EXACT: the heads have D dims.
 //
 // What bounds it: one new token a text, the stream of K and V (48 texts of 4096 .. 8192, 604 MB: 115 us, 5.2 TB/s; texts of one
@@ -796,7 +797,13 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const int dim = s < 2 * DC ? 16 * min(h + 4 * (s >> 1), dchunks - 1) + 8 * (s & 1) : 64 * DC + 8 * (64 * DC + 8 * h < d ? h : h & 1);
-          const i32x4 f = *reinterpret_cast<const i32x4*>(kt + (min(16 * hk + 4 * t + (lane & 3), left - 1) * d + dim));
+          i32x4 f = *reinterpret_cast<const i32x4*>(kt + (min(16 * hk + 4 * t + (lane & 3), left - 1) * d + dim));
+          // dims that the heads do not have: q is 0 there, which times an infinity of the dim read instead would be NaN
+          if constexpr (!EXACT) {
+            const int keep = (s < 2 * DC ? 16 * (h + 4 * (s >> 1)) : 64 * DC + 8 * h) < d ? -1 : 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] &= keep;
+          }
           sc[rb][t] = mfma16<DT>(f, q[s], sc[rb][t]);
         }
       if (RB > 1) asm volatile("" ::: "memory");
