@@ -12,3 +12,12 @@ pytestmark = pytest.mark.gpu
 def test_infinite_keys(gpu, dim, dtype):
     """Head dims that the kernels hold as they are, and those that they fill up to the next multiple of 32."""
     host.infinite_keys(gpu, dim, dtype)
+
+
+@pytest.mark.parametrize("dtype,power", host.LARGE)
+@pytest.mark.parametrize("dim,n,group,page,length,scale", [
+    (32, 2, 2, 16, 45, 0.125), (64, 1, 1, 64, 300, -0.3), (128, 1, 8, 32, 70, 0.17), (96, 5, 7, 32, 1500, 0.11), (48, 3, 6, 128, 5000, 0.125),
+    (128, 2, 16, 16, 40, -0.09), (64, 1, 4, 128, 60, 0.2)])
+def test_large_scores(gpu, dtype, power, dim, n, group, page, length, scale):
+    """In one page, over the waves of a workgroup, over parts, in the open page alone."""
+    host.large_scores(gpu, dtype, dim, n, group, page, length, power, scale)

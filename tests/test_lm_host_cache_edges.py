@@ -55,3 +55,60 @@ def infinite_keys(dev, dim, dtype, page=32):
 @pytest.mark.parametrize("dim", [16, 80, 128])
 def test_infinite_keys(dim, dtype):
     infinite_keys("cpu", dim, dtype)
+
+
+# ------------------------------------------------------------------------------ large scores
+def large_scores(dev, dtype, dim, n, group, page, length, power, scale):
+    """Scores up to where float32 has no fraction, and differences that are all or nothing: a row's output is the value of its best
+    key, or the mean of two that are as good, in pages whose scales differ and in the open page."""
+    dt, g = DTYPES[dtype], torch.Generator().manual_seed(page + length)
+    kv = 2
+    cache = random_cache(1, kv, dim, length, page, dtype, seed=length, dev="cpu")
+    whole, places = length // page, cache.ktail.shape[2]
+    at = torch.arange(whole * page, length)
+    sign = -1.0 if scale < 0 else 1.0
+    for c in range(kv):
+        best = torch.randint(0, length - n, (2,), generator=g).tolist()      # every row sees them
+        value = torch.randint(-100, 60, (length,), generator=g).double()     # of all of a key's dims: its score's sign and size
+        value[best] = 64.0
+        if c == 1:
+            value[best[1]] = -100.0
+        value *= sign
+        for j in range(whole):
+            e, ids = j % 3, int(cache.table[0, j])                            # the page's scale: value = int8 * 2^e
+            part = value[j * page:(j + 1) * page]
+            part = torch.where(part.abs() == 64, part, torch.trunc(part / 2 ** e) * 2 ** e)
+            cache.kpages[ids, c] = (part / 2 ** e).to(torch.int8)[:, None]
+            cache.kscales[ids, c] = 2.0 ** e * power[1]
+        cache.ktail[0, c][at % places] = (value[at] * power[1]).to(dt)[:, None]
+        best = [b for b in best if value[b] == 64.0 * sign]
+        v = []
+        for b in best:
+            if b < whole * page:
+                i = int(cache.table[0, b // page])
+                v.append(cache.vpages[i, c, :, b % page].double() * cache.vscales[i, c].double())
+            else:
+                v.append(cache.vtail[0, c][:, b % places].double())
+        if c == 0:
+            want = [torch.stack(v)]
+        else:
+            want.append(torch.stack(v))
+    cache = lm.Cache8(*(t.to(dev) for t in cache))
+    q = torch.full((1, n, kv * group, dim), power[0], dtype=dt, device=dev)
+    o = lm.attention_cache(q, cache, _i32([length], dev), scale)
+    for c in range(kv):
+        mean, size = want[c].mean(0), want[c].abs().mean(0)
+        # the weights (1 or 1/2, times the values' scale) round to 16 bits, the result once; float32 in between
+        tol = torch.finfo(dt).eps / 2 * (mean.abs() * (1 + 2.0 ** -6) + size * (1 + 2.0 ** -6)) + 16 * 2.0 ** -24 * size + torch.finfo(dt).tiny
+        rows = o[0, :, c * group:(c + 1) * group].reshape(-1, dim)
+        within(rows, mean.expand_as(rows), tol.expand_as(rows))
+
+
+# (q's values, keys' unit): scores of about 64 x dim x their product x scale
+LARGE = [("f16", (2.0 ** 13, 2.0 ** 8)), ("bf16", (2.0 ** 13, 2.0 ** 8)), ("bf16", (2.0 ** 40, 2.0 ** 30)), ("f16", (2.0 ** 8, 2.0 ** 5))]
+
+
+@pytest.mark.parametrize("dtype,power", LARGE)
+@pytest.mark.parametrize("page,length,scale", [(16, 45, 0.125), (64, 300, -0.3), (32, 70, 0.17)])
+def test_large_scores(dtype, power, page, length, scale):
+    large_scores("cpu", dtype, 32, 2, 2, page, length, power, scale)

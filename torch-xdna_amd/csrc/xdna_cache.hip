@@ -472,6 +472,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 // row of sixteen finds a larger one at nearly every step, and all of O is multiplied. O's weights are held 2^SHIFT times as
 // large, so that float16 takes them from 2^-22 of the maximum (normal) to 2^(SLACK + 1) times it.
 constexpr float SLACK = 6.0f, SHIFT = 8.0f;
+// The maximum of no scores but -inf: below every other, and a number, so that differences from it are none either.
+constexpr float LOWEST = -3.40282347e+38f;
 template <int DT>
 constexpr uint32_t ALL_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
 
@@ -484,40 +486,49 @@ struct Rows {
   static constexpr int ND = D / 16;
   f32x4 o[RB][ND];
   float l[RB], m[RB];       // sum of p, 2^m its unit
-  float mo[RB];             // 2^(mo - SHIFT) is O's
+  float ko[RB];             // 2^(m + ko - SHIFT) is O's: beside a large m the sum would have no fraction
 
   // The weights of T tiles of 16 keys as the second product's operand, 2^(c score) f 2^k in O's unit; c with K's scale, k and f
   // the lane's. same: k is that of all 64 keys.
   template <int DT, int T>
-  __device__ __forceinline__ void weigh(const f32x4* sc, int rb, float c, float k, float f, bool same, int* pf) {
+  __device__ __forceinline__ void weigh(f32x4* sc, int rb, float c, float k, float f, bool same, int* pf) {
     float top = sc[0][0];
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = __builtin_elementwise_maximum(top, sc[t][r]);
     top *= c;
-    const float mx = quad_max(top), mxo = same ? mx + k : quad_max(top + k);
-    const bool grow = mx > m[rb] + SLACK, growo = mxo > mo[rb] + SLACK;
-    if (__builtin_amdgcn_ballot_w64(grow || growo)) {
-      if (grow) {
-        l[rb] *= __builtin_amdgcn_exp2f(m[rb] - mx);                             // from -inf: 0
-        m[rb] = mx;
-      }
-      const float alpha = growo ? __builtin_amdgcn_exp2f(mo[rb] - mxo) : 1.0f;
+    const float mx = quad_max(top), rise = mx - m[rb], riseo = same ? rise + k : quad_max(top - m[rb] + k);
+    const bool grow = rise > SLACK;
+    if (__builtin_amdgcn_ballot_w64(grow || riseo - SLACK > ko[rb])) {
+      const float mn = grow ? mx : m[rb], kn = ko[rb] + (m[rb] - mn), kx = same ? mx - mn + k : quad_max(top - mn + k);
+      l[rb] *= __builtin_amdgcn_exp2f(m[rb] - mn);                               // from LOWEST: 0
+      m[rb] = mn;
+      const bool growo = kx - SLACK > kn;
+      const float alpha = growo ? __builtin_amdgcn_exp2f(kn - kx) : 1.0f;
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[rb][i] *= alpha;
-      mo[rb] = growo ? mxo : mo[rb];
+      ko[rb] = growo ? kx : kn;
     }
-    const float m0 = m[rb] == -INFINITY ? 0.0f : m[rb], mo0 = mo[rb] == -INFINITY ? 0.0f : mo[rb];       // only -inf scores so far: p = 0
-    const float shift = k + SHIFT - mo0, back = -(shift + m0);                   // of the weights, and from there to p
-    const bool far = __builtin_amdgcn_ballot_w64(back > 64.0f) != 0;             // too far for the weights to tell p
+    const float out = k + SHIFT - ko[rb];                                        // from p to the weights
+    float m0 = m[rb], shift = out - m0;
+    // A maximum past 2^20 is rounded by a 16th and more, past 2^28 by more than float16's range, and the products that fma takes
+    // are not. There the scores are rounded first, as the maximum was, and the maximum goes off them: the largest is 0.
+    if (__builtin_amdgcn_ballot_w64(fabsf(m0) > 0x1p20f)) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[t][r] = sc[t][r] * c - m0;
+      c = 1.0f, m0 = 0.0f, shift = out;
+    }
+    const bool far = __builtin_amdgcn_ballot_w64(out < -64.0f) != 0;             // too far for the weights to tell p
     if (far) {
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) l[rb] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -m0));
     }
-    const float scale = far ? 0.0f : __builtin_amdgcn_exp2f(back);
+    const float scale = far ? 0.0f : __builtin_amdgcn_exp2f(-out);
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -570,8 +581,8 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   Rows<D, RB> w;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    w.m[rb] = w.mo[rb] = -INFINITY;
-    w.l[rb] = 0.0f;
+    w.m[rb] = LOWEST;
+    w.l[rb] = w.ko[rb] = 0.0f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) w.o[rb][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -914,7 +925,7 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const float l = quad_sum(w.l[rb]);
-    if (h == 0) ml[0][wave][rb][i16] = w.m[rb], ml[1][wave][rb][i16] = l;
+    if (h == 0) ml[0][wave][rb][i16] = w.m[rb] == LOWEST ? -INFINITY : w.m[rb], ml[1][wave][rb][i16] = l;
   }
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -922,7 +933,7 @@ __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
       if (rb > 0) __syncthreads();                   // those before are read
 #pragma unroll
       for (int j = 0; j < JB; ++j) {
-        const float unit = w.mo[rb + j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.mo[rb + j] - SHIFT - w.m[rb + j]);     // O in p's
+        const float unit = __builtin_amdgcn_exp2f(w.ko[rb + j] - SHIFT);               // O in p's
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
           const f32x4 o = w.o[rb + j][i] * unit;
