@@ -21,3 +21,7 @@ def test_infinite_keys(gpu, dim, dtype):
 def test_large_scores(gpu, dtype, power, dim, n, group, page, length, scale):
     """In one page, over the waves of a workgroup, over parts, in the open page alone."""
     host.large_scores(gpu, dtype, dim, n, group, page, length, power, scale)
+
+
+def test_permuted(gpu):
+    host.permuted(gpu)

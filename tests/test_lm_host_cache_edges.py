@@ -112,3 +112,26 @@ LARGE = [("f16", (2.0 ** 13, 2.0 ** 8)), ("bf16", (2.0 ** 13, 2.0 ** 8)), ("bf16
 @pytest.mark.parametrize("page,length,scale", [(16, 45, 0.125), (64, 300, -0.3), (32, 70, 0.17)])
 def test_large_scores(dtype, power, page, length, scale):
     large_scores("cpu", dtype, 32, 2, 2, page, length, power, scale)
+
+
+# ------------------------------------------------------------------------------ permuted inputs
+def permuted(dev):
+    """Results are contiguous, as their shape functions say, whatever the inputs' strides; in a compiled function too."""
+    g = torch.Generator().manual_seed(0)
+    x, o, gate = (torch.randn(4, 3, 16, generator=g).to(dev).transpose(0, 1) for _ in range(3))
+    for args in ((x, o), (x, o, None, None, gate), (x.bfloat16(), o.bfloat16()), (x, o.half(), None, x[0, 0].contiguous()), (x,)):
+        got = torch.ops.xdna.residual_norm(*args)
+        want = torch.ops.xdna.residual_norm(*(None if t is None else t.contiguous() for t in args))
+        for a, b in zip(got, want):
+            assert a.is_contiguous() and torch.equal(a, b)
+        if len(args) > 1:
+            assert all(t.is_contiguous() for t in lm.residual_norm(*args))
+    backend = "inductor" if dev != "cpu" else "aot_eager"
+    with torch.no_grad():
+        both = torch.compile(lambda a, b: [t + 1 for t in torch.ops.xdna.residual_norm(a, b)], fullgraph=True, backend=backend)(x, o)
+        for a, b in zip(both, torch.ops.xdna.residual_norm(x, o)):
+            assert torch.equal(a, b + 1) and a.stride() == b.stride()
+
+
+def test_permuted():
+    permuted("cpu")

@@ -342,8 +342,8 @@ def residual_norm(x, o=None, weight=None, post=None, gate=None, scale=1.0, eps=1
     n = post * o / sqrt(mean(o^2) + eps) (o itself if post is None), s = x + scale * gate * n (gate 1 if None),
     y = weight * s / sqrt(mean(s^2) + eps) (weight 1 if None), y from s before it is rounded. In float32, each
     rounded once: s to x's type, y to o's. x is of o's type or float32 (float32, bfloat16 or float16); weight and post [W] of any
-    of them, gate of o's type, [W] or of x's shape (any strides: one that a sequence's tokens share can be expanded). o None:
-    (x, y), y of x's type. W at most 32768."""
+    of them, gate of o's type, [W] or of x's shape (any strides: one that a sequence's tokens share can be expanded). Results
+    are contiguous; o None: (x, y), y of x's type. W at most 32768."""
     if x.is_cuda:
         s, y = _on_gpu("residual_norm", x, o, weight, post, gate, scale, eps)
         return (x if o is None else s), y
@@ -376,9 +376,9 @@ def residual_norm(x, o=None, weight=None, post=None, gate=None, scale=1.0, eps=1
             n = n / torch.sqrt(n.square().mean(-1, keepdim=True) + eps) * post.float()
         s = s + scale * (n if gate is None else n * gate.float())
     y = s / torch.sqrt(s.square().mean(-1, keepdim=True) + eps)
-    y = (y if weight is None else y * weight.float()).to(x.dtype if o is None else o.dtype)
+    y = (y if weight is None else y * weight.float()).to(x.dtype if o is None else o.dtype).contiguous()
     stats.record("cpu", t0, 0)
-    return (x if o is None else s.to(x.dtype)), y
+    return (x if o is None else s.to(x.dtype).contiguous()), y
 
 
 # ------------------------------------------------------------------------------ a paged cache in 8 bits
