@@ -20,7 +20,9 @@ from .continuations import Decoder
 
 
 class Texts:
-    """The caches of `batch` texts in all layers: a Cache8 a layer over one table, and the texts' lengths."""
+    """The caches of `batch` texts in all layers: a Cache8 a layer over one table, and the texts' lengths. A row of the batch has a
+    text from the time that it has pages until they are given back; the tokens that a step has for the other rows go nowhere, and
+    its logits for those mean nothing."""
 
     def __init__(self, model, batch, capacity, page=64, pages=None, device=None):
         layer = model.layers[0]
@@ -34,6 +36,7 @@ class Texts:
         self.free = list(range(pages))
         self.given = [[] for _ in range(batch)]
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.live = torch.zeros(batch, dtype=torch.int32, device=device)       # 1: a text's row
 
     def reserve(self, text, tokens):
         """Pages for the first `tokens` tokens of a text."""
@@ -46,13 +49,14 @@ class Texts:
             at = len(self.given[text])
             self.layers[0].table[text, at:at + missing] = torch.tensor(new, dtype=torch.int32).to(self.lens.device)
             self.given[text] += new
+            self.live[text] = 1
 
     def release(self, text):
         """A text that has ended gives its pages back, and its place can have a new one."""
         self.free += self.given[text]
         self.given[text] = []
         self.layers[0].table[text] = -1
-        self.lens[text] = 0
+        self.lens[text] = self.live[text] = 0
 
 
 class Server(Decoder):
@@ -98,7 +102,7 @@ class Server(Decoder):
             qk, v = self.heads(layer, y)
             q = lm.cache_append(cache, texts.lens, qk[:, layer.heads:], v, None, qk[:, :layer.heads], self.freqs)
             x, y = self.finish(layer, x, lm.attention_cache(q.view(b, n, layer.heads, self.dim), cache, seen).flatten(0, 1))
-        texts.lens += n
+        texts.lens.add_(texts.live, alpha=n)
         return self.head(y).view(b, n, -1)
 
 
