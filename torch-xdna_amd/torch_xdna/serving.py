@@ -22,7 +22,8 @@ from .continuations import Decoder
 class Texts:
     """The caches of `batch` texts in all layers: a Cache8 a layer over one table, and the texts' lengths. A row of the batch has a
     text from the time that it has pages until they are given back; the tokens that a step has for the other rows go nowhere, and
-    its logits for those mean nothing."""
+    its logits for those mean nothing. What a text holds is counted on the host too, so that nothing grows past its pages: a program
+    that replays a captured step gives the pages out before (reserve), and counts each replay but the first (grow)."""
 
     def __init__(self, model, batch, capacity, page=64, pages=None, device=None):
         layer = model.layers[0]
@@ -35,6 +36,7 @@ class Texts:
         self.page, self.columns = page, columns
         self.free = list(range(pages))
         self.given = [[] for _ in range(batch)]
+        self.held = [0] * batch
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.live = torch.zeros(batch, dtype=torch.int32, device=device)       # 1: a text's row
 
@@ -51,10 +53,24 @@ class Texts:
             self.given[text] += new
             self.live[text] = 1
 
+    def grow(self, new):
+        """Counts new[i] more tokens of each text i, and gives out the pages that they need; without room for all, it raises and
+        nothing changes."""
+        held = [h + n for h, n in zip(self.held, new)]
+        missing = sum(max(0, -(-h // self.page) - len(g)) for h, n, g in zip(held, new, self.given) if n)
+        if max(held, default=0) > self.columns * self.page or missing > len(self.free):
+            raise ValueError(f"no room for texts of {held} tokens: {missing} pages are missing and {len(self.free)} free, of "
+                             f"{self.columns} a text")
+        for text, n in enumerate(new):
+            if n:
+                self.reserve(text, held[text])
+        self.held = held
+
     def release(self, text):
         """A text that has ended gives its pages back, and its place can have a new one."""
         self.free += self.given[text]
         self.given[text] = []
+        self.held[text] = 0
         self.layers[0].table[text] = -1
         self.lens[text] = self.live[text] = 0
 
@@ -78,7 +94,15 @@ class Server(Decoder):
         return lm.residual_norm(x, layer.down((F.silu(g.float()) * u.float()).to(x.dtype)))
 
     def start(self, texts, tokens, starts):
-        """Logits of every token [T] of the packed prompts, whose keys and values go into the texts' empty caches."""
+        """Logits of every token [T] of the packed prompts, whose keys and values go into the texts' empty caches. A text without a
+        prompt (two equal starts) stays as it is."""
+        first = starts.tolist()
+        new = [b - a for a, b in zip(first, first[1:])]
+        if len(new) != len(texts.held) or min(new, default=0) < 0 or first[0] < 0 or first[-1] > tokens.shape[0]:
+            raise ValueError(f"starts must be [{len(texts.held) + 1}], ascending, within the {tokens.shape[0]} tokens")
+        if any(n and h for n, h in zip(new, texts.held)):
+            raise ValueError("a prompt is for a text that holds nothing: release it first")
+        texts.grow(new)
         at = torch.arange(tokens.shape[0], device=tokens.device)
         place = at - starts.long()[torch.searchsorted(starts.long(), at, right=True) - 1]
         x = self.embed[tokens.long()]
@@ -95,6 +119,9 @@ class Server(Decoder):
     def step(self, texts, tokens):
         """Logits [B, N, V] of N new tokens [B, N] of every text, which go into their caches."""
         b, n = tokens.shape
+        if b != len(texts.held):
+            raise ValueError(f"a step takes tokens [{len(texts.held)}, N], got {list(tokens.shape)}")
+        texts.grow([n if given else 0 for given in texts.given])
         x = self.embed[tokens.long().flatten()]
         _, y = lm.residual_norm(x)
         seen = texts.lens + n
