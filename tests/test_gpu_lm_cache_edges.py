@@ -1,8 +1,10 @@
 """attention_cache on the MI355X at values where a kernel can part from the definition: the functions of
 test_lm_host_cache_edges.py."""
 import pytest
+import torch
 
 import test_lm_host_cache_edges as host
+from torch_xdna import lm
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +27,22 @@ def test_large_scores(gpu, dtype, power, dim, n, group, page, length, scale):
 
 def test_permuted(gpu):
     host.permuted(gpu)
+
+
+def test_limits(gpu):
+    """Sizes past what the kernels' indexes reach are wrong arguments like others: refused as such, before anything is launched."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    cache = lm.cache8(1, 1, 1, 16, 16, 16, device=gpu)
+    q = torch.zeros(1, 1, 1, 16, dtype=torch.bfloat16, device=gpu)
+    k = torch.zeros(1, 1, 16, dtype=torch.bfloat16, device=gpu)
+    f = lm.rotary_freqs(16, device=gpu)[0]
+    for x in (q.expand(1, 1 << 23, 1, 16), q.expand(1, 1, 1 << 16, 16), q.expand(1, 1 << 12, 1 << 11, 16)):
+        with pytest.raises(ValueError):
+            lm.attention_cache(x, cache, i32(1))
+    far = cache._replace(table=cache.table[:, :1].expand(1, 1 << 26))
+    for call in (lambda: lm.attention_cache(q, far, i32(1)), lambda: lm.cache_append(far, i32(0), k, k),
+                 lambda: lm.cache_append(cache, i32(0), k, k, None, k.expand(1, 1 << 16, 16), f),
+                 lambda: lm.cache_append(cache, i32(0), k.expand(1 << 24, 1, 16), k.expand(1 << 24, 1, 16)),
+                 lambda: lm.rotary(torch.zeros(1, 1 << 20, 16, dtype=torch.bfloat16, device=gpu), i32(0), f)):
+        with pytest.raises(ValueError):
+            call()

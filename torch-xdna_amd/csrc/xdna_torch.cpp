@@ -68,6 +68,8 @@ void check_whole(const char* name, const Tensor& t, int64_t dims, const char* wh
 const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; }
 
 void done(int status, const char* what) {
+  // sizes past what the kernels' indexes reach: wrong arguments like those that are refused above
+  TORCH_CHECK_VALUE(status != XDNA_EINVAL, "xdna ", what, ": ", xdna_last_error());
   TORCH_CHECK(status == 0, "xdna ", what, " failed (status ", status, "): ", xdna_last_error());
 }
 
@@ -421,7 +423,7 @@ Tensor cache_append(const Tensor& k, const Tensor& v, const Tensor& kpages, cons
   if (freqs) check_freqs(*freqs, s.d);
   if (q) {
     TORCH_CHECK_VALUE(freqs, "cache_append: q turns with freqs, and there are none");
-    TORCH_CHECK_VALUE(q->dim() == 3 && q->size(1) >= 1, "q must be [T, H, D], got ", q->sizes());
+    TORCH_CHECK_VALUE(q->dim() == 3 && q->size(1) >= 1 && q->size(1) < 65536, "q must be [T, H, D], H at most 65535, got ", q->sizes());
     check_shape("q", *q, {t, q->size(1), s.d});
   }
   check_device(k, v), check_device(k, starts), check_device(k, q), check_device(k, freqs);
@@ -452,7 +454,8 @@ Tensor attention_cache(const Tensor& q, const Tensor& kpages, const Tensor& vpag
   TORCH_CHECK_VALUE(q.dim() == 4, "attention_cache takes q [B, N, H, D], got ", q.sizes());
   const int64_t n = q.size(1), h = q.size(2);
   check_shape("q", q, {s.b, n, h, s.d});
-  TORCH_CHECK_VALUE(h && h % s.kv == 0, "attention_cache: ", h, " q heads do not share ", s.kv, " key heads evenly");
+  TORCH_CHECK_VALUE(h && h < 65536 && h % s.kv == 0, "attention_cache: ", h, " q heads, at most 65535, do not share ", s.kv,
+                    " key heads evenly");
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)s.d);
   const Launch go(q);
   Tensor out = at::empty(q.sizes(), q.options());

@@ -317,7 +317,8 @@ def rotary(x, positions, freqs, magnitude=1.0, interleaved=False):
     the first 2 R' dims, R' = len(freqs) (float64, radians a position, at most 1024), by theta = position * freqs[j]: (a, b) ->
     magnitude * (a cos - b sin, b cos + a sin). Pairs are dims (j, R' + j), or (2 j, 2 j + 1) if interleaved; the other dims
     are copied. theta in float64 (exact enough while it is below 2^50), the rest in float32, rounded once. A contiguous
-    result; on the GPU x is read where it lies if its last dim is dense and its leading dims can be seen as one."""
+    result; on the GPU x is read where it lies if its last dim is dense and its leading dims can be seen as one, and H D is below
+    2^24."""
     if x.is_cuda:
         return _on_gpu("rotary", x, positions, freqs, magnitude, interleaved)
     _floats("x", x)
@@ -474,7 +475,8 @@ def cache_append(cache, lens, k, v, starts=None, q=None, freqs=None, magnitude=1
     first token of each text, ascending, and behind the last; None: T / B tokens each. Keys are turned to their positions as
     by rotary (freqs None: they are already) and rounded to their type. q [T, H, D]: queries of the same tokens, turned the same
     way and returned (contiguous; rows of no text are zero); None is returned without.
-    Dropped: tokens that no text has or that its capacity has no room for. A page outside the pool is not written."""
+    Dropped: tokens that no text has or that its capacity has no room for. A page outside the pool is not written. On the GPU
+    T + 2 KV (T / G + 2 B) is below 2^24, P G below 2^30, H below 2^16."""
     if k.is_cuda:
         out = _on_gpu("cache_append", k, v, *cache, lens, starts, q, freqs, magnitude, interleaved)
         return None if q is None else out
@@ -548,7 +550,7 @@ def attention_cache(q, cache, lens, scale=None):
     their product with the values, on the host they are not.
     On the GPU q is copied unless its last dim is dense, it starts on 16 bytes and its strides are multiples of 8; the work is
     split for texts as long as the table is wide, so a table that is cut to its longest text (table[:, :pages]) is read
-    best."""
+    best; B N H is below 2^23, H below 2^16, P G below 2^30."""
     if q.is_cuda:
         return _on_gpu("attention_cache", q, *cache, lens, scale)
     b, p, pages, kv, g, d, r = _check_cache("attention_cache", q, cache, lens)
