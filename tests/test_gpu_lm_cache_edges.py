@@ -46,3 +46,7 @@ def test_limits(gpu):
                  lambda: lm.rotary(torch.zeros(1, 1 << 20, 16, dtype=torch.bfloat16, device=gpu), i32(0), f)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_logits_as_they_are(gpu):
+    host.logits_as_they_are(gpu)

@@ -135,3 +135,18 @@ def permuted(dev):
 
 def test_permuted():
     permuted("cpu")
+
+
+def logits_as_they_are(dev):
+    """Nothing to adjust, and permuted logits: a result of its own, contiguous."""
+    for dtype in DTYPES.values():
+        x = torch.randn(4, 40, generator=torch.Generator().manual_seed(1)).to(dtype).to(dev)
+        for logits in (x, x.t().contiguous().t()):
+            for y in (lm.logits_adjust(logits), torch.ops.xdna.logits_adjust(logits)):
+                assert torch.equal(y, x) and y.data_ptr() != logits.data_ptr() and y.is_contiguous()
+            y = torch.ops.xdna.logits_adjust(logits, None, None, None, None, None, torch.ones(40, device=dev))
+            assert y.is_contiguous() and torch.equal(y, (x.float() + 1).to(dtype))
+
+
+def test_logits_as_they_are():
+    logits_as_they_are("cpu")

@@ -275,7 +275,8 @@ def logits_adjust(logits, tokens=None, lens=None, repetition=None, presence=None
         ok = (allowed.unsqueeze(-1) >> torch.arange(32, dtype=torch.int32)) & 1
         x = x.masked_fill(ok.view(b, -1)[:, :v] == 0, -math.inf)
     stats.record("cpu", t0, 0)
-    return x.to(logits.dtype)
+    y = x.to(logits.dtype).contiguous()
+    return y.clone() if y is logits else y
 
 
 # ------------------------------------------------------------------------------ positions
