@@ -512,21 +512,24 @@ struct Rows {
     }
     const float out = k + SHIFT - ko[rb];                                        // from p to the weights
     float m0 = m[rb], shift = out - m0;
-    // A maximum past 2^20 is rounded by a 16th and more, past 2^28 by more than float16's range, and the products that fma takes
-    // are not. There the scores are rounded first, as the maximum was, and the maximum goes off them: the largest is 0.
-    if (__builtin_amdgcn_ballot_w64(fabsf(m0) > 0x1p20f)) {
+    bool far = false;                                                            // too far for the weights to tell p
+    if (__builtin_amdgcn_ballot_w64(fabsf(m0) > 0x1p20f || out < -64.0f)) {
+      // A maximum past 2^20 is rounded by a 16th and more, past 2^28 by more than float16's range, and the products that fma takes
+      // are not. There the scores are rounded first, as the maximum was, and the maximum goes off them: the largest is 0.
+      if (__builtin_amdgcn_ballot_w64(fabsf(m0) > 0x1p20f)) {
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[t][r] = sc[t][r] * c - m0;
-      c = 1.0f, m0 = 0.0f, shift = out;
-    }
-    const bool far = __builtin_amdgcn_ballot_w64(out < -64.0f) != 0;             // too far for the weights to tell p
-    if (far) {
+          for (int r = 0; r < 4; ++r) sc[t][r] = sc[t][r] * c - m0;
+        c = 1.0f, m0 = 0.0f, shift = out;
+      }
+      far = __builtin_amdgcn_ballot_w64(out < -64.0f) != 0;
+      if (far) {
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) l[rb] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -m0));
+          for (int r = 0; r < 4; ++r) l[rb] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], c, -m0));
+      }
     }
     const float scale = far ? 0.0f : __builtin_amdgcn_exp2f(-out);
 #pragma unroll
