@@ -75,6 +75,18 @@ constexpr float P_BIAS = DT == XDNA_F16 ? 14.0f : 0.0f;
 template <int DT>
 constexpr uint32_t EXP_ONES = DT == XDNA_F16 ? 0x7c00u : 0x7f80u;
 
+// A maximum past 2^20 (in powers of two) is a rounded product, by a 16th and more, past 2^26 by more than float16's range of p,
+// and the products that fma takes are not. There the maximum goes off the scores first, and their exponents' unit is the bias.
+template <int DT, int N>
+__device__ __forceinline__ void off_large(f32x16a (&sc)[N], float m, float& mc) {
+  if (!__builtin_amdgcn_ballot_w64(fabsf(mc) > 0x1p20f)) return;
+#pragma unroll
+  for (int b = 0; b < N; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[b][e] -= m == -INFINITY ? 0.0f : m;
+  mc = -P_BIAS<DT>;
+}
+
 // The keys of a workgroup: up to two runs of consecutive keys, one tile after another (no tile holds keys of both).
 struct Keys {
   const char *k, *v;          // first key of the run
@@ -226,7 +238,8 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
   for (int tile = wave; tile < tiles; tile += KW) {
     const int k0 = (tile >= t1 ? tile - t1 : tile) * KT, left = (tile >= t1 ? ks.n2 : ks.n) - k0;
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NI) : "memory");      // K is here, V need not be
-    f32x16a sc = f32x16a{};
+    f32x16a s1[1] = {f32x16a{}};
+    f32x16a& sc = s1[0];
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       sc = mfma32<DT>(*reinterpret_cast<const i32x4*>(kl_ + koff[s]), qf[s], sc);
@@ -252,7 +265,8 @@ __device__ __forceinline__ void attend_split(int8_t* kl_, int8_t* vl_, float* ml
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] *= alpha;
     m = mn;
-    const float mc = (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
+    float mc = (m == -INFINITY ? 0.0f : m * c) - P_BIAS<DT>;     // -inf: only -inf scores so far, p = 0
+    off_large<DT>(s1, m, mc);
     i32x4 pf[2];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
@@ -461,7 +475,8 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
     }
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
-    const float mc = follow(__builtin_elementwise_maximum(max16(sc[0]), max16(sc[1])));
+    float mc = follow(__builtin_elementwise_maximum(max16(sc[0]), max16(sc[1])));
+    off_large<DT>(sc, m, mc);
     weigh(sc[0], mc, pf[0]);
     weigh(sc[1], mc, pf[1]);
     __builtin_amdgcn_sched_barrier(0);
@@ -481,11 +496,13 @@ __device__ __forceinline__ void attend_wide(int8_t* lds0, int8_t* lds1, const Ke
       const int first = first_key(tile) + 32 * b;
       const int8_t* const vb = vt + b * 32 * RB;
       auto visible = [&](int key) { return CAUSAL ? key >= seen.lo && key <= seen.hi : key < ks.n; };
-      f32x16a sc = scores(kt + b * 32 * RB);
+      f32x16a s1[1] = {scores(kt + b * 32 * RB)};
+      f32x16a& sc = s1[0];
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (!visible(first + 8 * (e >> 2) + 4 * half + (e & 3))) sc[e] = -INFINITY;
-      const float mc = follow(max16(sc));
+      float mc = follow(max16(sc));
+      off_large<DT>(s1, m, mc);
       i32x4 pf[2];
       weigh(sc, mc, pf);
       bool odd = false;
