@@ -411,7 +411,8 @@ int xdna_logits_adjust(const void* logits, int dtype, int64_t ld, const void* to
                        void* stream);
 
 /* Heads turned to their positions, y [T, heads, d] (contiguous) of x [T, heads, d] (strides in elements, the last dim dense; dtype
- * F32 / BF16 / F16): pair j < half, theta = positions[t] * freqs[j] (formed in float64, good while it is below 2^50),
+ * F32 / BF16 / F16): pair j < half, theta = positions[t] * freqs[j] (formed in float64, off by up to 2^-52 of itself: good to float32
+ * up to 2^28 radians, of no meaning from 2^50 on),
  *   (a, b) -> magnitude * (a cos theta - b sin theta, b cos theta + a sin theta) of dims j, half + j (interleaved: 2 j, 2 j + 1),
  * in float32, rounded once; dims from 2 half on are copied. positions int32 or int64 (wide = 1); freqs float64 [half], radians a
  * position; half at most 1024. No counterpart in the reference. */
@@ -439,8 +440,8 @@ int xdna_residual_norm(const void* x, int x_dtype, const void* o, int dtype, con
  * k, v [T, nkv, d] (strides: {k token, k head, v token, v head, q token, q head}, elements, the last dim dense) are the tokens
  * starts[b] .. starts[b + 1] - 1 of text b (starts [B + 1] int32, ascending; NULL: T / B each), at positions lens[b] (clamped to 0 ..
  * P G) and on. Keys turn to them as by xdna_rotary (freqs [half]; half 0: as they are) and are rounded to dtype. q [T, nh, d] or
- * NULL: turned the same way into q_out (contiguous); rows of no text are zero. d a multiple of 16, at most 128. lens stays as it
- * is: the caller adds. No counterpart in the reference. */
+ * NULL: turned the same way into q_out (contiguous), to max(lens[b], 0) and on where keys are dropped too; rows of no text are
+ * zero. d a multiple of 16, at most 128. lens stays as it is: the caller adds. No counterpart in the reference. */
 int xdna_cache_append(const void* k, const void* v, int dtype, const int64_t* strides, void* kpages, void* vpages, float* kscales,
                       float* vscales, void* ktail, void* vtail, const int32_t* table, int64_t ldt, const int32_t* lens,
                       const int32_t* starts, const void* q, const double* freqs, int64_t half, float magnitude, int interleaved,
@@ -449,8 +450,8 @@ int xdna_cache_append(const void* k, const void* v, int dtype, const int64_t* st
 
 /* Attention of the newest N tokens of each of B texts over such a cache, which holds them already: out [B, N, nh, d] (contiguous)
  * of q [B, N, nh, d] (strides {text, token, head}, multiples of 8; 16-byte aligned). Token n of text b sees positions 0 ..
- * lens[b] - N + n (lens clamped to 0 .. P G); a page outside 0 .. pages - 1 is seen by no one. Float32 sums; p rounds to dtype
- * for its product with v. Rows that see nothing, or only scores of -inf, are zero. ws: xdna_attention_cache_ws_bytes(..) bytes (0:
+ * lens[b] - N + n (lens clamped to 0 .. P G); a page outside 0 .. pages - 1 is seen by no one. Float32 sums; for their products with v
+ * the pages' weights, p times the values' scale, round to float16, and the open page's p to dtype. Rows that see nothing, or only scores of -inf, are zero. ws: xdna_attention_cache_ws_bytes(..) bytes (0:
  * none needed) that the call may overwrite, 16-byte aligned. No counterpart in the reference. */
 int64_t xdna_attention_cache_ws_bytes(int64_t B, int64_t N, int nh, int nkv, int d, int64_t P, int64_t page);
 int xdna_attention_cache(const void* q, int dtype, const int64_t* strides, const void* kpages, const void* vpages, const float* kscales,

@@ -18,7 +18,11 @@
 //   O^T = V^T P^T: those 16 scores are lane h's values of two 32-deep steps, and 16 bytes of a row of V are the same keys.
 // The products with pages run in float16, which holds int8 exactly and is the cheaper to widen to: bfloat16 rows of q are brought
 // into its range by a power of two. K's scale goes into the exponent's factor, in float32; V's into the weights that P holds,
-// before their rounding to float16. The open page's products run in the tensors' own type.
+// before their rounding to float16. The open page's products run in the tensors' own type, whose range its values need. So weights
+// are held in 16 bits, as the matrix units take them. Against 64 bits the outputs' error grows by that, from plain float32
+// weights': float16 from 0.00021 of their norm to 0.00026 - 0.00029; bfloat16 from 0.00166 to 0.00168 - 0.0018 over pages and to 0.0021
+// for texts that lie in the open page whole. The open page's weights in two halves bring those to 0.00166 and cost 6 to 8% (4 x
+// 330 7.24 us for 6.83, 16 texts of 5 new tokens 25.9 for 23.8), so they are not.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -549,13 +553,15 @@ struct Rows {
 // step is a copy of the loop's body that loads nothing: past a branch around loads the compiler waits for all of them.
 // Heads are held as D dims, a multiple of 32; dims past a.d (D - 16 then) are copies of others (int8, finite; in the open page, where
 // keys may not be, zeros), times zeros of q, and of no output.
-// EXACT: the heads have D dims.
+// EXACT: the heads have D dims, and nothing is asked about a dim. Where rows are few beside the keys it is worth nothing (48 x 8192
+// 115.5 us, without 115.2; 24 x 2000 19.4 / 19.0), for short texts and more rows it is (4 x 330 6.83 / 7.07, 64 x 600 in heads of 64
+// 9.5 / 9.9; 16 x 5 new tokens in heads of 96 24.1 / 25.6; 128 x 2000 of 5 new tokens in heads of 128 72.5 / 81.7, of 64 36.3 / 37.4).
 //
 // What bounds it: one new token a text, the stream of K and V (48 texts of 4096 .. 8192, 604 MB: 115 us, 5.2 TB/s; texts of one
-// length 5.9; a kernel that only reads reaches 6.3), the rest the unequal lengths. More rows, the vector units: a step of 48
-// rows and heads of 96 is about 1000 vector instructions, 240 of them the widening, and 72 MFMAs; 16 texts x 5 tokens x 7 heads
-// a kv head over 2500 .. 5000 keys 18 to 21 us, vector units 48%, waits 45% of the waves' time. Short texts, the chain of lengths,
-// pages, keys, and about 2000 instructions of one wave (4 x 330: 6.8 us).
+// length 5.9; a kernel that only reads reaches 6.3), the rest the unequal lengths. More rows, the vector units and the registers, which
+// leave two waves a SIMD: a step of 48 rows and heads of 96 is about 1000 vector instructions, 240 of them the widening, and 72 MFMAs; 16
+// texts x 5 tokens x 7 heads a kv head over 2500 .. 5000 keys 21.5 us, vector units 48%, waits 45% of the waves' time. Short texts, the
+// chain of lengths, pages, keys, and about 2000 instructions of one wave (4 x 330: 6.8 us).
 template <int DT, int D, int RB, int W, bool EXACT>
 __global__ __launch_bounds__(W * 64, 2) void cache_kernel(CacheArgs a) {
   // a lane's bytes of K: 16 of each 64 dims, and 8 of the last 32
@@ -1039,14 +1045,18 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const float* __restrict
   *reinterpret_cast<uint32_t*>(out + row * d + 2 * lane) = pack16<DT>(x * inv, y * inv);
 }
 
-// How a call is split. A workgroup has up to 48 rows (heads over 96 dims: 32, more do not fit the registers): rows in one
-// workgroup share the widening of K and V. Up to a workgroup a CU, eight waves share out the keys, and a text's keys go to as
-// many parts as fill the CUs, none under 512 keys; with more of them four waves do, two workgroups side by side on a CU, and
-// parts are for balance, none under 2048 keys. A part is its share of the keys that there are; the host knows only how long
-// texts can be. Measured, eight waves / four (texts x longest, 16 / 8 heads of 128): 4 x 330 6.8 / 8.2 us, 20 x 600 9.0 / 9.7, 24 x 2000
-// 19.5 / 19.7, 8 x 32768 80.7 / 83.2, 48 x 1000 22.2 / 19.3, 64 x 600 19.8 / 16.5, 48 x 8192 125 / 116 (one part 133, two
-// 118, four 115.5, five 114); 1 x 131000 on 4 kv heads: 64 parts 16.7, 128 19.5. Keys of a part side by side and not spread over
-// the text: 8 x 32768 80.7 against 84.
+// How a call is split. A workgroup has up to 48 rows, heads over 96 dims 32: rows in one workgroup share the widening of K and V.
+// 48 rows take all 256 registers for heads of 96 already, and a few words of scratch a lane (5 registers, exact dims). Measured
+// there, 48 rows at most / 32: 16 texts of 5 new tokens (35 rows a kv head) over 5000 24.1 / 26.0 us, 128 over 2000 45.4 / 59.5; where
+// fewer rows make more workgroups on a card that has room for them it is the other way: 4 over 3000 14.4 / 11.7, 8 of 64 new
+// tokens over 5000 75.0 / 70.5.
+// Up to a workgroup a CU, eight waves share out the keys, and a text's keys go to as many parts as fill the CUs, at most one for
+// each 512 places of the table; with more of them four waves do, two workgroups side by side on a CU, and parts are for
+// balance, at most one for each 2048 places. A part is its share of the keys that there are, so short texts in a wide table have
+// parts of few keys, or of none: the host knows only how long texts can be. Measured, eight waves / four (texts x longest, 16 / 8
+// heads of 128): 4 x 330 6.8 / 8.3 us, 20 x 600 8.8 / 9.8, 24 x 2000 19.5 / 20.5, 8 x 32768 81 / 84, 48 x 1000 22.6 / 19.6, 64 x 600
+// 20.1 / 16.6, 48 x 8192 124 / 116 (one part 125, two 118, four 116, five 115); 1 x 131000 on 4 kv heads: 64 parts 17.0, 128 21.1. Keys
+// of a part side by side and not spread over the text: 8 x 32768 80.7 against 84.
 struct CachePlan {
   int blocks, rblocks, parts;
   bool eight;

@@ -3,8 +3,10 @@
 // A pair (a, b) of dims at place pos turns by theta = pos f: (a cos - b sin, b cos + a sin). In float32 pos f loses the
 // angle (100000 f is off by 0.004), so the quarter turns pos f 2 / pi are formed in float64: a fused multiply-add with
 // 1.5 * 2^52 rounds them to a whole number, whose low bits name the quadrant, and a second one leaves the rest, exact
-// to 2^-53 of the product, in -1/2 .. 1/2. Its sine and cosine are Taylor's series to r^9 and r^10: the terms left out are below
-// 2^-28. Holds while pos f stays under 2^50; beyond it, and where f is not finite, the result means nothing.
+// but for the rounding of f 2 / pi, in -1/2 .. 1/2. Its sine and cosine are Taylor's series to r^9 and r^10: the terms left out are
+// below 2^-28. f 2 / pi, and 2 / pi itself, are rounded to float64, so the angle is off by up to 2^-52 of itself: below float32's 2^-24 up
+// to 2^28 radians, 2.5e-4 at 2^40. From 2^50 on the quadrant is lost, and there, as where f is not finite, the result means
+// nothing.
 #pragma once
 
 #include "xdna_common.h"

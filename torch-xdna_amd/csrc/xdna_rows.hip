@@ -130,7 +130,8 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 
 // L lanes have a row, C times eight values each in registers between the sums; workgroups of max(L, 256) threads. 8192 rows of 4096,
 // a float32 stream, a bfloat16 block with its norm and a gate a row, 470 MB: 93 us (5.0 TB/s; a large copy 4.8); 4 rows of 1024
-// 3.3 us, the launch and a round trip.
+// 3.3 us, the launch and a round trip. Widths of 513 to 1024 leave half of a row's 256 lanes and more without values: 20000 rows of
+// 768 in bfloat16 2.8 TB/s, of 1024 3.9, where 16384 of 1536 have 5.0 and 60000 of 512 5.2.
 template <int DTX, int DTO, int L, int C>
 __global__ __launch_bounds__(L > 256 ? L : 256) void norm_kernel(NormArgs a) {
   constexpr int THREADS = L > 256 ? L : 256, ROWS = THREADS / L;

@@ -284,7 +284,9 @@ def rotary_freqs(dim, base=10000.0, factor=1.0, original=None, slow=1.0, fast=32
     """(radians a position, float64 [dim / 2], and the magnitude) for heads of which `dim` dims turn: base^(-2 j / dim). Scaled for
     contexts `factor` times as long as the model was made for: all frequencies by 1 / factor if `original` is None; else,
     with `original` positions then, those that turn at least `fast` times over them stay, those that turn at most `slow`
-    times go by 1 / factor, those between by a share of each, and the magnitude is 0.1 ln(factor) + 1."""
+    times go by 1 / factor, those between by a share of each, and the magnitude is 0.1 ln(factor) + 1. The share is linear in the
+    number of turns, as the YaRN paper has it. Programs that make it linear in the index of the dim have other frequencies
+    between the two: a checkpoint of theirs needs those, given as freqs."""
     if dim < 0 or dim % 2 or factor <= 0:
         raise ValueError(f"rotary_freqs takes an even number of dims and a factor above 0, got {dim} and {factor}")
     f = float(base) ** -(torch.arange(0, dim, 2, dtype=torch.float64, device=device) / max(dim, 1))
@@ -317,7 +319,8 @@ def rotary(x, positions, freqs, magnitude=1.0, interleaved=False):
     """Heads x [.., H, D] (float32, bfloat16 or float16) turned to the positions [..] (int32 or int64) of their tokens: pair j of
     the first 2 R' dims, R' = len(freqs) (float64, radians a position, at most 1024), by theta = position * freqs[j]: (a, b) ->
     magnitude * (a cos - b sin, b cos + a sin). Pairs are dims (j, R' + j), or (2 j, 2 j + 1) if interleaved; the other dims
-    are copied. theta in float64 (exact enough while it is below 2^50), the rest in float32, rounded once. A contiguous
+    are copied. theta in float64 (off by up to 2^-52 of itself: good to float32 up to 2^28 radians, on the GPU of no meaning from
+    2^50 on), the rest in float32, rounded once. A contiguous
     result; on the GPU x is read where it lies if its last dim is dense and its leading dims can be seen as one, and H D is below
     2^24."""
     if x.is_cuda:
@@ -475,7 +478,8 @@ def cache_append(cache, lens, k, v, starts=None, q=None, freqs=None, magnitude=1
     positions lens[b] (int32 [B]; clamped to 0 .. P G) and on of their texts; lens stays as it is. starts int32 [B + 1]: the
     first token of each text, ascending, and behind the last; None: T / B tokens each. Keys are turned to their positions as
     by rotary (freqs None: they are already) and rounded to their type. q [T, H, D]: queries of the same tokens, turned the same
-    way and returned (contiguous; rows of no text are zero); None is returned without.
+    way (to max(lens[b], 0) and on, also where keys are dropped) and returned (contiguous; rows of no text are zero); None is
+    returned without.
     Dropped: tokens that no text has or that its capacity has no room for. A page outside the pool is not written. On the GPU
     T + 2 KV (T / G + 2 B) is below 2^24, P G below 2^30, H below 2^16."""
     if k.is_cuda:
@@ -547,8 +551,8 @@ def attention_cache(q, cache, lens, scale=None):
     sees its positions 0 .. lens[b] - N + n (lens int32 [B], clamped to 0 .. P G, the new tokens counted): a text with fewer new
     ones has them last, and rows before the first position are zero. Full pages are read in 8 bits, the open one from the
     16-bit places; a page that is none of the pool is seen by no one. scale: 1 / sqrt(D) if None. Float32 sums, the
-    result rounded once; on the GPU the softmax's weights, times the values' scale, are rounded to q's dtype for
-    their product with the values, on the host they are not.
+    result rounded once; on the GPU the softmax's weights are rounded for their product with the values, a page's, times the
+    values' scale, to float16, the open page's to q's dtype, on the host they are not.
     On the GPU q is copied unless its last dim is dense, it starts on 16 bytes and its strides are multiples of 8; the work is
     split for texts as long as the table is wide, so a table that is cut to its longest text (table[:, :pages]) is read
     best; B N H is below 2^23, H below 2^16, P G below 2^30."""
