@@ -145,3 +145,37 @@ def test_captured_step(gpu):
             assert eager.held == replayed.held == eager.lens.tolist() == replayed.lens.tolist()
         with pytest.raises(ValueError):
             replayed.grow([80 - replayed.held[0] + 1, 0])
+
+
+def _drafts_taken_back(dev, page):
+    """Steps of drafts of which some are not taken: the program sets lens back, and only what is held counts against the capacity.
+    The tokens that were taken have the logits that they have one by one; a row set to 0 takes a new prompt."""
+    model, prompt = S.Server(**SIZES).to(dev), _prompt(page + 3, dev)
+    plain, drafts = (S.Texts(model, 1, 3 * page, page, device=dev) for _ in range(2))
+    with torch.no_grad():
+        for texts in (plain, drafts):
+            model.start(texts, prompt, _i32([0, page + 3], dev))
+        for i in range(2 * page - 7):
+            want = model.step(plain, _i32([[i]], dev))[0, 0]
+            got = model.step(drafts, _i32([[i, 250, 251, 252, 253]], dev))[0, 0]
+            drafts.lens -= 4
+            assert (got.float() - want.float()).norm() < 0.03 * want.float().norm(), i
+        assert drafts.lens.tolist() == plain.lens.tolist() == [3 * page - 4]
+        with pytest.raises(ValueError):
+            model.step(drafts, _i32([[1, 2, 3, 4, 5]], dev))
+        model.step(drafts, _i32([[1, 2, 3, 4]], dev))
+        with pytest.raises(ValueError):
+            model.start(drafts, prompt, _i32([0, page + 3], dev))
+        drafts.lens.zero_()
+        model.start(drafts, prompt, _i32([0, page + 3], dev))
+        assert drafts.lens.tolist() == [page + 3] == drafts.held
+
+
+def test_drafts_taken_back():
+    _drafts_taken_back("cpu", 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_drafts_taken_back_gpu(gpu, page):
+    _drafts_taken_back(gpu, page)

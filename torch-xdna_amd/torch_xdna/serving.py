@@ -23,7 +23,8 @@ class Texts:
     """The caches of `batch` texts in all layers: a Cache8 a layer over one table, and the texts' lengths. A row of the batch has a
     text from the time that it has pages until they are given back; the tokens that a step has for the other rows go nowhere, and
     its logits for those mean nothing. What a text holds is counted on the host too, so that nothing grows past its pages: a program
-    that replays a captured step gives the pages out before (reserve), and counts each replay but the first (grow)."""
+    that replays a captured step gives the pages out before (reserve), and counts each replay but the first (grow). A program may
+    set lens back (drafts that were not taken): the host's count, too high then, is read from it again before anything is refused."""
 
     def __init__(self, model, batch, capacity, page=64, pages=None, device=None):
         layer = model.layers[0]
@@ -56,11 +57,15 @@ class Texts:
     def grow(self, new):
         """Counts new[i] more tokens of each text i, and gives out the pages that they need; without room for all, it raises and
         nothing changes."""
-        held = [h + n for h, n in zip(self.held, new)]
-        missing = sum(max(0, -(-h // self.page) - len(g)) for h, n, g in zip(held, new, self.given) if n)
-        if max(held, default=0) > self.columns * self.page or missing > len(self.free):
-            raise ValueError(f"no room for texts of {held} tokens: {missing} pages are missing and {len(self.free)} free, of "
-                             f"{self.columns} a text")
+        for again in (False, True):
+            held = [h + n for h, n in zip(self.held, new)]
+            missing = sum(max(0, -(-h // self.page) - len(g)) for h, n, g in zip(held, new, self.given) if n)
+            if max(held, default=0) <= self.columns * self.page and missing <= len(self.free):
+                break
+            if again:
+                raise ValueError(f"no room for texts of {held} tokens: {missing} pages are missing and {len(self.free)} free, of "
+                                 f"{self.columns} a text")
+            self.held = self.lens.tolist()
         for text, n in enumerate(new):
             if n:
                 self.reserve(text, held[text])
@@ -101,7 +106,9 @@ class Server(Decoder):
         if len(new) != len(texts.held) or min(new, default=0) < 0 or first[0] < 0 or first[-1] > tokens.shape[0]:
             raise ValueError(f"starts must be [{len(texts.held) + 1}], ascending, within the {tokens.shape[0]} tokens")
         if any(n and h for n, h in zip(new, texts.held)):
-            raise ValueError("a prompt is for a text that holds nothing: release it first")
+            texts.held = texts.lens.tolist()
+            if any(n and h for n, h in zip(new, texts.held)):
+                raise ValueError("a prompt is for a text that holds nothing: release it first")
         texts.grow(new)
         at = torch.arange(tokens.shape[0], device=tokens.device)
         place = at - starts.long()[torch.searchsorted(starts.long(), at, right=True) - 1]
